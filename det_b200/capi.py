@@ -127,7 +127,42 @@ class FMoeOp(C.Structure):
                 ("counts", c_void_p), ("scratch", c_void_p)]
 
 
+class TreeRef(C.Structure):
+    """det_tree_ref (include/det_b200.h): the rows of a step of drafted tokens."""
+    _fields_ = [("table", c_void_p), ("first", c_void_p), ("len", c_void_p), ("seqs", c_int), ("rows", c_int),
+                ("max_nodes", c_int), ("max_len", c_int)]
+
+
+class FRopeOp(C.Structure):
+    _fields_ = [("dims", c_int), ("scaling", c_int), ("base", C.c_double), ("factor", C.c_double), ("orig_ctx", C.c_double),
+                ("low", C.c_double), ("high", C.c_double), ("mscale", c_float), ("pos0", c_int), ("n", c_int),
+                ("cos", c_void_p), ("sin", c_void_p)]
+
+
+class FQkOp(C.Structure):
+    _fields_ = [(n, c_int) for n in ("heads", "kv_heads", "dim", "vdim", "rot_dims", "half")] + [
+                ("eps", c_float), ("q_norm", c_void_p), ("k_norm", c_void_p), ("cap", c_int), ("dtype", c_int),
+                ("y", c_void_p), ("ldy", c_int), ("q_off", c_int), ("k_off", c_int), ("v_off", c_int), ("rope_len", c_int),
+                ("rope_cos", c_void_p), ("rope_sin", c_void_p), ("vrope_cos", c_void_p), ("vrope_sin", c_void_p),
+                ("pos", c_void_p), ("q", c_void_p), ("seq", TreeRef)]
+
+
+class FTreeOp(C.Structure):
+    _fields_ = [(n, c_int) for n in ("heads", "kv_heads", "dim", "vdim")] + [
+                ("scale", c_float), ("cap", c_int), ("dtype", c_int), ("q", c_void_p), ("mask", c_void_p), ("mask_ld", c_int),
+                ("gate", c_void_p), ("ldg", c_int), ("pos", c_void_p), ("rope_len", c_int), ("vrope_cos", c_void_p),
+                ("vrope_sin", c_void_p), ("out", c_void_p), ("ldo", c_int), ("scratch", c_void_p), ("seq", TreeRef)]
+
+
+class FKeepOp(C.Structure):
+    _fields_ = [("caches", c_int), ("seqs", c_int), ("cap", c_int), ("row_bytes", c_int), ("table", c_void_p),
+                ("len", c_void_p), ("keep", c_void_p), ("keep_ld", c_int), ("count", c_void_p), ("max_count", c_int),
+                ("len_out", c_void_p)]
+
+
 DET_F32, DET_BF16 = 0, 1
+DET_ROPE_PLAIN, DET_ROPE_LINEAR, DET_ROPE_BASE, DET_ROPE_RAMP = 0, 1, 2, 3
+DET_MAX_TREE = 1024
 DET_FF_SWIGLU, DET_FF_REGLU, DET_FF_RELU2 = 0, 1, 2
 DET_MAX_ROUTER = 1024
 DET_DECAY_SIGMOID, DET_DECAY_EXP = 0, 1
@@ -233,6 +268,11 @@ CUDA_ABI = {
     "det_f_mingru": (None, [C.POINTER(FMinGruOp), c_void_p]),
     "det_f_moe_scratch_bytes": (c_size_t, [c_int] * 6),
     "det_f_moe": (None, [C.POINTER(FMoeOp), c_void_p]),
+    "det_f_rope_table": (c_int, [C.POINTER(FRopeOp), c_void_p]),
+    "det_f_qk_rope": (c_int, [C.POINTER(FQkOp), c_void_p]),
+    "det_f_tree_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "det_f_tree_attn": (c_int, [C.POINTER(FTreeOp), c_void_p]),
+    "det_f_tree_keep": (c_int, [C.POINTER(FKeepOp), c_void_p]),
     "det_debug_set_float": (None, [c_int]),
     "det_attn_set_workspace": (None, [c_void_p, c_size_t]),
     "det_debug_set_attn_tc": (None, [c_int, c_int]),

@@ -1,0 +1,320 @@
+// Attention of a step of drafted tokens (include/det_b200.h, det_ftree_op): one pass over the keys with the running maximum and sum of
+// the softmax, in 32-bit.  ftree.cuh says how the work is dealt out.
+//
+//   k_ftree_simt   32-bit products on the CUDA cores: 256 threads over a tile of query rows x 64 keys, keys and values staged in
+//                  shared memory as fp32.
+//   k_ftree_merge  adds the pieces of the segments that several CTAs shared.
+#include "ftree.cuh"
+#include <algorithm>
+#include <cmath>
+
+namespace detb {
+
+constexpr int TS_KEYS = 64, TS_THREADS = 256;
+
+static size_t simt_smem(int block, int kd, int vd) {
+    return ((size_t)(block + TS_KEYS) * (kd + 4) + (size_t)TS_KEYS * (vd + 4) + (size_t)block * (TS_KEYS + 4)) * sizeof(float);
+}
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const bf16* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_float4(bf_lo(v.x), bf_hi(v.x), bf_lo(v.y), bf_hi(v.y));
+}
+__device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
+    return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s))));
+}
+// maximum and sum over the 16 lanes that share a row
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, off));
+    return v;
+}
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) v += __shfl_xor_sync(FULL, v, off);
+    return v;
+}
+
+// Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.
+template <class T, int TR, int VJ>
+__global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
+    extern __shared__ __align__(16) float tsm[];
+    __shared__ TreeShare share;
+    constexpr int RB = 16 * TR;
+    const int ldk = a.kd + 4, ldv = a.vd + 4, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    float* Q = tsm;                              // [RB][ldk]
+    float* K = Q + RB * ldk;                     // [64][ldk]
+    float* V = K + TS_KEYS * ldk;                // [64][ldv]
+    float* P = V + TS_KEYS * ldv;                // [RB][68]
+    constexpr int LDP = TS_KEYS + 4;
+    pdl_trigger();
+    pdl_wait();
+    if (tid < 32) {
+        const TreeShare w = tree_start(a, blockIdx.x, tid);
+        if (tid == 0) share = w;
+    }
+    __syncthreads();
+    TreeWalk walk{share, false};
+    TreeItem it;
+    while (tree_next(a, walk, it)) {
+        const TreeSeg& s = it.s;
+        const T* cache = static_cast<const T*>(a.seq.table[s.b].cache);
+        const T* q = static_cast<const T*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
+        __syncthreads();
+        for (int i = tid; i < RB * (a.kd / 4); i += TS_THREADS) {
+            const int r = i / (a.kd / 4), e = (i - r * (a.kd / 4)) * 4, row = s.r0 + r;
+            float4 v = make_float4(0, 0, 0, 0);
+            if (r < s.rows) v = load4(q + (size_t)(row / a.per_kv) * a.ldq + (row % a.per_kv) * a.kd + e);
+            *reinterpret_cast<float4*>(Q + r * ldk + e) = v;
+        }
+        float m[TR], l[TR];
+        float4 o[TR][VJ];
+#pragma unroll
+        for (int i = 0; i < TR; i++) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < VJ; j++) o[i][j] = make_float4(0, 0, 0, 0);
+        }
+        for (int t = it.tile; t < it.tile + it.n; t++) {
+            const int k0 = t * TS_KEYS, last = s.len + s.n;
+            const bool tree = k0 + TS_KEYS > s.len;
+            __syncthreads();
+            const T* kp = cache + (size_t)k0 * a.ld + it.g * a.kd;
+            for (int i = tid; i < TS_KEYS * (a.kd / 4); i += TS_THREADS) {
+                const int k = i / (a.kd / 4), e = (i - k * (a.kd / 4)) * 4;
+                *reinterpret_cast<float4*>(K + k * ldk + e) = k0 + k < last ? load4(kp + (size_t)k * a.ld + e) : make_float4(0, 0, 0, 0);
+            }
+            const T* vp = cache + (size_t)k0 * a.ld + a.kv_heads * a.kd + it.g * a.vd;
+            for (int i = tid; i < TS_KEYS * (a.vd / 4); i += TS_THREADS) {
+                const int k = i / (a.vd / 4), e = (i - k * (a.vd / 4)) * 4;
+                *reinterpret_cast<float4*>(V + k * ldv + e) = k0 + k < last ? load4(vp + (size_t)k * a.ld + e) : make_float4(0, 0, 0, 0);
+            }
+            __syncthreads();
+            float sc[TR][4];
+#pragma unroll
+            for (int i = 0; i < TR; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) sc[i][j] = 0.0f;
+            for (int e = 0; e < a.kd; e += 4) {
+                float4 kv[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) kv[j] = load4(K + (tx + 16 * j) * ldk + e);
+#pragma unroll
+                for (int i = 0; i < TR; i++) {
+                    const float4 qv = load4(Q + (ty + 16 * i) * ldk + e);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sc[i][j] = dot4(qv, kv[j], sc[i][j]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < TR; i++) {
+                const int r = ty + 16 * i;
+                unsigned seen[2] = {FULL, FULL};
+                if (tree) {
+                    const int node = (s.r0 + min(r, s.rows - 1)) / a.per_kv;
+                    seen[0] = tree_seen(a, s, node, k0);
+                    seen[1] = tree_seen(a, s, node, k0 + 32);
+                }
+                float mx = m[i];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    sc[i][j] = (seen[j >> 1] >> (tx + 16 * (j & 1))) & 1u ? sc[i][j] * a.scale2 : -INFINITY;
+                    mx = fmaxf(mx, sc[i][j]);
+                }
+                mx = row_max(mx);
+                const float base = mx == -INFINITY ? 0.0f : mx, f = exp2f(m[i] - base);
+                m[i] = mx;
+                l[i] *= f;
+#pragma unroll
+                for (int j = 0; j < VJ; j++) {
+                    o[i][j].x *= f;
+                    o[i][j].y *= f;
+                    o[i][j].z *= f;
+                    o[i][j].w *= f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float p = exp2f(sc[i][j] - base);
+                    l[i] += p;
+                    P[r * LDP + tx + 16 * j] = p;
+                }
+            }
+            __syncthreads();
+            for (int k = 0; k < TS_KEYS; k++) {
+                float4 v[VJ];
+#pragma unroll
+                for (int j = 0; j < VJ; j++) {
+                    const int c = 4 * tx + 64 * j;
+                    v[j] = c < a.vd ? load4(V + k * ldv + c) : make_float4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < TR; i++) {
+                    const float p = P[(ty + 16 * i) * LDP + k];
+                    if (tree && p == 0.0f) continue;          // a masked node's value may be anything
+#pragma unroll
+                    for (int j = 0; j < VJ; j++) {
+                        o[i][j].x = fmaf(p, v[j].x, o[i][j].x);
+                        o[i][j].y = fmaf(p, v[j].y, o[i][j].y);
+                        o[i][j].z = fmaf(p, v[j].z, o[i][j].z);
+                        o[i][j].w = fmaf(p, v[j].w, o[i][j].w);
+                    }
+                }
+            }
+        }
+        float* piece = a.part + ((size_t)blockIdx.x * 2 + it.piece) * tree_piece_floats(RB, a.vd);
+#pragma unroll
+        for (int i = 0; i < TR; i++) {
+            const int r = ty + 16 * i, row = s.r0 + r;
+            const float sum = row_sum(l[i]);
+            if (r >= s.rows) continue;
+            if (!it.whole && tx == 0) {
+                piece[r] = m[i];
+                piece[RB + r] = sum;
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // no key seen
+#pragma unroll
+            for (int j = 0; j < VJ; j++) {
+                const int c = 4 * tx + 64 * j;
+                if (c >= a.vd) continue;
+                if (it.whole) {
+                    tree_put<T>(a, s.first + row / a.per_kv, it.g * a.per_kv + row % a.per_kv, c,
+                                make_float4(o[i][j].x * inv, o[i][j].y * inv, o[i][j].z * inv, o[i][j].w * inv));
+                } else {
+                    put4(piece + 2 * RB + ((size_t)(c / 4) * RB + r) * 4, o[i][j]);
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ pieces
+constexpr int TM_THREADS = 256;
+// grid (key/value heads x pieces of a block's (row, four values) pairs, segments)
+template <class T>
+__global__ void __launch_bounds__(TM_THREADS) k_ftree_merge(const TreeArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, g = blockIdx.x % a.kv_heads, chunk = blockIdx.x / a.kv_heads, chunks = gridDim.x / a.kv_heads;
+    const TreeSeg s = tree_seg(a, blockIdx.y);
+    if (s.tiles <= 1) return;
+    long long before = 0, total = 0;
+    for (int i = lane; i < a.seq.seqs * a.blocks; i += 32) {
+        const int t = tree_seg(a, i).tiles;
+        total += t;
+        if (i < (int)blockIdx.y) before += t;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        total += __shfl_xor_sync(FULL, total, off);
+        before += __shfl_xor_sync(FULL, before, off);
+    }
+    total *= a.kv_heads;
+    const int ctas = tree_ctas(a, total);
+    const long long u0 = before * a.kv_heads + (long long)g * s.tiles, u1 = u0 + s.tiles - 1;
+    int c0 = (int)(u0 * ctas / total), c1 = (int)(u1 * ctas / total);
+    while (c0 + 1 < ctas && tree_bound(total, ctas, c0 + 1) <= u0) c0++;
+    while (c0 > 0 && tree_bound(total, ctas, c0) > u0) c0--;
+    while (c1 + 1 < ctas && tree_bound(total, ctas, c1 + 1) <= u1) c1++;
+    while (c1 > 0 && tree_bound(total, ctas, c1) > u1) c1--;
+    if (c0 == c1) return;
+    const size_t size = tree_piece_floats(a.block, a.vd);
+    const float* head = a.part + ((size_t)c0 * 2 + (tree_bound(total, ctas, c0) == u0 ? 0 : 1)) * size;   // the others are their CTAs' first
+    const int vq = a.vd / 4;
+    for (int i = chunk * TM_THREADS + threadIdx.x; i < s.rows * vq; i += chunks * TM_THREADS) {
+        const int v = i / s.rows, r = i - v * s.rows;
+        float m = head[r];
+        for (int c = c0 + 1; c <= c1; c++) m = fmaxf(m, a.part[(size_t)c * 2 * size + r]);
+        const float base = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f;
+        float4 o = make_float4(0, 0, 0, 0);
+        for (int c = c0; c <= c1; c++) {
+            const float* p = c == c0 ? head : a.part + (size_t)c * 2 * size;
+            const float f = exp2f(p[r] - base);
+            const float4 x = load4(p + 2 * a.block + ((size_t)v * a.block + r) * 4);
+            l = fmaf(f, p[a.block + r], l);
+            o.x = fmaf(f, x.x, o.x);
+            o.y = fmaf(f, x.y, o.y);
+            o.z = fmaf(f, x.z, o.z);
+            o.w = fmaf(f, x.w, o.w);
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int row = s.r0 + r;
+        tree_put<T>(a, s.first + row / a.per_kv, g * a.per_kv + row % a.per_kv, v * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ host side
+template <class T, int TR, int VJ>
+static cudaError_t launch_simt(const TreeArgs& a, cudaStream_t q) {
+    const size_t smem = simt_smem(a.block, a.kd, a.vd);
+    const cudaError_t e = cudaFuncSetAttribute(k_ftree_simt<T, TR, VJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl_try(k_ftree_simt<T, TR, VJ>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a);
+}
+template <class T, int TR>
+static cudaError_t launch_simt_v(const TreeArgs& a, cudaStream_t q) {
+    return a.vd <= 64 ? launch_simt<T, TR, 1>(a, q) : a.vd <= 128 ? launch_simt<T, TR, 2>(a, q) : launch_simt<T, TR, 4>(a, q);
+}
+template <class T>
+static cudaError_t launch_all(const TreeArgs& a, cudaStream_t q) {
+    cudaError_t e = a.block == 16 ? launch_simt_v<T, 1>(a, q) : launch_simt_v<T, 4>(a, q);
+    if (e != cudaSuccess) return e;
+    const int chunks = std::max(1, std::min(16, a.block * (a.vd / 4) / TM_THREADS));
+    return launch_pdl_try(k_ftree_merge<T>, dim3(a.kv_heads * chunks, a.seq.seqs * a.blocks), dim3(TM_THREADS), 0, q, 1, a);
+}
+// Rows of a block: as many as fill the tile, 64 at most.
+static int rows_of_block(int rows) { return rows <= 16 ? 16 : 64; }
+
+}  // namespace detb
+
+using namespace detb;
+
+extern "C" {
+
+size_t det_f_tree_scratch_bytes(int heads, int kv_heads, int vdim, int max_nodes) {
+    if (heads <= 0 || kv_heads <= 0 || vdim <= 0 || max_nodes <= 0) return 16;
+    const long long rows = (long long)max_nodes * (heads / kv_heads);
+    const int block = rows_of_block((int)std::min<long long>(rows, 1 << 20));
+    return TREE_CTAS * 2 * tree_piece_floats(block, round8(vdim)) * sizeof(float);
+}
+
+int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
+    const char* name = "det_f_tree_attn";
+    DETB_TAKE(op != nullptr, "no descriptor");
+    DETB_TAKE(op->heads > 0 && op->kv_heads > 0 && op->heads <= 4096 && op->heads % op->kv_heads == 0 && op->dim > 0 && op->vdim > 0 && op->cap > 0,
+              "bad sizes");
+    DETB_TAKE(op->dim <= 256 && op->vdim <= 256, "the head is too large");
+    DETB_TAKE(op->dtype == DET_F32 || op->dtype == DET_BF16, "unknown activation type");
+    DETB_TAKE(std::isfinite(op->scale) && op->scale > 0.0f, "bad scale");
+    DETB_TAKE(!op->vrope_cos == !op->vrope_sin && (!op->vrope_cos || (op->vdim % 2 == 0 && op->pos && op->rope_len > 0)), "bad rotation of the values");
+    if (const char* why = bad_ref(op->seq)) return refuse(name, why);
+    const long long rows = (long long)op->seq.max_nodes * (op->heads / op->kv_heads);
+    DETB_TAKE(rows <= 1 << 24, "too many rows");
+    DETB_TAKE(!op->mask || (op->seq.max_nodes <= DET_MAX_TREE && op->mask_ld * 32ll >= op->seq.max_nodes), "the mask is too small");
+    DETB_TAKE(op->ldo >= op->heads * op->vdim && (!op->gate || op->ldg >= op->heads), "rows overlap");
+    if (op->seq.rows == 0 || op->seq.seqs == 0 || rows == 0) return 0;
+    DETB_TAKE(op->q && op->out && op->scratch && aligned16(op->q) && aligned16(op->scratch), "q, out or scratch is NULL or misaligned");
+    TreeArgs a{};
+    a.block = rows_of_block((int)rows);
+    a.tile = TS_KEYS;
+    const long long blocks = (rows + a.block - 1) / a.block;
+    DETB_TAKE(blocks * op->seq.seqs <= 65535, "too many rows");
+    DETB_TAKE(runtime_ready(), "no usable device");
+    a.heads = op->heads; a.kv_heads = op->kv_heads; a.per_kv = op->heads / op->kv_heads; a.dim = op->dim; a.vdim = op->vdim;
+    a.kd = round8(op->dim); a.vd = round8(op->vdim);
+    a.ld = det_f_attn_ld(op->kv_heads, op->dim, op->vdim);
+    a.ldq = det_f_attn_q_ld(op->heads, op->dim);
+    a.scale2 = op->scale * 1.4426950408889634f;
+    a.cap = op->cap; a.q = op->q; a.mask = op->mask; a.mask_ld = op->mask_ld; a.gate = op->gate; a.ldg = op->ldg; a.pos = op->pos;
+    a.rope_len = op->rope_len; a.vcs = op->vrope_cos; a.vsn = op->vrope_sin; a.out = op->out; a.ldo = op->ldo;
+    a.part = static_cast<float*>(op->scratch);
+    a.error_flag = error_word();
+    a.blocks = (int)blocks;
+    a.seq = op->seq;
+    a.ctas = std::min(TREE_CTAS, sm_count());
+    cudaStream_t q = queue_of(st);
+    return launched(name, op->dtype == DET_BF16 ? launch_all<bf16>(a, q) : launch_all<float>(a, q));
+}
+
+}  // extern "C"

@@ -1,0 +1,240 @@
+// Pieces shared by the ops of a step of drafted tokens (include/det_b200.h, det_tree_ref): refusals, which sequence a row belongs to,
+// and how the attention's work is dealt out.
+#pragma once
+#include "fops.cuh"
+
+namespace detb {
+
+inline int refuse(const char* op, const char* why) {
+    fprintf(stderr, "det_b200: %s refused: %s\n", op, why);
+    return 1;
+}
+#define DETB_TAKE(cond, why)                   \
+    do {                                       \
+        if (!(cond)) return refuse(name, why); \
+    } while (0)
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// The verdict of a launch as a return code.
+inline int launched(const char* name, cudaError_t e) {
+    if (e == cudaSuccess) return 0;
+    (void)cudaGetLastError();
+    return refuse(name, cudaGetErrorString(e));
+}
+inline const char* bad_ref(const det_tree_ref& s) {
+    if (s.seqs < 0 || s.rows < 0 || s.max_len < 0 || s.max_nodes < 0) return "negative sizes";
+    if (s.seqs > 65535) return "too many sequences";
+    if (s.seqs && s.rows && (!s.table || !s.first || !s.len)) return "table, first or len is NULL";
+    return nullptr;
+}
+
+__device__ __forceinline__ void report_size(int* error_flag) { atomicExch(error_flag, DETB_ERR_SIZE); }
+
+__device__ __forceinline__ void put4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void put4(bf16* p, float4 v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf(v.x, v.y), pack_bf(v.z, v.w)); }
+
+// A cache pointer from device memory.
+__device__ __forceinline__ bool usable_cache(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The place of a row: sequence, node of its tree, row of its cache.  b < 0: nobody's row.  Called by whole warps with one row.
+struct TreePlace {
+    int b, node, slot;
+};
+__device__ __forceinline__ TreePlace tree_place(const det_tree_ref& s, int row, int lane) {
+    int b = 0;
+    for (int i = lane; i - lane < s.seqs; i += 32) b += __popc(__ballot_sync(FULL, i < s.seqs && s.first[i + 1] <= row));
+    if (b >= s.seqs) return {-1, 0, 0};
+    const int node = row - s.first[b];
+    return {b, node, s.len[b] + node};
+}
+
+// ------------------------------------------------------------------------------------------------------ attention
+// The query rows of a sequence and key/value head are (node, query head of the group) pairs, node first, in blocks of `block` rows;
+// its keys come in tiles.  The tiles of all (sequence, row block, key/value head) segments, in that order, are dealt out evenly: CTA
+// c takes the tiles bound(c) .. bound(c + 1), whatever segments they belong to, so unequal lengths leave no CTA idle.  A segment that
+// falls to one CTA is finished there; of the others every CTA leaves a piece (maximum, sum, values per row) in scratch, and the
+// merge kernel adds the pieces in order of the keys.  A CTA has at most two such pieces, of its first and of its last segment.
+constexpr int TREE_CTAS = 148;
+constexpr int TREE_SHARE = 2;      // tiles of a CTA, if there are enough
+
+struct TreeArgs {
+    int heads, kv_heads, per_kv, dim, vdim, kd, vd, ld, ldq;
+    float scale2;                  // scale * log2(e)
+    int cap;
+    const void* q;
+    const unsigned* mask;
+    int mask_ld;
+    const float* gate;
+    int ldg;
+    const int* pos;
+    int rope_len;
+    const float* vcs;
+    const float* vsn;
+    void* out;
+    int ldo;
+    float* part;                   // [CTA][2] pieces of tree_piece_floats(block, vd)
+    int* error_flag;
+    int block, tile, blocks;       // rows of a block, keys of a tile, row blocks of the largest tree
+    int ctas;
+    det_tree_ref seq;
+};
+// A piece: m[block] | l[block] | o[vd / 4][block][4].
+__host__ __device__ constexpr size_t tree_piece_floats(int block, int vd) { return (size_t)block * (2 + vd); }
+
+struct TreeSeg {
+    int b, r0, rows;               // sequence, first row of the block, its rows
+    int first, n, len, keys;       // first row of the step, nodes, cached rows, keys that some row of the block may see
+    int tiles;                     // 0: nothing to do (a sequence that does not fit is left out)
+    bool bad;
+};
+__device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, int seg) {
+    TreeSeg s;
+    s.b = seg / a.blocks;
+    s.r0 = (seg - s.b * a.blocks) * a.block;
+    s.first = a.seq.first[s.b];
+    s.n = a.seq.first[s.b + 1] - s.first;
+    s.len = a.seq.len[s.b];
+    s.bad = s.first < 0 || s.n < 0 || s.n > a.seq.max_nodes || s.first > a.seq.rows - s.n || s.len < 0 || s.n > a.cap || s.len > a.cap - s.n ||
+            !usable_cache(a.seq.table[s.b].cache);
+    if (s.bad) s.n = 0;
+    s.rows = min(a.block, s.n * a.per_kv - s.r0);
+    const int seen = a.mask ? s.n : min(s.n, (s.r0 + s.rows + a.per_kv - 1) / a.per_kv);
+    s.keys = s.len + seen;
+    s.tiles = s.rows > 0 ? (s.keys + a.tile - 1) / a.tile : 0;
+    return s;
+}
+// Where a CTA's share begins and how long it is.  tree_start is called by a whole warp; every lane gets the result.
+struct TreeShare {
+    int seg, g, tile;              // segment, key/value head, tile within them
+    long long left;                // tiles of the share
+};
+__device__ __forceinline__ int tree_ctas(const TreeArgs& a, long long total) {
+    return (int)max(1ll, min((long long)a.ctas, total / TREE_SHARE));
+}
+__device__ __forceinline__ long long tree_bound(long long total, int ctas, int c) { return c >= ctas ? total : total * c / ctas; }
+__device__ __forceinline__ long long tree_total(const TreeArgs& a, int lane, bool report) {
+    long long t = 0;
+    bool bad = false;
+    for (int i = lane; i < a.seq.seqs * a.blocks; i += 32) {
+        const TreeSeg s = tree_seg(a, i);
+        t += s.tiles;
+        bad |= s.bad;
+    }
+    if (report && bad) report_size(a.error_flag);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) t += __shfl_xor_sync(FULL, t, off);
+    return t * a.kv_heads;
+}
+__device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int lane) {
+    const long long total = tree_total(a, lane, cta == 0);
+    const int ctas = tree_ctas(a, total);
+    TreeShare w{0, 0, 0, 0};
+    if (cta >= ctas || total == 0) return w;
+    const long long u0 = tree_bound(total, ctas, cta);
+    w.left = tree_bound(total, ctas, cta + 1) - u0;
+    long long base = 0;                                       // tiles ahead of this round's segments
+    for (int i = lane;; i += 32) {
+        const int tiles = i < a.seq.seqs * a.blocks ? tree_seg(a, i).tiles : 0;
+        long long sum = (long long)tiles * a.kv_heads;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long v = __shfl_up_sync(FULL, sum, off);
+            if (lane >= off) sum += v;
+        }
+        const unsigned holds = __ballot_sync(FULL, base + sum > u0);
+        if (holds) {
+            const int src = __ffs(holds) - 1;
+            const long long before = __shfl_sync(FULL, base + sum - (long long)tiles * a.kv_heads, src);
+            const int per = __shfl_sync(FULL, tiles, src);
+            w.seg = i - lane + src;
+            w.g = (int)((u0 - before) / per);
+            w.tile = (int)((u0 - before) % per);
+            return w;
+        }
+        base += __shfl_sync(FULL, sum, 31);
+    }
+}
+// The next stretch of a share: `n` tiles from `tile` on of key/value head g of the segment; false when the share is done.
+struct TreeItem {
+    TreeSeg s;
+    int g, tile, n;
+    bool whole;                    // all tiles of the segment and head
+    int piece;                     // else: which of the CTA's pieces
+};
+struct TreeWalk {
+    TreeShare w;
+    bool begun;
+};
+__device__ __forceinline__ bool tree_next(const TreeArgs& a, TreeWalk& k, TreeItem& it) {
+    if (k.w.left <= 0) return false;
+    it.s = tree_seg(a, k.w.seg);
+    while (it.s.tiles == 0) {                                  // only segments behind the first can be empty
+        k.w.seg++;
+        it.s = tree_seg(a, k.w.seg);
+    }
+    it.g = k.w.g;
+    it.tile = k.w.tile;
+    it.n = (int)min((long long)(it.s.tiles - it.tile), k.w.left);
+    it.whole = it.n == it.s.tiles;
+    it.piece = k.begun ? 1 : 0;
+    k.begun = true;
+    k.w.left -= it.n;
+    k.w.tile = 0;
+    if (++k.w.g == a.kv_heads) {
+        k.w.g = 0;
+        k.w.seg++;
+    }
+    return true;
+}
+// The 32 keys from c0 on that row r of the block sees, as bits; keys from the end of the tree on are never seen.
+__device__ __forceinline__ unsigned tree_seen(const TreeArgs& a, const TreeSeg& s, int node, int c0) {
+    const int t0 = c0 - s.len;                                 // node of the first key, negative ahead of the tree
+    if (t0 <= -32) return FULL;
+    if (t0 >= s.n) return 0;
+    const int lo = max(t0, 0);
+    unsigned w;                                                // nodes lo .. lo + 31
+    if (a.mask) {
+        const unsigned* m = a.mask + (size_t)(s.first + node) * a.mask_ld;
+        const int i = lo >> 5, last = (s.n - 1) >> 5;
+        w = __funnelshift_r(m[i], i < last ? m[i + 1] : 0u, lo & 31);
+    } else {
+        const int k = node + 1 - lo;
+        w = k >= 32 ? FULL : k <= 0 ? 0u : (1u << k) - 1u;
+    }
+    if (s.n - lo < 32) w &= (1u << (s.n - lo)) - 1u;
+    return t0 < 0 ? (w << -t0) | ((1u << -t0) - 1u) : w;
+}
+// Elements v .. v + 3 of a finished head of a row: turned back, gated, stored.
+template <class T>
+__device__ __forceinline__ void tree_put(const TreeArgs& a, int row, int h, int v, float4 x) {
+    float o[4] = {x.x, x.y, x.z, x.w};
+    if (a.vcs) {
+        const int pos = a.pos[row];
+        if (pos < 0 || pos >= a.rope_len) {
+            report_size(a.error_flag);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j += 2)
+            if (v + j < a.vdim) {
+                const size_t at = (size_t)pos * (a.vdim / 2) + (v + j) / 2;
+                const float c = a.vcs[at], s = a.vsn[at], u = o[j];
+                o[j] = fmaf(u, c, o[j + 1] * s);
+                o[j + 1] = fmaf(o[j + 1], c, -(u * s));
+            }
+    }
+    if (a.gate) {
+        const float w = sigmoid_fast(a.gate[(size_t)row * a.ldg + h]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] *= w;
+    }
+    T* out = static_cast<T*>(a.out) + (size_t)row * a.ldo + (size_t)h * a.vdim + v;
+    if (v + 4 <= a.vdim && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0) {
+        put4(out, make_float4(o[0], o[1], o[2], o[3]));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (v + j < a.vdim) put(out + j, o[j]);
+}
+
+}  // namespace detb

@@ -659,6 +659,133 @@ typedef struct {
 size_t det_f_moe_scratch_bytes(int M, int experts, int top, int ff, int n, int dtype);
 void det_f_moe(const det_fmoe_op* op, cudaStream_t st);
 
+/* ---- A step of drafted tokens (speculative decoding): several sequences, each with a tree of tokens behind its cached rows.
+ * The entry points below return 0 when the work was queued and 1 when the call was refused (bad sizes, a NULL pointer, a misaligned
+ * buffer, no usable device): a refusal prints its reason, launches nothing and leaves every buffer as it was; they never abort.
+ * What only device memory knows (first, len, pos, keep, count) is checked by the kernels: a sequence whose entries do not fit its
+ * cache, the bounds of the call or the tables is left out, its outputs stay as they were, and det_last_error() returns 2.
+ *
+ * The rows of a step.  Sequence b owns the rows first[b] .. first[b + 1] - 1 (first[0] = 0, ascending; none is allowed), node i of
+ * its tree being row first[b] + i; its cache table[b].cache holds len[b] rows ahead of them, and node i belongs at cache row
+ * len[b] + i.  table, first [seqs + 1] and len [seqs] are device arrays, so a captured step can be replayed with other lengths.
+ * `rows` is the number of rows of the buffers: rows from first[seqs] on belong to nobody and are left as they were.  max_nodes
+ * bounds a sequence's rows; max_len (>= 0) is the expected largest len: it sizes the launch, and results hold for any len.   */
+typedef struct {
+    const det_seq_slot* table;
+    const int* first;
+    const int* len;
+    int seqs;
+    int rows;
+    int max_nodes;
+    int max_len;
+} det_tree_ref;
+
+/* Tables of the position rotation: cos[p][i] = mscale * cos((pos0 + p) * f_i), sin likewise, p < n, i < dims / 2 (fp32, computed
+ * in binary64 up to the last rounding).  f_i = base^(-2i / dims), scaled for contexts longer than the model was made for:
+ *   DET_ROPE_LINEAR  f_i / factor
+ *   DET_ROPE_BASE    base * factor^(dims / (dims - 2)) instead of base (dims > 2)
+ *   DET_ROPE_RAMP    f_i * (w + (1 - w) / factor), w = (orig_ctx * f_i / 2 pi - low) / (high - low) clamped to 0 .. 1: columns
+ *                    that turn more than `high` times within orig_ctx positions stay, those below `low` turns are stretched */
+#define DET_ROPE_PLAIN 0
+#define DET_ROPE_LINEAR 1
+#define DET_ROPE_BASE 2
+#define DET_ROPE_RAMP 3
+typedef struct {
+    int dims;
+    int scaling;
+    double base;
+    double factor;
+    double orig_ctx;
+    double low;
+    double high;
+    float mscale;
+    int pos0;
+    int n;
+    float* cos;
+    float* sin;
+} det_frope_op;
+int det_f_rope_table(const det_frope_op* op, cudaStream_t st);
+
+/* Norm of every query and key head, rotation, and the rows' cache entries in one pass over the fp32 rows y (stride ldy; q, k, v at
+ * q_off, k_off, v_off): x / sqrt(mean over dim of x^2 + eps) * norm (q_norm, k_norm [dim], NULL: no norm), then the first rot_dims
+ * elements rotated by the row's position: half = 0 pairs (2i, 2i + 1), half = 1 pairs (i, i + rot_dims / 2) (tables
+ * [position][rot_dims / 2] with rope_len rows).  vrope_cos / vrope_sin ([position][vdim / 2], NULL: none) rotate the values' pairs
+ * (2i, 2i + 1).  pos [rows] (device) are the positions, NULL: len[b] + i.  q [rows][det_f_attn_q_ld] and the cache rows (the layout
+ * of det_f_attn: det_f_attn_ld elements) are in the activation type, both 16-byte aligned, heads padded with zeros; q is not
+ * scaled.  dim, vdim <= 256.                                                                                                 */
+typedef struct {
+    int heads, kv_heads, dim, vdim, rot_dims;
+    int half;
+    float eps;
+    const float* q_norm;
+    const float* k_norm;
+    int cap;
+    int dtype;
+    const float* y;
+    int ldy;
+    int q_off, k_off, v_off;
+    int rope_len;
+    const float* rope_cos;
+    const float* rope_sin;
+    const float* vrope_cos;
+    const float* vrope_sin;
+    const int* pos;
+    void* q;
+    det_tree_ref seq;
+} det_fqk_op;
+int det_f_qk_rope(const det_fqk_op* op, cudaStream_t st);
+
+/* Attention of a step's rows over their sequences' caches (rows as det_f_qk_rope or det_f_attn_prep leave them).  Row i of sequence
+ * b attends the cached rows j < len[b] and, of its own tree, the nodes j whose bit j % 32 of word mask[row * mask_ld + j / 32] is
+ * set (its ancestors and itself, as a rule); mask NULL: the nodes j <= i, that is, the rows are a run of tokens.  Query head h reads
+ * key/value head h / (heads / kv_heads); out[row][h * vdim + j] = sum softmax(scale * q . k) v, times sigmoid(gate[row * ldg + h])
+ * (gate NULL: 1), in the activation type, row stride ldo.  A row that attends nothing gets zeros; what masked and missing rows hold,
+ * NaN included, has no influence.  vrope_cos / vrope_sin: the values are rotated, and a head's output is turned back by pos[row]
+ * (then needed; rope_len rows in the tables).  scale > 0.  dim, vdim <= 256; with a mask max_nodes <= DET_MAX_TREE.
+ * `scratch` (16-byte aligned, det_f_tree_scratch_bytes) holds the pieces of rows whose keys several CTAs share: calls that may
+ * overlap on the GPU need scratch of their own.  Results do not depend on the order of arrival.                              */
+#define DET_MAX_TREE 1024
+typedef struct {
+    int heads, kv_heads, dim, vdim;
+    float scale;
+    int cap;
+    int dtype;
+    const void* q;
+    const unsigned* mask;
+    int mask_ld;
+    const float* gate;
+    int ldg;
+    const int* pos;
+    int rope_len;
+    const float* vrope_cos;
+    const float* vrope_sin;
+    void* out;
+    int ldo;
+    void* scratch;
+    det_tree_ref seq;
+} det_ftree_op;
+size_t det_f_tree_scratch_bytes(int heads, int kv_heads, int vdim, int max_nodes);
+int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st);
+
+/* The accepted nodes of every tree become cached rows: in each cache, row len[b] + keep[b * keep_ld + i] moves to row len[b] + i,
+ * i < count[b].  keep must ascend strictly.  table holds `caches` slots, layer after layer: entry e belongs to sequence e % seqs
+ * (no cache twice).  row_bytes is a multiple of 16 (any cache of this part whose rows are 16-byte aligned).  len_out (not len;
+ * NULL: none) receives len[b] + count[b].  max_count bounds count, <= DET_MAX_TREE.  All arrays are device arrays.          */
+typedef struct {
+    int caches;
+    int seqs;
+    int cap;
+    int row_bytes;
+    const det_seq_slot* table;
+    const int* len;
+    const int* keep;
+    int keep_ld;
+    const int* count;
+    int max_count;
+    int* len_out;
+} det_fkeep_op;
+int det_f_tree_keep(const det_fkeep_op* op, cudaStream_t st);
+
 /* Measurement switches of the floating-point ops (results agree up to rounding): bit 0 no norm in the GEMV's prologue, bit 1 no
  * GEMV, bit 2 no split of K in the tensor-core GEMM, bit 3 no tensor-core attention.                                   */
 void det_debug_set_float(int flags);
