@@ -1,8 +1,9 @@
 // Attention of a step of drafted tokens (include/det_b200.h, det_ftree_op): one pass over the keys with the running maximum and sum of
 // the softmax, in 32-bit.  ftree.cuh says how the work is dealt out.
 //
+//   k_ftree_tc     bfloat16: ftree_tc.cu.
 //   k_ftree_simt   32-bit products on the CUDA cores: 256 threads over a tile of query rows x 64 keys, keys and values staged in
-//                  shared memory as fp32.
+//                  shared memory.
 //   k_ftree_merge  adds the pieces of the segments that several CTAs shared.
 #include "ftree.cuh"
 #include <algorithm>
@@ -16,10 +17,6 @@ static size_t simt_smem(int block, int kd, int vd) {
     return ((size_t)(block + TS_KEYS) * (kd + 4) + (size_t)TS_KEYS * (vd + 4) + (size_t)block * (TS_KEYS + 4)) * sizeof(float);
 }
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const bf16* p) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    return make_float4(bf_lo(v.x), bf_hi(v.x), bf_lo(v.y), bf_hi(v.y));
-}
 __device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
     return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s))));
 }
@@ -36,7 +33,7 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 // Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.
-template <class T, int TR, int VJ>
+template <int TR, int VJ>
 __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
     extern __shared__ __align__(16) float tsm[];
     __shared__ TreeShare share;
@@ -58,8 +55,8 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
     TreeItem it;
     while (tree_next(a, walk, it)) {
         const TreeSeg& s = it.s;
-        const T* cache = static_cast<const T*>(a.seq.table[s.b].cache);
-        const T* q = static_cast<const T*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
+        const float* cache = static_cast<const float*>(a.seq.table[s.b].cache);
+        const float* q = static_cast<const float*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
         __syncthreads();
         for (int i = tid; i < RB * (a.kd / 4); i += TS_THREADS) {
             const int r = i / (a.kd / 4), e = (i - r * (a.kd / 4)) * 4, row = s.r0 + r;
@@ -80,12 +77,12 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
             const int k0 = t * TS_KEYS, last = s.len + s.n;
             const bool tree = k0 + TS_KEYS > s.len;
             __syncthreads();
-            const T* kp = cache + (size_t)k0 * a.ld + it.g * a.kd;
+            const float* kp = cache + (size_t)k0 * a.ld + it.g * a.kd;
             for (int i = tid; i < TS_KEYS * (a.kd / 4); i += TS_THREADS) {
                 const int k = i / (a.kd / 4), e = (i - k * (a.kd / 4)) * 4;
                 *reinterpret_cast<float4*>(K + k * ldk + e) = k0 + k < last ? load4(kp + (size_t)k * a.ld + e) : make_float4(0, 0, 0, 0);
             }
-            const T* vp = cache + (size_t)k0 * a.ld + a.kv_heads * a.kd + it.g * a.vd;
+            const float* vp = cache + (size_t)k0 * a.ld + a.kv_heads * a.kd + it.g * a.vd;
             for (int i = tid; i < TS_KEYS * (a.vd / 4); i += TS_THREADS) {
                 const int k = i / (a.vd / 4), e = (i - k * (a.vd / 4)) * 4;
                 *reinterpret_cast<float4*>(V + k * ldv + e) = k0 + k < last ? load4(vp + (size_t)k * a.ld + e) : make_float4(0, 0, 0, 0);
@@ -173,13 +170,13 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
                 piece[RB + r] = sum;
             }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // no key seen
+            const TreeOut<float> out(a, s.first + row / a.per_kv, it.g * a.per_kv + row % a.per_kv);
 #pragma unroll
             for (int j = 0; j < VJ; j++) {
                 const int c = 4 * tx + 64 * j;
                 if (c >= a.vd) continue;
                 if (it.whole) {
-                    tree_put<T>(a, s.first + row / a.per_kv, it.g * a.per_kv + row % a.per_kv, c,
-                                make_float4(o[i][j].x * inv, o[i][j].y * inv, o[i][j].z * inv, o[i][j].w * inv));
+                    out.put4at(c, scaled4(o[i][j], inv));
                 } else {
                     put4(piece + 2 * RB + ((size_t)(c / 4) * RB + r) * 4, o[i][j]);
                 }
@@ -240,31 +237,32 @@ __global__ void __launch_bounds__(TM_THREADS) k_ftree_merge(const TreeArgs a) {
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const int row = s.r0 + r;
-        tree_put<T>(a, s.first + row / a.per_kv, g * a.per_kv + row % a.per_kv, v * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        TreeOut<T>(a, s.first + row / a.per_kv, g * a.per_kv + row % a.per_kv).put4at(v * 4, scaled4(o, inv));
     }
 }
 
 // ------------------------------------------------------------------------------------------------------ host side
-template <class T, int TR, int VJ>
+template <int TR, int VJ>
 static cudaError_t launch_simt(const TreeArgs& a, cudaStream_t q) {
     const size_t smem = simt_smem(a.block, a.kd, a.vd);
-    const cudaError_t e = cudaFuncSetAttribute(k_ftree_simt<T, TR, VJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(k_ftree_simt<TR, VJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl_try(k_ftree_simt<T, TR, VJ>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a);
+    return launch_pdl_try(k_ftree_simt<TR, VJ>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a);
 }
-template <class T, int TR>
+template <int TR>
 static cudaError_t launch_simt_v(const TreeArgs& a, cudaStream_t q) {
-    return a.vd <= 64 ? launch_simt<T, TR, 1>(a, q) : a.vd <= 128 ? launch_simt<T, TR, 2>(a, q) : launch_simt<T, TR, 4>(a, q);
+    return a.vd <= 64 ? launch_simt<TR, 1>(a, q) : a.vd <= 128 ? launch_simt<TR, 2>(a, q) : launch_simt<TR, 4>(a, q);
 }
 template <class T>
-static cudaError_t launch_all(const TreeArgs& a, cudaStream_t q) {
-    cudaError_t e = a.block == 16 ? launch_simt_v<T, 1>(a, q) : launch_simt_v<T, 4>(a, q);
-    if (e != cudaSuccess) return e;
+static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
     const int chunks = std::max(1, std::min(16, a.block * (a.vd / 4) / TM_THREADS));
     return launch_pdl_try(k_ftree_merge<T>, dim3(a.kv_heads * chunks, a.seq.seqs * a.blocks), dim3(TM_THREADS), 0, q, 1, a);
 }
-// Rows of a block: as many as fill the tile, 64 at most.
-static int rows_of_block(int rows) { return rows <= 16 ? 16 : 64; }
+// Rows of a block and keys of a tile.
+static void simt_shape(int rows, int* block, int* tile) {
+    *block = rows <= 16 ? 16 : 64;
+    *tile = TS_KEYS;
+}
 
 }  // namespace detb
 
@@ -274,9 +272,12 @@ extern "C" {
 
 size_t det_f_tree_scratch_bytes(int heads, int kv_heads, int vdim, int max_nodes) {
     if (heads <= 0 || kv_heads <= 0 || vdim <= 0 || max_nodes <= 0) return 16;
-    const long long rows = (long long)max_nodes * (heads / kv_heads);
-    const int block = rows_of_block((int)std::min<long long>(rows, 1 << 20));
-    return TREE_CTAS * 2 * tree_piece_floats(block, round8(vdim)) * sizeof(float);
+    const int rows = (int)std::min((long long)max_nodes * (heads / kv_heads), 1ll << 24), vd = round8(vdim);
+    int block = 0, other = 0, tile = 0;
+    simt_shape(rows, &block, &tile);
+    ftree_tc_shape(rows, 8, vd, &other, &tile);      // the smallest keys have the largest blocks
+    block = std::max(block, other);
+    return TREE_CTAS * 2 * tree_piece_floats(block, vd) * sizeof(float);
 }
 
 int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
@@ -296,13 +297,13 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     if (op->seq.rows == 0 || op->seq.seqs == 0 || rows == 0) return 0;
     DETB_TAKE(op->q && op->out && op->scratch && aligned16(op->q) && aligned16(op->scratch), "q, out or scratch is NULL or misaligned");
     TreeArgs a{};
-    a.block = rows_of_block((int)rows);
-    a.tile = TS_KEYS;
+    a.kd = round8(op->dim); a.vd = round8(op->vdim);
+    if (op->dtype == DET_BF16) ftree_tc_shape((int)rows, a.kd, a.vd, &a.block, &a.tile);
+    else simt_shape((int)rows, &a.block, &a.tile);
     const long long blocks = (rows + a.block - 1) / a.block;
     DETB_TAKE(blocks * op->seq.seqs <= 65535, "too many rows");
     DETB_TAKE(runtime_ready(), "no usable device");
     a.heads = op->heads; a.kv_heads = op->kv_heads; a.per_kv = op->heads / op->kv_heads; a.dim = op->dim; a.vdim = op->vdim;
-    a.kd = round8(op->dim); a.vd = round8(op->vdim);
     a.ld = det_f_attn_ld(op->kv_heads, op->dim, op->vdim);
     a.ldq = det_f_attn_q_ld(op->heads, op->dim);
     a.scale2 = op->scale * 1.4426950408889634f;
@@ -314,7 +315,12 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     a.seq = op->seq;
     a.ctas = std::min(TREE_CTAS, sm_count());
     cudaStream_t q = queue_of(st);
-    return launched(name, op->dtype == DET_BF16 ? launch_all<bf16>(a, q) : launch_all<float>(a, q));
+    if (op->dtype == DET_BF16) {
+        if (int rc = launched(name, ftree_tc_launch(a, q))) return rc;
+        return launched(name, launch_merge<bf16>(a, q));
+    }
+    if (int rc = launched(name, a.block == 16 ? launch_simt_v<1>(a, q) : launch_simt_v<4>(a, q))) return rc;
+    return launched(name, launch_merge<float>(a, q));
 }
 
 }  // extern "C"

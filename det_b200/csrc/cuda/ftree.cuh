@@ -54,7 +54,7 @@ __device__ __forceinline__ TreePlace tree_place(const det_tree_ref& s, int row, 
 // falls to one CTA is finished there; of the others every CTA leaves a piece (maximum, sum, values per row) in scratch, and the
 // merge kernel adds the pieces in order of the keys.  A CTA has at most two such pieces, of its first and of its last segment.
 constexpr int TREE_CTAS = 148;
-constexpr int TREE_SHARE = 2;      // tiles of a CTA, if there are enough
+constexpr int TREE_SHARE = 2;      // tiles of a CTA at least, if there are enough
 
 struct TreeArgs {
     int heads, kv_heads, per_kv, dim, vdim, kd, vd, ld, ldq;
@@ -203,38 +203,52 @@ __device__ __forceinline__ unsigned tree_seen(const TreeArgs& a, const TreeSeg& 
     if (s.n - lo < 32) w &= (1u << (s.n - lo)) - 1u;
     return t0 < 0 ? (w << -t0) | ((1u << -t0) - 1u) : w;
 }
-// Elements v .. v + 3 of a finished head of a row: turned back, gated, stored.
+// A finished head of a row: elements v .. v + 3 are turned back, gated and stored.
 template <class T>
-__device__ __forceinline__ void tree_put(const TreeArgs& a, int row, int h, int v, float4 x) {
-    float o[4] = {x.x, x.y, x.z, x.w};
-    if (a.vcs) {
-        const int pos = a.pos[row];
-        if (pos < 0 || pos >= a.rope_len) {
-            report_size(a.error_flag);
+struct TreeOut {
+    T* out;
+    const float* c;                // turn of the row's position, or NULL
+    const float* s;
+    float w;
+    int vdim;
+    bool skip;
+    __device__ __forceinline__ TreeOut(const TreeArgs& a, int row, int h)
+        : out(static_cast<T*>(a.out) + (size_t)row * a.ldo + (size_t)h * a.vdim), c(nullptr), s(nullptr), w(1.0f), vdim(a.vdim), skip(false) {
+        if (a.vcs) {
+            const int pos = a.pos[row];
+            skip = pos < 0 || pos >= a.rope_len;
+            if (skip) report_size(a.error_flag);
+            c = a.vcs + (size_t)(skip ? 0 : pos) * (a.vdim / 2);
+            s = a.vsn + (size_t)(skip ? 0 : pos) * (a.vdim / 2);
+        }
+        if (a.gate) w = sigmoid_fast(a.gate[(size_t)row * a.ldg + h]);
+    }
+    __device__ __forceinline__ void put4at(int v, float4 x) const {
+        if (skip) return;
+        float o[4] = {x.x * w, x.y * w, x.z * w, x.w * w};
+        if (c) {
+#pragma unroll
+            for (int j = 0; j < 4; j += 2)
+                if (v + j < vdim) {
+                    const float cj = c[(v + j) / 2], sj = s[(v + j) / 2], u = o[j];
+                    o[j] = fmaf(u, cj, o[j + 1] * sj);
+                    o[j + 1] = fmaf(o[j + 1], cj, -(u * sj));
+                }
+        }
+        T* to = out + v;
+        if (v + 4 <= vdim && (reinterpret_cast<uintptr_t>(to) & (4 * sizeof(T) - 1)) == 0) {
+            put4(to, make_float4(o[0], o[1], o[2], o[3]));
             return;
         }
 #pragma unroll
-        for (int j = 0; j < 4; j += 2)
-            if (v + j < a.vdim) {
-                const size_t at = (size_t)pos * (a.vdim / 2) + (v + j) / 2;
-                const float c = a.vcs[at], s = a.vsn[at], u = o[j];
-                o[j] = fmaf(u, c, o[j + 1] * s);
-                o[j + 1] = fmaf(o[j + 1], c, -(u * s));
-            }
+        for (int j = 0; j < 4; j++)
+            if (v + j < vdim) put(to + j, o[j]);
     }
-    if (a.gate) {
-        const float w = sigmoid_fast(a.gate[(size_t)row * a.ldg + h]);
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] *= w;
-    }
-    T* out = static_cast<T*>(a.out) + (size_t)row * a.ldo + (size_t)h * a.vdim + v;
-    if (v + 4 <= a.vdim && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0) {
-        put4(out, make_float4(o[0], o[1], o[2], o[3]));
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (v + j < a.vdim) put(out + j, o[j]);
-}
+};
+__device__ __forceinline__ float4 scaled4(float4 v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
+
+// ftree_tc.cu: bfloat16 activations.  Rows of a block and keys of a tile are the kernel's.
+void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile);
+cudaError_t ftree_tc_launch(const TreeArgs& a, cudaStream_t q);
 
 }  // namespace detb

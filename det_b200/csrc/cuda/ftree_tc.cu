@@ -1,0 +1,541 @@
+// Tree attention over bfloat16 caches on the tensor cores: tcgen05.mma kind::f16, scores and outputs in TMEM, one pass over the keys.
+//
+// A slot is 128 query rows (TMEM lanes) with scores S = Q K^T [128 x keys of a tile], weights P over the same columns (bfloat16, read
+// by the second product straight from TMEM) and outputs O += P V [128 x vd].  A thread of a slot's four warps owns one row: running
+// reference, sum and weights of its scores need no exchange.  The reference moves (and O is scaled) only when a row's maximum has
+// grown by more than 2^8 over it, so the weights stay below 2^8 and O is touched rarely.
+//
+// Two slots per CTA take turns, so that the products of one run beside the exponentials of the other.  Up to 128 rows: both hold the
+// same rows and take every other tile of keys, and their results are added at the end; more rows: 128 rows each over the same tiles.
+// Heads above 128: one slot (TMEM and shared memory hold no more), tiles of 64 keys.
+//
+// Warps: four per slot for the softmax; three that bring rows of Q, K and V into shared memory by 16-byte asynchronous copies, laid
+// out as the products want them (128-byte swizzle; K and Q K-major, V as it lies in the cache, MN-major); one that issues the products.
+// The caches' addresses are in device memory, so a tensor map on the host cannot describe them.
+//
+// A weight is rounded to bfloat16 for its product, as any tensor-core form must (half a step, 2^-8 relative, independent from key to
+// key); sums and references are fp32.
+#include "ftree.cuh"
+#include "umma.cuh"
+#include <algorithm>
+
+namespace detb {
+
+constexpr int TT_ROWS = 128;
+constexpr int TT_COPY = 96;                          // threads that copy
+constexpr float TT_GROWTH = 8.0f;                   // log2 of how far a maximum may outgrow the reference
+
+template <int SLOTS, int KT>
+struct TtCfg {
+    static constexpr int SOFT = 4 * SLOTS, THREADS = (SOFT + TT_COPY / 32 + 1) * 32, PRODUCTS = SOFT + TT_COPY / 32;   // warps
+    static constexpr int O_COL = SLOTS * KT;
+    static constexpr int PEND = 3;                  // tiles whose copies are in flight (flush() counts on three; PEND + 2 <= stages)
+};
+struct TtShape {
+    int nkb, nvb;                                   // 64-element blocks of a key, of a value
+    int stages, stage_bytes;
+    int both;                                       // the slots hold the same rows
+    int q_bytes;                                    // of one slot's rows
+};
+
+constexpr int TT_STAGES = 12;
+struct TtTables {
+    unsigned long long full[TT_STAGES], empty[TT_STAGES], q_full[2], q_empty[2], s_full[2], p_full[2], o_full, o_empty;
+    float2 ml[2][TT_ROWS];                           // [slot]: reference and sum of a row
+    TreeShare share;
+    unsigned tmem_slot;
+    int odd[4];                                      // number (+ 1) of the stretch whose values were not all finite
+};
+constexpr size_t TT_SMEM = 227 * 1024;
+
+__device__ __forceinline__ void umma_f16_ss(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(unsigned d, unsigned a, unsigned long long b, unsigned idesc, unsigned acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// MN-major, SWIZZLE_128B: 64 neighbouring values of a key per 128-byte row, 8-key groups 1024 bytes apart, blocks of 64 values `lead`
+// bytes apart.
+__device__ __forceinline__ unsigned long long umma_desc_mn(const void* smem, unsigned lead) {
+    const unsigned addr = smem_addr(smem);
+    unsigned long long d = 0;
+    d |= (unsigned long long)((addr & 0x3FFFF) >> 4);
+    d |= (unsigned long long)(lead >> 4) << 16;
+    d |= (unsigned long long)(1024 >> 4) << 32;
+    d |= (unsigned long long)1 << 46;
+    d |= (unsigned long long)2 << 61;
+    return d;
+}
+// fp32 accumulator, bfloat16 operands, M = 128, N = n; b_mn: B is MN-major.
+__device__ __forceinline__ unsigned tt_idesc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((unsigned)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_st(unsigned taddr, const unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {      // relative error about 2^-22; 2^-inf = 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Rows of 16-byte pieces into swizzled blocks of `rows` rows x 128 bytes; pieces past `real` and rows past `have` become zeros.
+// row_of(r): address of row r.
+template <class F>
+__device__ __forceinline__ void tt_copy(unsigned dst, int rows, int pieces, int real, int have, int tid, F row_of) {
+    const int dr = TT_COPY / pieces, dc = TT_COPY - dr * pieces;
+    int r = tid / pieces, c = tid - r * pieces;
+    const int total = rows * pieces;
+    for (int i = tid; i < total; i += TT_COPY) {
+        const bool ok = c < real && r < have;
+        copy16(dst + (unsigned)((c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4)), ok ? row_of(r) + c * 8 : row_of(0), ok);
+        r += dr;
+        c += dc;
+        if (c >= pieces) {
+            c -= pieces;
+            r++;
+        }
+    }
+}
+// Values of the tree that are not finite become zeros in the staged tile; true when there were any.  A thread looks at its own copies.
+__device__ __forceinline__ bool tt_clean(uint8_t* tile, int rows, int pieces, int tid) {
+    bool odd = false;
+    for (int i = tid; i < rows * pieces; i += TT_COPY) {
+        const int r = i / pieces, c = i - r * pieces;
+        uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4));
+        uint4 v = *p;
+        unsigned w[4] = {v.x, v.y, v.z, v.w};
+        bool hit = false;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, hit = true;
+            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, hit = true;
+        }
+        if (hit) *p = make_uint4(w[0], w[1], w[2], w[3]);
+        odd |= hit;
+    }
+    return odd;
+}
+
+template <int SLOTS, int KT>
+__global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const TreeArgs a, const TtShape sh) {
+    using Cfg = TtCfg<SLOTS, KT>;
+    constexpr int SOFT = Cfg::SOFT, PRODUCTS = Cfg::PRODUCTS;
+    extern __shared__ __align__(1024) uint8_t Qs[];                     // [SLOTS][nkb][128][128 B], the ring, the tables
+    uint8_t* ring = Qs + SLOTS * sh.q_bytes;
+    TtTables& tb = *reinterpret_cast<TtTables*>(ring + (size_t)sh.stages * sh.stage_bytes);
+    auto &full = tb.full, &empty = tb.empty;
+    auto &q_full = tb.q_full, &q_empty = tb.q_empty, &s_full = tb.s_full, &p_full = tb.p_full;
+    auto &o_full = tb.o_full, &o_empty = tb.o_empty;
+    auto &odd = tb.odd;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long wl = wait_limit(a.error_flag);
+    pdl_trigger();
+    if (smem_addr(Qs) & 1023) {                      // the layout of the operands needs it
+        pdl_wait();
+        if (threadIdx.x == 0) report_size(a.error_flag);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < sh.stages; s++) {
+            mbar_init(&full[s], TT_COPY / 32);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&q_full[i], TT_COPY / 32);
+            mbar_init(&q_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+        }
+        mbar_init(&o_full, 1);
+        mbar_init(&o_empty, SOFT);
+        for (int i = 0; i < 4; i++) odd[i] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == PRODUCTS) tmem_alloc(&tb.tmem_slot, 512);
+    pdl_wait();
+    if (warp == 0) {
+        const TreeShare w = tree_start(a, blockIdx.x, lane);
+        if (lane == 0) tb.share = w;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tb.tmem_slot;
+    TreeWalk walk{tb.share, false};
+    TreeItem it;
+    bool ok = true;
+    auto wait = [&](unsigned long long* bar, unsigned parity) { return __all_sync(FULL, mbar_wait(bar, parity, wl)) != 0; };   // by whole warps
+    const bool both = SLOTS == 2 && sh.both;         // the slots take every other tile of the same rows
+    const int lead = both ? 2 : 1;                   // tiles whose scores are asked for ahead
+    unsigned item = 0;                               // stretches so far
+
+    if (warp >= SOFT && warp < PRODUCTS) {
+        // ---- copies
+        const int tid = threadIdx.x - SOFT * 32;
+        const int kp = (a.kd + 15) / 16 * 2, vp = (a.vd + 15) / 16 * 2;
+        // a copy in flight: stage, and whether it begins a stretch (1), holds values of a tree (2), the stretch (from bit 2)
+        int st[Cfg::PEND], what[Cfg::PEND];
+#pragma unroll
+        for (int i = 0; i < Cfg::PEND; i++) st[i] = -1, what[i] = 0;
+        unsigned c = 0;                              // tiles issued
+        auto land = [&](int s, int w) {
+            if (s < 0) return;
+            if (w & 2) {
+                if (tt_clean(ring + (size_t)s * sh.stage_bytes, KT, vp, tid)) *reinterpret_cast<volatile int*>(&odd[(w >> 2) & 3]) = (w >> 2) + 1;
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+                if (w & 1) mbar_arrive(&q_full[both ? (w >> 2) & 1 : 0]);
+                mbar_arrive(&full[s]);
+            }
+        };
+        auto flush = [&]() {
+            copies_wait<2>();
+            land(st[2], what[2]);
+            copies_wait<1>();
+            land(st[1], what[1]);
+            copies_wait<0>();
+            land(st[0], what[0]);
+            st[0] = st[1] = st[2] = -1;
+        };
+        while (ok && tree_next(a, walk, it)) {
+            const TreeSeg& s = it.s;
+            const bf16* cache = static_cast<const bf16*>(a.seq.table[s.b].cache);
+            const int qb = both ? item & 1 : 0;
+            if (!both) flush();                      // the wait below needs what is in flight
+            if (item >= (both ? 2u : 1u)) ok = wait(&q_empty[qb], ((both ? item >> 1 : item) & 1u) ^ 1u);
+            if (!ok) break;
+            const bf16* q = static_cast<const bf16*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
+            auto q_row = [&](int r) {
+                const int row = s.r0 + r;
+                return q + (size_t)(row / a.per_kv) * a.ldq + (row % a.per_kv) * a.kd;
+            };
+            for (int slot = 0; slot < (both ? 1 : SLOTS); slot++) {
+                const int r0 = slot * TT_ROWS;
+                if (slot && s.rows <= r0) break;
+                tt_copy(smem_addr(Qs + (size_t)(both ? qb : slot) * sh.q_bytes), TT_ROWS, kp, a.kd / 8, s.rows - r0, tid,
+                        [&](int r) { return q_row(r0 + r); });
+            }
+            auto fetch = [&](bool value, int t) {
+                const unsigned sn = c % sh.stages;
+                if (c >= (unsigned)sh.stages) ok = wait(&empty[sn], ((c / sh.stages) & 1u) ^ 1u);
+                if (!ok) return;
+                const int k0 = (it.tile + t) * KT;
+                const bf16* rows = cache + (size_t)k0 * a.ld + (value ? a.kv_heads * a.kd + it.g * a.vd : it.g * a.kd);
+                tt_copy(smem_addr(ring + (size_t)sn * sh.stage_bytes), KT, value ? vp : kp, (value ? a.vd : a.kd) / 8, s.len + s.n - k0, tid,
+                        [&](int r) { return rows + (size_t)r * a.ld; });
+                copies_commit();
+                copies_wait<Cfg::PEND>();
+                land(st[Cfg::PEND - 1], what[Cfg::PEND - 1]);
+#pragma unroll
+                for (int i = Cfg::PEND - 1; i > 0; i--) st[i] = st[i - 1], what[i] = what[i - 1];
+                st[0] = (int)sn;
+                what[0] = (!value && t == 0 ? 1 : 0) | (value && k0 + KT > s.len ? 2 : 0) | (int)(item << 2);
+                c++;
+            };
+            for (int t = 0; t < min(lead, it.n) && ok; t++) fetch(false, t);
+            for (int t = 0; t < it.n && ok; t++) {
+                fetch(true, t);
+                if (ok && t + lead < it.n) fetch(false, t + lead);
+            }
+            item++;
+        }
+        flush();
+    } else if (warp == PRODUCTS) {
+        // ---- products
+        if (lane == 0) {
+            const unsigned id_s = tt_idesc(KT, false), vn = (unsigned)(a.vd + 15) / 16 * 16, id_o = tt_idesc((int)vn, true);
+            const int ksteps = (a.kd + 15) / 16;
+            unsigned c = 0, np[2] = {0, 0};          // tiles taken, weights taken per slot
+            while (ok && tree_next(a, walk, it)) {
+                const int qb = both ? item & 1 : 0;
+                const bool second = !both && SLOTS == 2 && it.s.rows > TT_ROWS;
+                ok = mbar_wait(&q_full[qb], ((both ? item >> 1 : item) & 1u), wl);
+                if (!ok) break;
+                auto scores = [&](int slot, const uint8_t* K) {
+                    const uint8_t* Q = Qs + (size_t)(both ? qb : slot) * sh.q_bytes;
+                    for (int k = 0; k < ksteps; k++)
+                        umma_f16_ss(tmem + slot * KT, umma_desc(Q + (size_t)(k >> 2) * TT_ROWS * 128) + 2 * (k & 3),
+                                    umma_desc(K + (size_t)(k >> 2) * KT * 128) + 2 * (k & 3), id_s, k ? 1u : 0u);
+                    umma_commit(&s_full[slot]);
+                };
+                auto outputs = [&](int slot, const uint8_t* V, bool first) {
+                    for (int k = 0; k < KT / 16; k++)
+                        umma_f16_ts(tmem + Cfg::O_COL + slot * (256 / SLOTS), tmem + slot * KT + k * 8, umma_desc_mn(V + k * 2048, KT * 128), id_o,
+                                    first && k == 0 ? 0u : 1u);
+                };
+                auto stage = [&]() {
+                    const unsigned s = c % sh.stages;
+                    ok = mbar_wait(&full[s], (c / sh.stages) & 1u, wl);
+                    c++;
+                    tc_fence_after();
+                    return s;
+                };
+                auto weights = [&](int slot) {
+                    ok = mbar_wait(&p_full[slot], np[slot] & 1u, wl);
+                    np[slot]++;
+                    tc_fence_after();
+                };
+                for (int t = 0; t < min(lead, it.n) && ok; t++) {
+                    const unsigned s = stage();
+                    if (!ok) break;
+                    scores(both ? t & 1 : 0, ring + (size_t)s * sh.stage_bytes);
+                    if (second) scores(1, ring + (size_t)s * sh.stage_bytes);
+                    umma_commit(&empty[s]);
+                    if (t + 1 == it.n) umma_commit(&q_empty[qb]);
+                }
+                for (int t = 0; t < it.n && ok; t++) {
+                    const unsigned sv = stage();
+                    if (!ok) break;
+                    const uint8_t* V = ring + (size_t)sv * sh.stage_bytes;
+                    if (t == 0 && item > 0) {        // the outputs of the stretch before have been read
+                        ok = mbar_wait(&o_empty, (item & 1u) ^ 1u, wl);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    const int slot = both ? t & 1 : 0;
+                    const bool more = t + lead < it.n;
+                    unsigned sk = 0;
+                    weights(slot);
+                    if (!ok) break;
+                    outputs(slot, V, both ? t < 2 : t == 0);
+                    if (!second) umma_commit(&empty[sv]);
+                    if (more) {
+                        sk = stage();
+                        if (!ok) break;
+                        scores(slot, ring + (size_t)sk * sh.stage_bytes);
+                    }
+                    if (second) {
+                        weights(1);
+                        if (!ok) break;
+                        outputs(1, V, t == 0);
+                        umma_commit(&empty[sv]);
+                        if (more) scores(1, ring + (size_t)sk * sh.stage_bytes);
+                    }
+                    if (more) {
+                        umma_commit(&empty[sk]);
+                        if (t + lead + 1 == it.n) umma_commit(&q_empty[qb]);
+                    }
+                }
+                if (ok) umma_commit(&o_full);
+                item++;
+            }
+        }
+    } else {
+        // ---- softmax
+        const int slot = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const unsigned lanes = (unsigned)(quarter * 32) << 16;
+        const unsigned ts = tmem + lanes + slot * KT, to = tmem + lanes + Cfg::O_COL + slot * (256 / SLOTS);
+        const int chunks = (a.vd + 31) / 32;
+        unsigned ns = 0;                             // scores taken
+        // after an expired wait the stretches are gone through without waiting, so that all warps meet at the barrier below
+        while (tree_next(a, walk, it)) {
+            const TreeSeg& s = it.s;
+            const int br = both ? r : slot * TT_ROWS + r;                     // row of the block
+            const bool mine = br < s.rows, any = (both ? quarter * 32 : slot * TT_ROWS + quarter * 32) < s.rows;
+            const int row = s.r0 + min(br, s.rows - 1), node = row / a.per_kv;
+            float m = -INFINITY, l = 0.0f;
+            const bool idle = !both && slot && s.rows <= TT_ROWS;            // the slot has no rows in this stretch
+            const int jobs = idle ? 0 : both ? (it.n + 1 - slot) / 2 : it.n;
+            for (int j = 0; j < jobs; j++) {
+                if (ok) ok = wait(&s_full[slot], ns & 1u);
+                ns++;
+                tc_fence_after();
+                if (any) {
+                    const int k0 = (it.tile + (both ? 2 * j + slot : j)) * KT;
+                    const bool tree = k0 + KT > s.len;
+                    float mt = -INFINITY;
+                    unsigned seen[KT / 32];
+#pragma unroll
+                    for (int q = 0; q < KT / 32; q++) {
+                        seen[q] = tree ? tree_seen(a, s, node, k0 + q * 32) : FULL;
+                        int v[32];
+                        tmem_ld(ts + q * 32, v);
+                        tmem_wait_ld();
+                        if (tree) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) mt = fmaxf(mt, (seen[q] >> i) & 1u ? __int_as_float(v[i]) : -INFINITY);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) mt = fmaxf(mt, __int_as_float(v[i]));
+                        }
+                    }
+                    const bool grow = (mt - m) * a.scale2 > TT_GROWTH;
+                    if (__any_sync(FULL, grow)) {
+                        const float f = grow ? ex2((m - mt) * a.scale2) : 1.0f;
+                        if (grow) m = mt;
+                        l *= f;
+                        __syncwarp();
+                        if (j > 0) {
+                            for (int q = 0; q < chunks; q++) {
+                                int v[32];
+                                tmem_ld(to + q * 32, v);
+                                tmem_wait_ld();
+                                unsigned w[16];
+#pragma unroll
+                                for (int h = 0; h < 2; h++) {
+#pragma unroll
+                                    for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__int_as_float(v[h * 16 + i]) * f);
+                                    tmem_st(to + q * 32 + h * 16, w);
+                                }
+                            }
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.0f : -m * a.scale2;
+                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int q = 0; q < KT / 32; q++) {
+                        int v[32];
+                        tmem_ld(ts + q * 32, v);
+                        tmem_wait_ld();
+                        unsigned w[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float p0 = ex2(fmaf(__int_as_float(v[i]), a.scale2, base)), p1 = ex2(fmaf(__int_as_float(v[i + 1]), a.scale2, base));
+                            if (tree) {
+                                p0 = (seen[q] >> i) & 1u ? p0 : 0.0f;
+                                p1 = (seen[q] >> (i + 1)) & 1u ? p1 : 0.0f;
+                            }
+                            part[i & 2] += p0;
+                            part[(i & 2) + 1] += p1;
+                            w[i / 2] = pack_bf(p0, p1);
+                        }
+                        tmem_st(ts + q * 16, w);
+                    }
+                    l += (part[0] + part[1]) + (part[2] + part[3]);
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[slot]);
+            }
+            if (ok) ok = wait(&o_full, item & 1u);
+            tc_fence_after();
+            // ---- end of the stretch
+            float f0 = 1.0f, f1 = 0.0f;
+            bool other = false;
+            if (both) {
+                asm volatile("bar.sync 1, %0;" ::"n"(SOFT * 32) : "memory");   // the last stretch's have been read
+                tb.ml[slot][r] = make_float2(m, l);
+                asm volatile("bar.sync 1, %0;" ::"n"(SOFT * 32) : "memory");
+                other = it.n > 1;                     // else the second slot had no tile and its outputs hold nothing
+                const float2 x = tb.ml[0][r], y = tb.ml[1][r];
+                m = fmaxf(x.x, y.x);
+                const float b = m == -INFINITY ? 0.0f : m;
+                f0 = ex2((x.x - b) * a.scale2);
+                f1 = ex2((y.x - b) * a.scale2);
+                l = f0 * x.y + f1 * y.y;
+            }
+            if (any && !idle) {
+                const unsigned o0 = tmem + lanes + Cfg::O_COL + (both ? 0 : slot * (256 / SLOTS)), o1 = o0 + 256 / SLOTS;
+                const bool fix = *reinterpret_cast<volatile int*>(&odd[item & 3]) == (int)item + 1;
+                const int orow = s.first + node, h = it.g * a.per_kv + row % a.per_kv;
+                const TreeOut<bf16> out(a, orow, h);
+                const float inv = it.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+                float* piece = a.part + ((size_t)blockIdx.x * 2 + it.piece) * tree_piece_floats(a.block, a.vd);
+                for (int q = both ? slot : 0; q < chunks; q += both ? 2 : 1) {
+                    int v[32];
+                    tmem_ld(o0 + q * 32, v);
+                    tmem_wait_ld();
+                    float o[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] = __int_as_float(v[i]) * f0;
+                    if (other) {
+                        tmem_ld(o1 + q * 32, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = fmaf(__int_as_float(v[i]), f1, o[i]);
+                    }
+                    if (fix) {                        // warps agree on it
+                        // values of attended nodes that are not finite (they entered the product as zeros)
+                        const int k0 = it.tile * KT, k1 = min(s.len + s.n, k0 + it.n * KT);
+                        for (int k = max(k0, s.len); k < k1; k++) {
+                            if (!(tree_seen(a, s, node, k) & 1u)) continue;
+                            const bf16* val = static_cast<const bf16*>(a.seq.table[s.b].cache) + (size_t)k * a.ld + a.kv_heads * a.kd + it.g * a.vd + q * 32;
+#pragma unroll
+                            for (int i = 0; i < 32; i++) {
+                                const float x = q * 32 + i < a.vd ? to_f(val[i]) : 0.0f;
+                                if (!isfinite(x)) o[i] += x;
+                            }
+                        }
+                    }
+                    if (mine) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const int e = q * 32 + i;
+                            if (e < a.vd) {
+                                const float4 x = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                                if (it.whole) out.put4at(e, x);
+                                else put4(piece + 2 * a.block + ((size_t)(e / 4) * a.block + br) * 4, x);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (mine && !it.whole && (!both || slot == 0)) {
+                    piece[br] = m * a.scale2;
+                    piece[a.block + br] = l;
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty);
+            item++;
+        }
+    }
+    __syncwarp();
+    if (!ok && lane == 0) atomicExch(a.error_flag, DETB_ERR_WAIT_EXPIRED);
+    copies_wait<0>();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == PRODUCTS) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------------------ host side
+void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile) {
+    const bool wide = kd > 128 || vd > 128;
+    *block = wide || rows <= TT_ROWS ? TT_ROWS : 2 * TT_ROWS;
+    *tile = wide ? 64 : 128;
+}
+
+template <int SLOTS, int KT>
+static cudaError_t launch(const TreeArgs& a, cudaStream_t q) {
+    using Cfg = TtCfg<SLOTS, KT>;
+    static_assert(Cfg::PEND == 3 && KT % 32 == 0);
+    TtShape sh{};
+    sh.nkb = (a.kd + 63) / 64;
+    sh.nvb = (a.vd + 63) / 64;
+    sh.q_bytes = sh.nkb * TT_ROWS * 128;
+    sh.stage_bytes = std::max(sh.nkb, sh.nvb) * KT * 128;
+    sh.both = SLOTS == 2 && a.block == TT_ROWS;
+    const size_t fixed = (size_t)SLOTS * sh.q_bytes + sizeof(TtTables);
+    sh.stages = (int)std::min<size_t>(TT_STAGES, (TT_SMEM - fixed) / sh.stage_bytes);
+    const size_t smem = fixed + (size_t)sh.stages * sh.stage_bytes;
+    const cudaError_t e = cudaFuncSetAttribute(k_ftree_tc<SLOTS, KT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl_try(k_ftree_tc<SLOTS, KT>, dim3(a.ctas), dim3(Cfg::THREADS), smem, q, 1, a, sh);
+}
+
+cudaError_t ftree_tc_launch(const TreeArgs& a, cudaStream_t q) { return a.tile == 128 ? launch<2, 128>(a, q) : launch<1, 64>(a, q); }
+
+}  // namespace detb
