@@ -13,6 +13,9 @@ kernels that a profiler capture needs (a few hundred MB on the device, a handful
     python bench_kernel.py mingru [n M]                     # minimal gated recurrence, default 5120 512
     python bench_kernel.py moe [experts identity top ff n M]   # mixture of experts, default 64 8 6 2880 5120 512
     python bench_kernel.py seam [n M taps]                  # seam between sublayers, default 5120 512 4; taps 0: no convolution
+    python bench_kernel.py tree [heads kv dim vdim cached nodes seqs masked f32]   # step of drafted tokens, default 40 8 128 128 2048 1 1 0 0
+    python bench_kernel.py qkrope [heads kv dim vdim rot half rows f32]   # head norms, rotation, cache rows, default 40 8 128 128 128 1 512 0
+    python bench_kernel.py table [dims n scaling]           # rotation tables, default 128 262144 3
 
 attn: one det_attention call of M tokens behind pos0 cached positions (head_dim 256, random cache contents); tc = 0
 keeps it on the CUDA-core kernels; 2 warm-up calls, then 5 timed ones.
@@ -308,6 +311,83 @@ def seam(argv):
           f"device error word {d.det_last_error()}")
 
 
+def _tree_ref(d, rng, cap, ld, esize, cached, nodes, seqs):
+    caches = [_rand(d, rng, (cap, ld), 1.0, True) if esize == 2 else _rand(d, rng, (cap, ld)) for _ in range(seqs)]
+
+    def up(a):
+        p = d.det_malloc(a.nbytes)
+        d.det_memcpy(p, a.ctypes.data, a.nbytes, None)
+        d.det_sync()
+        return p
+    table = up(np.frombuffer(b"".join(bytes(capi.SeqSlot(cache=c)) for c in caches), np.uint8))
+    first, length = up((np.arange(seqs + 1) * nodes).astype(np.int32)), up(np.full(seqs, cached, np.int32))
+    return capi.TreeRef(table=table, first=first, len=length, seqs=seqs, rows=nodes * seqs, max_nodes=nodes, max_len=cached), up
+
+
+def tree(argv):
+    heads, kv, dim, vdim, cached, nodes, seqs, masked, f32 = (list(map(int, argv[1:])) + [40, 8, 128, 128, 2048, 1, 1, 0, 0][len(argv) - 1:])
+    d = capi.cuda()
+    assert d.det_init() == 0
+    rng, ev, esize = np.random.default_rng(1), _Events(d.det_cuda_stream()), 4 if f32 else 2
+    ld, cap = d.det_f_attn_ld(kv, dim, vdim), cached + nodes
+    ref, up = _tree_ref(d, rng, cap, ld, esize, cached, nodes, seqs)
+    ldq = d.det_f_attn_q_ld(heads, dim)
+    words = (nodes + 31) // 32
+    mask = None
+    if masked:                                       # a node's parent is the node half as far along
+        m = np.zeros((nodes, words), np.uint32)
+        for i in range(nodes):
+            if i:
+                m[i] = m[(i - 1) // 2]
+            m[i, i // 32] |= np.uint32(1 << (i % 32))
+        mask = up(np.tile(m, (seqs, 1)))
+    op = capi.FTreeOp(heads=heads, kv_heads=kv, dim=dim, vdim=vdim, scale=dim ** -0.5, cap=cap, dtype=capi.DET_F32 if f32 else capi.DET_BF16,
+                      q=_rand(d, rng, (nodes * seqs, ldq), 1.0, not f32), mask=mask, mask_ld=words, out=d.det_malloc(4 * nodes * seqs * heads * vdim),
+                      ldo=heads * vdim, scratch=d.det_malloc(d.det_f_tree_scratch_bytes(heads, kv, vdim, nodes)), seq=ref)
+
+    def call():
+        assert d.det_f_tree_attn(C.byref(op), None) == 0
+    us = _time(ev, call)
+    pairs = nodes * cached + (nodes * (nodes + 1) // 2 if not masked else nodes)
+    flops, nbytes = 2 * seqs * pairs * heads * (dim + vdim), esize * seqs * ((cached + nodes) * ld + nodes * heads * (dim + vdim))
+    print(f"det_f_tree_attn {heads}/{kv} x {dim}/{vdim}, {seqs} x {nodes} rows behind {cached}: {us:.2f} us, {nbytes / us / 1e3:.0f} GB/s, "
+          f"{flops / us / 1e6:.1f} TFLOP/s; device error word {d.det_last_error()}")
+
+
+def qkrope(argv):
+    heads, kv, dim, vdim, rot, half, rows, f32 = (list(map(int, argv[1:])) + [40, 8, 128, 128, 128, 1, 512, 0][len(argv) - 1:])
+    d = capi.cuda()
+    assert d.det_init() == 0
+    rng, ev, esize = np.random.default_rng(1), _Events(d.det_cuda_stream()), 4 if f32 else 2
+    ld, width = d.det_f_attn_ld(kv, dim, vdim), heads * dim + kv * (dim + vdim)
+    ref, _ = _tree_ref(d, rng, rows, ld, esize, 0, rows, 1)
+    op = capi.FQkOp(heads=heads, kv_heads=kv, dim=dim, vdim=vdim, rot_dims=rot, half=half, eps=1e-6, q_norm=_rand(d, rng, (dim,)), k_norm=_rand(d, rng, (dim,)),
+                    cap=rows, dtype=capi.DET_F32 if f32 else capi.DET_BF16, y=_rand(d, rng, (rows, width)), ldy=width, q_off=0, k_off=heads * dim,
+                    v_off=(heads + kv) * dim, rope_len=rows, rope_cos=_rand(d, rng, (rows, rot // 2)), rope_sin=_rand(d, rng, (rows, rot // 2)),
+                    q=d.det_malloc(4 * rows * d.det_f_attn_q_ld(heads, dim)), seq=ref)
+
+    def call():
+        assert d.det_f_qk_rope(C.byref(op), None) == 0
+    us = _time(ev, call)
+    nbytes = rows * (4 * width + 4 * rot + esize * (d.det_f_attn_q_ld(heads, dim) + ld))
+    print(f"det_f_qk_rope {heads}/{kv} x {dim}/{vdim}, {rot} rotated, {rows} rows: {us:.2f} us, {nbytes / us / 1e3:.0f} GB/s; "
+          f"device error word {d.det_last_error()}")
+
+
+def table(argv):
+    dims, n, scaling = (list(map(int, argv[1:])) + [128, 262144, 3][len(argv) - 1:])
+    d = capi.cuda()
+    assert d.det_init() == 0
+    ev = _Events(d.det_cuda_stream())
+    op = capi.FRopeOp(dims=dims, scaling=scaling, base=1e6, factor=8.0, orig_ctx=32768.0, low=1.0, high=32.0, mscale=1.0, n=n,
+                      cos=d.det_malloc(2 * dims * n), sin=d.det_malloc(2 * dims * n))
+
+    def call():
+        assert d.det_f_rope_table(C.byref(op), None) == 0
+    us = _time(ev, call)
+    print(f"det_f_rope_table {n} x {dims}: {us:.2f} us, {4 * dims * n / us / 1e3:.0f} GB/s; device error word {d.det_last_error()}")
+
+
 def main(argv):
     kind = argv[0] if argv else "gemv"
     if kind == "umma_peak":
@@ -345,7 +425,8 @@ def main(argv):
         return
     if kind == "attn":
         return attn(argv)
-    cases = {"fgemm": fgemm, "recur": recur, "latent": latent, "fattn": fattn, "mingru": mingru, "moe": moe, "seam": seam}
+    cases = {"fgemm": fgemm, "recur": recur, "latent": latent, "fattn": fattn, "mingru": mingru, "moe": moe, "seam": seam, "tree": tree, "qkrope": qkrope,
+             "table": table}
     if kind in cases:
         return cases[kind](argv)
     if kind not in ("gemv", "gemm_tc"):

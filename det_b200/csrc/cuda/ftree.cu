@@ -207,33 +207,33 @@ __global__ void __launch_bounds__(TM_THREADS) k_ftree_merge(const TreeArgs a) {
         before += __shfl_xor_sync(FULL, before, off);
     }
     total *= a.kv_heads;
-    const int ctas = tree_ctas(a, total);
-    const long long u0 = before * a.kv_heads + (long long)g * s.tiles, u1 = u0 + s.tiles - 1;
-    int c0 = (int)(u0 * ctas / total), c1 = (int)(u1 * ctas / total);
-    while (c0 + 1 < ctas && tree_bound(total, ctas, c0 + 1) <= u0) c0++;
-    while (c0 > 0 && tree_bound(total, ctas, c0) > u0) c0--;
-    while (c1 + 1 < ctas && tree_bound(total, ctas, c1 + 1) <= u1) c1++;
-    while (c1 > 0 && tree_bound(total, ctas, c1) > u1) c1--;
-    if (c0 == c1) return;
+    const long long share = tree_share(a, total), u0 = before * a.kv_heads + (long long)g * s.tiles, left = u0 % share;
+    const int c0 = (int)(u0 / share), n = (int)((left + s.tiles + share - 1) / share);      // the first CTA, and how many
+    if (n == 1) return;
     const size_t size = tree_piece_floats(a.block, a.vd);
-    const float* head = a.part + ((size_t)c0 * 2 + (tree_bound(total, ctas, c0) == u0 ? 0 : 1)) * size;   // the others are their CTAs' first
+    const float* head = a.part + ((size_t)c0 * 2 + (left ? 1 : 0)) * size;    // the others are their CTAs' first pieces
+    const float* rest = a.part + (size_t)(c0 + 1) * 2 * size;
     const int vq = a.vd / 4;
     for (int i = chunk * TM_THREADS + threadIdx.x; i < s.rows * vq; i += chunks * TM_THREADS) {
         const int v = i / s.rows, r = i - v * s.rows;
         float m = head[r];
-        for (int c = c0 + 1; c <= c1; c++) m = fmaxf(m, a.part[(size_t)c * 2 * size + r]);
+#pragma unroll 8
+        for (int c = 0; c < n - 1; c++) m = fmaxf(m, rest[(size_t)c * 2 * size + r]);
         const float base = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f;
-        float4 o = make_float4(0, 0, 0, 0);
-        for (int c = c0; c <= c1; c++) {
-            const float* p = c == c0 ? head : a.part + (size_t)c * 2 * size;
-            const float f = exp2f(p[r] - base);
-            const float4 x = load4(p + 2 * a.block + ((size_t)v * a.block + r) * 4);
-            l = fmaf(f, p[a.block + r], l);
-            o.x = fmaf(f, x.x, o.x);
-            o.y = fmaf(f, x.y, o.y);
-            o.z = fmaf(f, x.z, o.z);
-            o.w = fmaf(f, x.w, o.w);
+        const float f = exp2f(head[r] - base);
+        float l = f * head[a.block + r];
+        const size_t at = 2 * a.block + ((size_t)v * a.block + r) * 4;
+        float4 o = scaled4(load4(head + at), f);
+#pragma unroll 4
+        for (int c = 0; c < n - 1; c++) {
+            const float* p = rest + (size_t)c * 2 * size;
+            const float w = exp2f(p[r] - base);
+            const float4 x = load4(p + at);
+            l = fmaf(w, p[a.block + r], l);
+            o.x = fmaf(w, x.x, o.x);
+            o.y = fmaf(w, x.y, o.y);
+            o.z = fmaf(w, x.z, o.z);
+            o.w = fmaf(w, x.w, o.w);
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const int row = s.r0 + r;
@@ -291,7 +291,7 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     DETB_TAKE(!op->vrope_cos == !op->vrope_sin && (!op->vrope_cos || (op->vdim % 2 == 0 && op->pos && op->rope_len > 0)), "bad rotation of the values");
     if (const char* why = bad_ref(op->seq)) return refuse(name, why);
     const long long rows = (long long)op->seq.max_nodes * (op->heads / op->kv_heads);
-    DETB_TAKE(rows <= 1 << 24, "too many rows");
+    DETB_TAKE(rows <= 1 << 24 && rows * (op->heads / op->kv_heads) < 1ll << 32, "too many rows");
     DETB_TAKE(!op->mask || (op->seq.max_nodes <= DET_MAX_TREE && op->mask_ld * 32ll >= op->seq.max_nodes), "the mask is too small");
     DETB_TAKE(op->ldo >= op->heads * op->vdim && (!op->gate || op->ldg >= op->heads), "rows overlap");
     if (op->seq.rows == 0 || op->seq.seqs == 0 || rows == 0) return 0;
@@ -303,7 +303,8 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     const long long blocks = (rows + a.block - 1) / a.block;
     DETB_TAKE(blocks * op->seq.seqs <= 65535, "too many rows");
     DETB_TAKE(runtime_ready(), "no usable device");
-    a.heads = op->heads; a.kv_heads = op->kv_heads; a.per_kv = op->heads / op->kv_heads; a.dim = op->dim; a.vdim = op->vdim;
+    a.heads = op->heads; a.kv_heads = op->kv_heads; a.per_kv = op->heads / op->kv_heads;
+    a.per_magic = ((1ull << 32) + a.per_kv - 1) / a.per_kv; a.dim = op->dim; a.vdim = op->vdim;
     a.ld = det_f_attn_ld(op->kv_heads, op->dim, op->vdim);
     a.ldq = det_f_attn_q_ld(op->heads, op->dim);
     a.scale2 = op->scale * 1.4426950408889634f;

@@ -50,7 +50,7 @@ __device__ __forceinline__ TreePlace tree_place(const det_tree_ref& s, int row, 
 // ------------------------------------------------------------------------------------------------------ attention
 // The query rows of a sequence and key/value head are (node, query head of the group) pairs, node first, in blocks of `block` rows;
 // its keys come in tiles.  The tiles of all (sequence, row block, key/value head) segments, in that order, are dealt out evenly: CTA
-// c takes the tiles bound(c) .. bound(c + 1), whatever segments they belong to, so unequal lengths leave no CTA idle.  A segment that
+// c takes `share` tiles from c * share on, whatever segments they belong to, so unequal lengths leave no CTA idle.  A segment that
 // falls to one CTA is finished there; of the others every CTA leaves a piece (maximum, sum, values per row) in scratch, and the
 // merge kernel adds the pieces in order of the keys.  A CTA has at most two such pieces, of its first and of its last segment.
 constexpr int TREE_CTAS = 148;
@@ -58,6 +58,7 @@ constexpr int TREE_SHARE = 2;      // tiles of a CTA at least, if there are enou
 
 struct TreeArgs {
     int heads, kv_heads, per_kv, dim, vdim, kd, vd, ld, ldq;
+    unsigned long long per_magic;  // row / per_kv = row * per_magic >> 32, as row * per_kv < 2^32
     float scale2;                  // scale * log2(e)
     int cap;
     const void* q;
@@ -102,38 +103,36 @@ __device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, int seg) {
     s.tiles = s.rows > 0 ? (s.keys + a.tile - 1) / a.tile : 0;
     return s;
 }
+// Tiles of a CTA.
+__device__ __forceinline__ long long tree_share(const TreeArgs& a, long long total) {
+    return max((long long)TREE_SHARE, (total + a.ctas - 1) / a.ctas);
+}
 // Where a CTA's share begins and how long it is.  tree_start is called by a whole warp; every lane gets the result.
 struct TreeShare {
     int seg, g, tile;              // segment, key/value head, tile within them
     long long left;                // tiles of the share
 };
-__device__ __forceinline__ int tree_ctas(const TreeArgs& a, long long total) {
-    return (int)max(1ll, min((long long)a.ctas, total / TREE_SHARE));
-}
-__device__ __forceinline__ long long tree_bound(long long total, int ctas, int c) { return c >= ctas ? total : total * c / ctas; }
-__device__ __forceinline__ long long tree_total(const TreeArgs& a, int lane, bool report) {
-    long long t = 0;
+__device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int lane) {
+    const int segs = a.seq.seqs * a.blocks;
+    long long total = 0;
+    int mine = 0;                                             // tiles of the lane's last segment
     bool bad = false;
-    for (int i = lane; i < a.seq.seqs * a.blocks; i += 32) {
+    for (int i = lane; i < segs; i += 32) {
         const TreeSeg s = tree_seg(a, i);
-        t += s.tiles;
+        total += mine = s.tiles;
         bad |= s.bad;
     }
-    if (report && bad) report_size(a.error_flag);
+    if (cta == 0 && bad) report_size(a.error_flag);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) t += __shfl_xor_sync(FULL, t, off);
-    return t * a.kv_heads;
-}
-__device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int lane) {
-    const long long total = tree_total(a, lane, cta == 0);
-    const int ctas = tree_ctas(a, total);
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(FULL, total, off);
+    total *= a.kv_heads;
+    const long long share = tree_share(a, total), u0 = cta * share;
     TreeShare w{0, 0, 0, 0};
-    if (cta >= ctas || total == 0) return w;
-    const long long u0 = tree_bound(total, ctas, cta);
-    w.left = tree_bound(total, ctas, cta + 1) - u0;
+    if (u0 >= total) return w;
+    w.left = min(share, total - u0);
     long long base = 0;                                       // tiles ahead of this round's segments
     for (int i = lane;; i += 32) {
-        const int tiles = i < a.seq.seqs * a.blocks ? tree_seg(a, i).tiles : 0;
+        const int tiles = i >= segs ? 0 : segs <= 32 ? mine : tree_seg(a, i).tiles;
         long long sum = (long long)tiles * a.kv_heads;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -142,12 +141,12 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
         }
         const unsigned holds = __ballot_sync(FULL, base + sum > u0);
         if (holds) {
-            const int src = __ffs(holds) - 1;
-            const long long before = __shfl_sync(FULL, base + sum - (long long)tiles * a.kv_heads, src);
-            const int per = __shfl_sync(FULL, tiles, src);
+            const int src = __ffs(holds) - 1, per = __shfl_sync(FULL, tiles, src);
+            // tiles of the segment ahead of the share: below kv_heads * per, which fits 31 bits (per < 2^19, kv_heads <= 2^12)
+            const unsigned in = (unsigned)(u0 - __shfl_sync(FULL, base + sum - (long long)tiles * a.kv_heads, src));
             w.seg = i - lane + src;
-            w.g = (int)((u0 - before) / per);
-            w.tile = (int)((u0 - before) % per);
+            w.g = (int)(in / (unsigned)per);
+            w.tile = (int)(in % (unsigned)per);
             return w;
         }
         base += __shfl_sync(FULL, sum, 31);

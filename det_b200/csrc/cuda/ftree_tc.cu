@@ -89,49 +89,78 @@ __device__ __forceinline__ float ex2(float x) {      // relative error about 2^-
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes) {      // what is missing of 16 bytes becomes zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Rows of 16-byte pieces into swizzled blocks of `rows` rows x 128 bytes; pieces past `real` and rows past `have` become zeros.
-// row_of(r): address of row r.
-template <class F>
-__device__ __forceinline__ void tt_copy(unsigned dst, int rows, int pieces, int real, int have, int tid, F row_of) {
-    const int dr = TT_COPY / pieces, dc = TT_COPY - dr * pieces;
-    int r = tid / pieces, c = tid - r * pieces;
-    const int total = rows * pieces;
-    for (int i = tid; i < total; i += TT_COPY) {
-        const bool ok = c < real && r < have;
-        copy16(dst + (unsigned)((c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4)), ok ? row_of(r) + c * 8 : row_of(0), ok);
-        r += dr;
-        c += dc;
-        if (c >= pieces) {
-            c -= pieces;
-            r++;
+// One warp's part of a tile: rows of `pieces` 16-byte pieces, `ldb` bytes apart, into swizzled blocks of `rows` rows x 128 bytes.  LANES
+// lanes take the pieces of a row, so a lane keeps its piece and the swizzle of its rows repeats every 8: an address is one addition.
+// Pieces past `real` become zeros, as do rows past `have` (`zero`; else they keep what is there).
+template <int LANES>
+__device__ __forceinline__ void tt_copy(unsigned dst, const char* src, size_t ldb, int rows, int pieces, int real, int have, bool zero, int warp, int lane) {
+    constexpr int AT_ONCE = 32 / LANES, J = 8 / AT_ONCE;
+    const int c = lane % LANES, rr = lane / LANES;
+    if (c >= pieces) return;
+    const int bytes = c < real ? 16 : 0;
+    unsigned to[J];
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int r = j * AT_ONCE + rr;
+        to[j] = dst + (unsigned)((c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4)) + warp * 1024;
+    }
+    const char* first = src;
+    src += (size_t)(warp * 8 + rr) * ldb + (bytes ? c * 16 : 0);
+    const size_t step = (size_t)AT_ONCE * ldb, skip = (size_t)(TT_COPY / 4 - 8) * ldb;
+    const int end = zero ? rows : min(rows, have);
+    for (int r = warp * 8; r < end; r += TT_COPY / 4) {
+        if (r + 8 <= have) {
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                copy16(to[j], src, bytes);
+                src += step;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const bool in = r + j * AT_ONCE + rr < have;
+                if (in || zero) copy16(to[j], in ? src : first, in ? bytes : 0);
+                src += step;
+            }
         }
+        src += skip;
+#pragma unroll
+        for (int j = 0; j < J; j++) to[j] += (TT_COPY / 4) * 128;
     }
 }
-// Values of the tree that are not finite become zeros in the staged tile; true when there were any.  A thread looks at its own copies.
-__device__ __forceinline__ bool tt_clean(uint8_t* tile, int rows, int pieces, int tid) {
+__device__ __forceinline__ void tt_tile(unsigned dst, const bf16* src, size_t ldb, int rows, int pieces, int real, int have, bool zero, int warp, int lane) {
+    const char* p = reinterpret_cast<const char*>(src);
+    if (pieces <= 8) tt_copy<8>(dst, p, ldb, rows, pieces, real, have, zero, warp, lane);
+    else if (pieces <= 16) tt_copy<16>(dst, p, ldb, rows, pieces, real, have, zero, warp, lane);
+    else tt_copy<32>(dst, p, ldb, rows, pieces, real, have, zero, warp, lane);
+}
+// Values of the tree that are not finite become zeros in the staged tile; true when there were any.  A lane looks at its own copies.
+__device__ __forceinline__ bool tt_clean(uint8_t* tile, int rows, int pieces, int warp, int lane) {
+    const int lanes = pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32, c = lane % lanes;
     bool odd = false;
-    for (int i = tid; i < rows * pieces; i += TT_COPY) {
-        const int r = i / pieces, c = i - r * pieces;
-        uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4));
-        uint4 v = *p;
-        unsigned w[4] = {v.x, v.y, v.z, v.w};
-        bool hit = false;
+    if (c < pieces)
+        for (int r0 = warp * 8; r0 < rows; r0 += TT_COPY / 4)
+            for (int r = r0 + lane / lanes; r < r0 + 8; r += 32 / lanes) {
+                uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4));
+                const uint4 v = *p;
+                unsigned w[4] = {v.x, v.y, v.z, v.w};
+                bool hit = false;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, hit = true;
-            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, hit = true;
-        }
-        if (hit) *p = make_uint4(w[0], w[1], w[2], w[3]);
-        odd |= hit;
-    }
+                for (int j = 0; j < 4; j++) {
+                    if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, hit = true;
+                    if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, hit = true;
+                }
+                if (hit) *p = make_uint4(w[0], w[1], w[2], w[3]);
+                odd |= hit;
+            }
     return odd;
 }
 
@@ -190,7 +219,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
 
     if (warp >= SOFT && warp < PRODUCTS) {
         // ---- copies
-        const int tid = threadIdx.x - SOFT * 32;
+        const int cw = warp - SOFT;
         const int kp = (a.kd + 15) / 16 * 2, vp = (a.vd + 15) / 16 * 2;
         // a copy in flight: stage, and whether it begins a stretch (1), holds values of a tree (2), the stretch (from bit 2)
         int st[Cfg::PEND], what[Cfg::PEND];
@@ -200,7 +229,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
         auto land = [&](int s, int w) {
             if (s < 0) return;
             if (w & 2) {
-                if (tt_clean(ring + (size_t)s * sh.stage_bytes, KT, vp, tid)) *reinterpret_cast<volatile int*>(&odd[(w >> 2) & 3]) = (w >> 2) + 1;
+                if (tt_clean(ring + (size_t)s * sh.stage_bytes, KT, vp, cw, lane)) *reinterpret_cast<volatile int*>(&odd[(w >> 2) & 3]) = (w >> 2) + 1;
             }
             fence_async();
             __syncwarp();
@@ -225,25 +254,25 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
             if (!both) flush();                      // the wait below needs what is in flight
             if (item >= (both ? 2u : 1u)) ok = wait(&q_empty[qb], ((both ? item >> 1 : item) & 1u) ^ 1u);
             if (!ok) break;
+            // query rows: a row per LANES lanes; rows that are not there keep what is there (a row's scores are its own)
             const bf16* q = static_cast<const bf16*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
-            auto q_row = [&](int r) {
-                const int row = s.r0 + r;
-                return q + (size_t)(row / a.per_kv) * a.ldq + (row % a.per_kv) * a.kd;
-            };
-            for (int slot = 0; slot < (both ? 1 : SLOTS); slot++) {
-                const int r0 = slot * TT_ROWS;
-                if (slot && s.rows <= r0) break;
-                tt_copy(smem_addr(Qs + (size_t)(both ? qb : slot) * sh.q_bytes), TT_ROWS, kp, a.kd / 8, s.rows - r0, tid,
-                        [&](int r) { return q_row(r0 + r); });
-            }
+            const int lanes = kp <= 8 ? 8 : kp <= 16 ? 16 : 32, qc = lane % lanes, qstep = TT_COPY / lanes;
+            if (qc < kp)
+                for (int r = (cw * 32 + lane) / lanes; r < s.rows; r += qstep) {
+                    const int row = s.r0 + r, node = (int)(row * a.per_magic >> 32), x = r & (TT_ROWS - 1);
+                    const bf16* src = q + (size_t)node * a.ldq + (row - node * a.per_kv) * a.kd;
+                    copy16(smem_addr(Qs + (size_t)(both ? qb : r / TT_ROWS) * sh.q_bytes) + (unsigned)((qc >> 3) * TT_ROWS * 128 + x * 128 + (((qc ^ x) & 7) << 4)),
+                           qc * 8 < a.kd ? src + qc * 8 : src, qc * 8 < a.kd ? 16 : 0);
+                }
             auto fetch = [&](bool value, int t) {
                 const unsigned sn = c % sh.stages;
                 if (c >= (unsigned)sh.stages) ok = wait(&empty[sn], ((c / sh.stages) & 1u) ^ 1u);
                 if (!ok) return;
                 const int k0 = (it.tile + t) * KT;
                 const bf16* rows = cache + (size_t)k0 * a.ld + (value ? a.kv_heads * a.kd + it.g * a.vd : it.g * a.kd);
-                tt_copy(smem_addr(ring + (size_t)sn * sh.stage_bytes), KT, value ? vp : kp, (value ? a.vd : a.kd) / 8, s.len + s.n - k0, tid,
-                        [&](int r) { return rows + (size_t)r * a.ld; });
+                // rows behind the last key: zeros for values (their weights are zero), anything for keys (their scores are masked)
+                tt_tile(smem_addr(ring + (size_t)sn * sh.stage_bytes), rows, (size_t)a.ld * 2, KT, value ? vp : kp, (value ? a.vd : a.kd) / 8,
+                        s.len + s.n - k0, value, cw, lane);
                 copies_commit();
                 copies_wait<Cfg::PEND>();
                 land(st[Cfg::PEND - 1], what[Cfg::PEND - 1]);
@@ -364,7 +393,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 if (any) {
                     const int k0 = (it.tile + (both ? 2 * j + slot : j)) * KT;
                     const bool tree = k0 + KT > s.len;
-                    float mt = -INFINITY;
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     unsigned seen[KT / 32];
 #pragma unroll
                     for (int q = 0; q < KT / 32; q++) {
@@ -374,12 +403,13 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                         tmem_wait_ld();
                         if (tree) {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) mt = fmaxf(mt, (seen[q] >> i) & 1u ? __int_as_float(v[i]) : -INFINITY);
+                            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], (seen[q] >> i) & 1u ? __int_as_float(v[i]) : -INFINITY);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) mt = fmaxf(mt, __int_as_float(v[i]));
+                            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __int_as_float(v[i]));
                         }
                     }
+                    const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                     const bool grow = (mt - m) * a.scale2 > TT_GROWTH;
                     if (__any_sync(FULL, grow)) {
                         const float f = grow ? ex2((m - mt) * a.scale2) : 1.0f;
