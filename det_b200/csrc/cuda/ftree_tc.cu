@@ -89,6 +89,35 @@ __device__ __forceinline__ float ex2(float x) {      // relative error about 2^-
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two neighbouring fp32 values in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(r) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&r);
+}
+// Waits for the loads of TMEM; what they brought is not used before.
+__device__ __forceinline__ void tmem_landed(int (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                   "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_landed(int (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes) {      // what is missing of 16 bytes becomes zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -162,6 +191,48 @@ __device__ __forceinline__ bool tt_clean(uint8_t* tile, int rows, int pieces, in
                 odd |= hit;
             }
     return odd;
+}
+
+// The largest of a row's scores in the KT columns from `ts` on; MASKED: of those it sees.
+template <int KT, bool MASKED>
+__device__ __forceinline__ float tt_max(const TreeArgs& a, const TreeSeg& s, unsigned ts, int node, int k0) {
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+    for (int q = 0; q < KT / 32; q++) {
+        int v[32];
+        tmem_ld(ts + q * 32, v);
+        const unsigned seen = MASKED ? tree_seen(a, s, node, k0 + q * 32) : FULL;
+        __syncwarp();
+        tmem_landed(v);
+#pragma unroll
+        for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], !MASKED || (seen >> i) & 1u ? __int_as_float(v[i]) : -INFINITY);
+    }
+    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+// The row's weights 2^(score * scale + base) in place of its scores; returns their sum.
+template <int KT, bool MASKED>
+__device__ __forceinline__ float tt_weights(const TreeArgs& a, const TreeSeg& s, unsigned ts, int node, int k0, float base) {
+    const float2 scale = make_float2(a.scale2, a.scale2), off = make_float2(base, base);
+    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll 1
+    for (int q = 0; q < KT / 32; q++) {
+        int v[32];
+        tmem_ld(ts + q * 32, v);
+        const unsigned seen = MASKED ? tree_seen(a, s, node, k0 + q * 32) : FULL;
+        __syncwarp();
+        tmem_landed(v);
+        unsigned w[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float2 x = fma2(make_float2(__int_as_float(v[i]), __int_as_float(v[i + 1])), scale, off);
+            float2 p = make_float2(ex2(x.x), ex2(x.y));
+            if (MASKED) p = make_float2((seen >> i) & 1u ? p.x : 0.0f, (seen >> (i + 1)) & 1u ? p.y : 0.0f);
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], p);
+            w[i / 2] = pack_bf(p.x, p.y);
+        }
+        tmem_st(ts + q * 16, w);
+    }
+    return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
 
 template <int SLOTS, int KT>
@@ -375,7 +446,6 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
         const int slot = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const unsigned lanes = (unsigned)(quarter * 32) << 16;
         const unsigned ts = tmem + lanes + slot * KT, to = tmem + lanes + Cfg::O_COL + slot * (256 / SLOTS);
-        const int chunks = (a.vd + 31) / 32;
         unsigned ns = 0;                             // scores taken
         // after an expired wait the stretches are gone through without waiting, so that all warps meet at the barrier below
         while (tree_next(a, walk, it)) {
@@ -393,23 +463,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 if (any) {
                     const int k0 = (it.tile + (both ? 2 * j + slot : j)) * KT;
                     const bool tree = k0 + KT > s.len;
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    unsigned seen[KT / 32];
-#pragma unroll
-                    for (int q = 0; q < KT / 32; q++) {
-                        seen[q] = tree ? tree_seen(a, s, node, k0 + q * 32) : FULL;
-                        int v[32];
-                        tmem_ld(ts + q * 32, v);
-                        tmem_wait_ld();
-                        if (tree) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], (seen[q] >> i) & 1u ? __int_as_float(v[i]) : -INFINITY);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __int_as_float(v[i]));
-                        }
-                    }
-                    const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const float mt = tree ? tt_max<KT, true>(a, s, ts, node, k0) : tt_max<KT, false>(a, s, ts, node, k0);
                     const bool grow = (mt - m) * a.scale2 > TT_GROWTH;
                     if (__any_sync(FULL, grow)) {
                         const float f = grow ? ex2((m - mt) * a.scale2) : 1.0f;
@@ -417,42 +471,20 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                         l *= f;
                         __syncwarp();
                         if (j > 0) {
-                            for (int q = 0; q < chunks; q++) {
-                                int v[32];
-                                tmem_ld(to + q * 32, v);
-                                tmem_wait_ld();
+#pragma unroll 1
+                            for (int q = 0; q < a.vd; q += 16) {
+                                int v[16];
+                                tmem_ld(to + q, v);
+                                tmem_landed(v);
                                 unsigned w[16];
 #pragma unroll
-                                for (int h = 0; h < 2; h++) {
-#pragma unroll
-                                    for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__int_as_float(v[h * 16 + i]) * f);
-                                    tmem_st(to + q * 32 + h * 16, w);
-                                }
+                                for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__int_as_float(v[i]) * f);
+                                tmem_st(to + q, w);
                             }
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : -m * a.scale2;
-                    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int q = 0; q < KT / 32; q++) {
-                        int v[32];
-                        tmem_ld(ts + q * 32, v);
-                        tmem_wait_ld();
-                        unsigned w[16];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            float p0 = ex2(fmaf(__int_as_float(v[i]), a.scale2, base)), p1 = ex2(fmaf(__int_as_float(v[i + 1]), a.scale2, base));
-                            if (tree) {
-                                p0 = (seen[q] >> i) & 1u ? p0 : 0.0f;
-                                p1 = (seen[q] >> (i + 1)) & 1u ? p1 : 0.0f;
-                            }
-                            part[i & 2] += p0;
-                            part[(i & 2) + 1] += p1;
-                            w[i / 2] = pack_bf(p0, p1);
-                        }
-                        tmem_st(ts + q * 16, w);
-                    }
-                    l += (part[0] + part[1]) + (part[2] + part[3]);
+                    l += tree ? tt_weights<KT, true>(a, s, ts, node, k0, base) : tt_weights<KT, false>(a, s, ts, node, k0, base);
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -483,42 +515,41 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 const TreeOut<bf16> out(a, orow, h);
                 const float inv = it.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
                 float* piece = a.part + ((size_t)blockIdx.x * 2 + it.piece) * tree_piece_floats(a.block, a.vd);
-                for (int q = both ? slot : 0; q < chunks; q += both ? 2 : 1) {
-                    int v[32];
-                    tmem_ld(o0 + q * 32, v);
-                    tmem_wait_ld();
-                    float o[32];
+#pragma unroll 1
+                for (int q = both ? slot * 16 : 0; q < a.vd; q += both ? 32 : 16) {
+                    int v[16];
+                    tmem_ld(o0 + q, v);
+                    tmem_landed(v);
+                    float o[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = __int_as_float(v[i]) * f0;
+                    for (int i = 0; i < 16; i++) o[i] = __int_as_float(v[i]) * f0;
                     if (other) {
-                        tmem_ld(o1 + q * 32, v);
-                        tmem_wait_ld();
+                        tmem_ld(o1 + q, v);
+                        tmem_landed(v);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = fmaf(__int_as_float(v[i]), f1, o[i]);
+                        for (int i = 0; i < 16; i++) o[i] = fmaf(__int_as_float(v[i]), f1, o[i]);
                     }
                     if (fix) {                        // warps agree on it
                         // values of attended nodes that are not finite (they entered the product as zeros)
                         const int k0 = it.tile * KT, k1 = min(s.len + s.n, k0 + it.n * KT);
                         for (int k = max(k0, s.len); k < k1; k++) {
                             if (!(tree_seen(a, s, node, k) & 1u)) continue;
-                            const bf16* val = static_cast<const bf16*>(a.seq.table[s.b].cache) + (size_t)k * a.ld + a.kv_heads * a.kd + it.g * a.vd + q * 32;
+                            const bf16* val = static_cast<const bf16*>(a.seq.table[s.b].cache) + (size_t)k * a.ld + a.kv_heads * a.kd + it.g * a.vd + q;
 #pragma unroll
-                            for (int i = 0; i < 32; i++) {
-                                const float x = q * 32 + i < a.vd ? to_f(val[i]) : 0.0f;
+                            for (int i = 0; i < 16; i++) {
+                                const float x = q + i < a.vd ? to_f(val[i]) : 0.0f;
                                 if (!isfinite(x)) o[i] += x;
                             }
                         }
                     }
                     if (mine) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const int e = q * 32 + i;
-                            if (e < a.vd) {
+                        for (int i = 0; i < 16; i += 4)
+                            if (q + i < a.vd) {
                                 const float4 x = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
-                                if (it.whole) out.put4at(e, x);
-                                else put4(piece + 2 * a.block + ((size_t)(e / 4) * a.block + br) * 4, x);
+                                if (it.whole) out.put4at(q + i, x);
+                                else put4(piece + 2 * a.block + ((size_t)((q + i) / 4) * a.block + br) * 4, x);
                             }
-                        }
                     }
                     __syncwarp();
                 }
