@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
         }
         for (int t = it.tile; t < it.tile + it.n; t++) {
             const int k0 = t * TS_KEYS, last = s.len + s.n;
-            const bool tree = k0 + TS_KEYS > s.len;
+            const bool tree = k0 + TS_KEYS > s.edge;
             __syncthreads();
             const float* kp = cache + (size_t)k0 * a.ld + it.g * a.kd;
             for (int i = tid; i < TS_KEYS * (a.kd / 4); i += TS_THREADS) {
@@ -277,7 +277,7 @@ size_t det_f_tree_scratch_bytes(int heads, int kv_heads, int vdim, int max_nodes
     simt_shape(rows, &block, &tile);
     ftree_tc_shape(rows, 8, vd, &other, &tile);      // the smallest keys have the largest blocks
     block = std::max(block, other);
-    return TREE_CTAS * 2 * tree_piece_floats(block, vd) * sizeof(float);
+    return TREE_MAP_BYTES + TREE_CTAS * 2 * tree_piece_floats(block, vd) * sizeof(float);
 }
 
 int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
@@ -295,7 +295,8 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     DETB_TAKE(!op->mask || (op->seq.max_nodes <= DET_MAX_TREE && op->mask_ld * 32ll >= op->seq.max_nodes), "the mask is too small");
     DETB_TAKE(op->ldo >= op->heads * op->vdim && (!op->gate || op->ldg >= op->heads), "rows overlap");
     if (op->seq.rows == 0 || op->seq.seqs == 0 || rows == 0) return 0;
-    DETB_TAKE(op->q && op->out && op->scratch && aligned16(op->q) && aligned16(op->scratch), "q, out or scratch is NULL or misaligned");
+    DETB_TAKE(op->q && op->out && op->scratch && aligned16(op->q) && reinterpret_cast<uintptr_t>(op->scratch) % 128 == 0,
+              "q, out or scratch is NULL or misaligned");
     TreeArgs a{};
     a.kd = round8(op->dim); a.vd = round8(op->vdim);
     if (op->dtype == DET_BF16) ftree_tc_shape((int)rows, a.kd, a.vd, &a.block, &a.tile);
@@ -310,7 +311,8 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     a.scale2 = op->scale * 1.4426950408889634f;
     a.cap = op->cap; a.q = op->q; a.mask = op->mask; a.mask_ld = op->mask_ld; a.gate = op->gate; a.ldg = op->ldg; a.pos = op->pos;
     a.rope_len = op->rope_len; a.vcs = op->vrope_cos; a.vsn = op->vrope_sin; a.out = op->out; a.ldo = op->ldo;
-    a.part = static_cast<float*>(op->scratch);
+    a.maps = op->scratch;
+    a.part = reinterpret_cast<float*>(static_cast<char*>(op->scratch) + TREE_MAP_BYTES);
     a.error_flag = error_word();
     a.blocks = (int)blocks;
     a.seq = op->seq;

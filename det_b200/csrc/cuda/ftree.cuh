@@ -73,17 +73,21 @@ struct TreeArgs {
     void* out;
     int ldo;
     float* part;                   // [CTA][2] pieces of tree_piece_floats(block, vd)
+    void* maps;                    // [CTA][TREE_MAPS][2] tensor maps
     int* error_flag;
     int block, tile, blocks;       // rows of a block, keys of a tile, row blocks of the largest tree
     int ctas;
     det_tree_ref seq;
 };
+constexpr int TREE_MAPS = 8;
+constexpr size_t TREE_MAP_BYTES = (size_t)TREE_CTAS * TREE_MAPS * 2 * 128;
 // A piece: m[block] | l[block] | o[vd / 4][block][4].
 __host__ __device__ constexpr size_t tree_piece_floats(int block, int vd) { return (size_t)block * (2 + vd); }
 
 struct TreeSeg {
     int b, r0, rows;               // sequence, first row of the block, its rows
     int first, n, len, keys;       // first row of the step, nodes, cached rows, keys that some row of the block may see
+    int edge;                      // keys that every row of the block sees
     int tiles;                     // 0: nothing to do (a sequence that does not fit is left out)
     bool bad;
 };
@@ -100,6 +104,7 @@ __device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, int seg) {
     s.rows = min(a.block, s.n * a.per_kv - s.r0);
     const int seen = a.mask ? s.n : min(s.n, (s.r0 + s.rows + a.per_kv - 1) / a.per_kv);
     s.keys = s.len + seen;
+    s.edge = a.mask ? s.len : s.len + s.r0 / a.per_kv + 1;
     s.tiles = s.rows > 0 ? (s.keys + a.tile - 1) / a.tile : 0;
     return s;
 }

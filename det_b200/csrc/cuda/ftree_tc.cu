@@ -9,9 +9,14 @@
 // same rows and take every other tile of keys, and their results are added at the end; more rows: 128 rows each over the same tiles.
 // Heads above 128: one slot (TMEM and shared memory hold no more), tiles of 64 keys.
 //
-// Warps: four per slot for the softmax; three that bring rows of Q, K and V into shared memory by 16-byte asynchronous copies, laid
-// out as the products want them (128-byte swizzle; K and Q K-major, V as it lies in the cache, MN-major); one that issues the products.
-// The caches' addresses are in device memory, so a tensor map on the host cannot describe them.
+// Warps: four per slot for the softmax; one that loads tiles of K and V (TMA, 128-byte swizzle; K K-major, V as it lies in the cache,
+// MN-major); one that issues the products; two that bring the query rows (16-byte asynchronous copies, a head's rows are not evenly
+// spaced) and look through the values of tiles that not every row sees.  The caches' addresses and lengths are in device memory: the
+// loading warp writes them into a tensor map of its CTA (tensormap.replace) when a stretch begins another sequence, and rows behind the
+// last key then read as zeros.
+//
+// A masked weight is zero, but zero times a value that is not finite is not: in tiles that not every row sees such values enter the
+// product as zeros, and the end of the stretch adds them to the rows that do see them.
 //
 // A weight is rounded to bfloat16 for its product, as any tensor-core form must (half a step, 2^-8 relative, independent from key to
 // key); sums and references are fp32.
@@ -22,14 +27,13 @@
 namespace detb {
 
 constexpr int TT_ROWS = 128;
-constexpr int TT_COPY = 96;                          // threads that copy
+constexpr int TT_COPY = 64;                          // threads that bring rows
 constexpr float TT_GROWTH = 8.0f;                   // log2 of how far a maximum may outgrow the reference
 
 template <int SLOTS, int KT>
 struct TtCfg {
-    static constexpr int SOFT = 4 * SLOTS, THREADS = (SOFT + TT_COPY / 32 + 1) * 32, PRODUCTS = SOFT + TT_COPY / 32;   // warps
+    static constexpr int SOFT = 4 * SLOTS, LOADS = SOFT, PRODUCTS = SOFT + 1, ROWS = SOFT + 2, THREADS = (SOFT + 4) * 32;   // first warps of the roles
     static constexpr int O_COL = SLOTS * KT;
-    static constexpr int PEND = 3;                  // tiles whose copies are in flight (flush() counts on three; PEND + 2 <= stages)
 };
 struct TtShape {
     int nkb, nvb;                                   // 64-element blocks of a key, of a value
@@ -39,7 +43,9 @@ struct TtShape {
 };
 
 constexpr int TT_STAGES = 12;
-struct TtTables {
+struct alignas(128) TtTables {
+    unsigned char map[2][128];
+    unsigned long long raw[TT_STAGES];               // a tile of values that is looked through before it is full
     unsigned long long full[TT_STAGES], empty[TT_STAGES], q_full[2], q_empty[2], s_full[2], p_full[2], o_full, o_empty;
     float2 ml[2][TT_ROWS];                           // [slot]: reference and sum of a row
     TreeShare share;
@@ -121,75 +127,52 @@ __device__ __forceinline__ void tmem_landed(int (&r)[16]) {
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes) {      // what is missing of 16 bytes becomes zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// One warp's part of a tile: rows of `pieces` 16-byte pieces, `ldb` bytes apart, into swizzled blocks of `rows` rows x 128 bytes.  LANES
-// lanes take the pieces of a row, so a lane keeps its piece and the swizzle of its rows repeats every 8: an address is one addition.
-// Pieces past `real` become zeros, as do rows past `have` (`zero`; else they keep what is there).
-template <int LANES>
-__device__ __forceinline__ void tt_copy(unsigned dst, const char* src, size_t ldb, int rows, int pieces, int real, int have, bool zero, int warp, int lane) {
-    constexpr int AT_ONCE = 32 / LANES, J = 8 / AT_ONCE;
-    const int c = lane % LANES, rr = lane / LANES;
-    if (c >= pieces) return;
-    const int bytes = c < real ? 16 : 0;
-    unsigned to[J];
-#pragma unroll
-    for (int j = 0; j < J; j++) {
-        const int r = j * AT_ONCE + rr;
-        to[j] = dst + (unsigned)((c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4)) + warp * 1024;
+// The tensor maps of a sequence's keys and values, made from the launch's by the whole warp: their addresses and number of rows are set
+// in shared memory and the maps copied to `to`, where loads may name them.
+__device__ __forceinline__ void tt_maps(const CUtensorMap& mk, const CUtensorMap& mv, unsigned char (*sm)[128], const bf16* keys, const bf16* values, int rows,
+                                        unsigned char* to, int lane) {
+    reinterpret_cast<unsigned*>(sm[0])[lane] = reinterpret_cast<const unsigned*>(&mk)[lane];
+    reinterpret_cast<unsigned*>(sm[1])[lane] = reinterpret_cast<const unsigned*>(&mv)[lane];
+    __syncwarp();
+    if (lane < 2) {
+        const unsigned m = smem_addr(sm[lane]);
+        asm volatile("tensormap.replace.tile.global_address.shared::cta.b1024.b64 [%0], %1;" ::"r"(m), "l"(lane ? values : keys) : "memory");
+        asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 2, %1;" ::"r"(m), "r"(rows) : "memory");
     }
-    const char* first = src;
-    src += (size_t)(warp * 8 + rr) * ldb + (bytes ? c * 16 : 0);
-    const size_t step = (size_t)AT_ONCE * ldb, skip = (size_t)(TT_COPY / 4 - 8) * ldb;
-    const int end = zero ? rows : min(rows, have);
-    for (int r = warp * 8; r < end; r += TT_COPY / 4) {
-        if (r + 8 <= have) {
+    __syncwarp();
 #pragma unroll
-            for (int j = 0; j < J; j++) {
-                copy16(to[j], src, bytes);
-                src += step;
-            }
-        } else {
+    for (int i = 0; i < 2; i++)
+        asm volatile("tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned [%0], [%1], 128;" ::"l"(to + i * 128),
+                     "r"(smem_addr(sm[i]))
+                     : "memory");
 #pragma unroll
-            for (int j = 0; j < J; j++) {
-                const bool in = r + j * AT_ONCE + rr < have;
-                if (in || zero) copy16(to[j], in ? src : first, in ? bytes : 0);
-                src += step;
-            }
-        }
-        src += skip;
-#pragma unroll
-        for (int j = 0; j < J; j++) to[j] += (TT_COPY / 4) * 128;
-    }
+    for (int i = 0; i < 2; i++) asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(to + i * 128) : "memory");
 }
-__device__ __forceinline__ void tt_tile(unsigned dst, const bf16* src, size_t ldb, int rows, int pieces, int real, int have, bool zero, int warp, int lane) {
-    const char* p = reinterpret_cast<const char*>(src);
-    if (pieces <= 8) tt_copy<8>(dst, p, ldb, rows, pieces, real, have, zero, warp, lane);
-    else if (pieces <= 16) tt_copy<16>(dst, p, ldb, rows, pieces, real, have, zero, warp, lane);
-    else tt_copy<32>(dst, p, ldb, rows, pieces, real, have, zero, warp, lane);
+__device__ __forceinline__ void tt_load(void* dst, const void* map, int x, int head, int row, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+                 "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_addr(bar))
+                 : "memory");
 }
-// Values of the tree that are not finite become zeros in the staged tile; true when there were any.  A lane looks at its own copies.
-__device__ __forceinline__ bool tt_clean(uint8_t* tile, int rows, int pieces, int warp, int lane) {
-    const int lanes = pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32, c = lane % lanes;
+// Values that are not finite become zeros in a staged tile (blocks of 64 columns x `rows` keys); true when there were any.
+__device__ __forceinline__ bool tt_clean(uint8_t* tile, int bytes, int tid) {
     bool odd = false;
-    if (c < pieces)
-        for (int r0 = warp * 8; r0 < rows; r0 += TT_COPY / 4)
-            for (int r = r0 + lane / lanes; r < r0 + 8; r += 32 / lanes) {
-                uint4* p = reinterpret_cast<uint4*>(tile + (c >> 3) * rows * 128 + r * 128 + (((c ^ r) & 7) << 4));
-                const uint4 v = *p;
-                unsigned w[4] = {v.x, v.y, v.z, v.w};
-                bool hit = false;
+#pragma unroll 4
+    for (int i = tid * 16; i < bytes; i += TT_COPY * 16) {
+        uint4* p = reinterpret_cast<uint4*>(tile + i);
+        const uint4 v = *p;
+        unsigned w[4] = {v.x, v.y, v.z, v.w};
+        bool hit = false;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, hit = true;
-                    if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, hit = true;
-                }
-                if (hit) *p = make_uint4(w[0], w[1], w[2], w[3]);
-                odd |= hit;
-            }
+        for (int j = 0; j < 4; j++) {
+            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, hit = true;
+            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, hit = true;
+        }
+        if (hit) *p = make_uint4(w[0], w[1], w[2], w[3]);
+        odd |= hit;
+    }
     return odd;
 }
 
@@ -236,13 +219,14 @@ __device__ __forceinline__ float tt_weights(const TreeArgs& a, const TreeSeg& s,
 }
 
 template <int SLOTS, int KT>
-__global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const TreeArgs a, const TtShape sh) {
+__global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                               const TreeArgs a, const TtShape sh) {
     using Cfg = TtCfg<SLOTS, KT>;
-    constexpr int SOFT = Cfg::SOFT, PRODUCTS = Cfg::PRODUCTS;
+    constexpr int SOFT = Cfg::SOFT, LOADS = Cfg::LOADS, PRODUCTS = Cfg::PRODUCTS, ROWS = Cfg::ROWS;
     extern __shared__ __align__(1024) uint8_t Qs[];                     // [SLOTS][nkb][128][128 B], the ring, the tables
     uint8_t* ring = Qs + SLOTS * sh.q_bytes;
     TtTables& tb = *reinterpret_cast<TtTables*>(ring + (size_t)sh.stages * sh.stage_bytes);
-    auto &full = tb.full, &empty = tb.empty;
+    auto &full = tb.full, &empty = tb.empty, &raw = tb.raw;
     auto &q_full = tb.q_full, &q_empty = tb.q_empty, &s_full = tb.s_full, &p_full = tb.p_full;
     auto &o_full = tb.o_full, &o_empty = tb.o_empty;
     auto &odd = tb.odd;
@@ -256,11 +240,12 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < sh.stages; s++) {
-            mbar_init(&full[s], TT_COPY / 32);
+            mbar_init(&raw[s], 1);
+            mbar_init(&full[s], 2);
             mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(&q_full[i], TT_COPY / 32);
+            mbar_init(&q_full[i], 2);
             mbar_init(&q_empty[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
@@ -288,79 +273,85 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
     const int lead = both ? 2 : 1;                   // tiles whose scores are asked for ahead
     unsigned item = 0;                               // stretches so far
 
-    if (warp >= SOFT && warp < PRODUCTS) {
-        // ---- copies
-        const int cw = warp - SOFT;
-        const int kp = (a.kd + 15) / 16 * 2, vp = (a.vd + 15) / 16 * 2;
-        // a copy in flight: stage, and whether it begins a stretch (1), holds values of a tree (2), the stretch (from bit 2)
-        int st[Cfg::PEND], what[Cfg::PEND];
-#pragma unroll
-        for (int i = 0; i < Cfg::PEND; i++) st[i] = -1, what[i] = 0;
+    if (warp == LOADS) {
+        // ---- tiles of keys and values
         unsigned c = 0;                              // tiles issued
-        auto land = [&](int s, int w) {
-            if (s < 0) return;
-            if (w & 2) {
-                if (tt_clean(ring + (size_t)s * sh.stage_bytes, KT, vp, cw, lane)) *reinterpret_cast<volatile int*>(&odd[(w >> 2) & 3]) = (w >> 2) + 1;
-            }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) {
-                if (w & 1) mbar_arrive(&q_full[both ? (w >> 2) & 1 : 0]);
-                mbar_arrive(&full[s]);
-            }
-        };
-        auto flush = [&]() {
-            copies_wait<2>();
-            land(st[2], what[2]);
-            copies_wait<1>();
-            land(st[1], what[1]);
-            copies_wait<0>();
-            land(st[0], what[0]);
-            st[0] = st[1] = st[2] = -1;
-        };
+        int seq = -1, maps = 0;
+        unsigned char* map = nullptr;
         while (ok && tree_next(a, walk, it)) {
             const TreeSeg& s = it.s;
-            const bf16* cache = static_cast<const bf16*>(a.seq.table[s.b].cache);
+            if (s.b != seq) {
+                // a map is written again TREE_MAPS sequences later: by then more tiles have passed the ring than it has stages
+                const bf16* cache = static_cast<const bf16*>(a.seq.table[s.b].cache);
+                map = static_cast<unsigned char*>(a.maps) + ((size_t)blockIdx.x * TREE_MAPS + maps % TREE_MAPS) * 256;
+                tt_maps(map_k, map_v, tb.map, cache, cache + a.kv_heads * a.kd, s.len + s.n, map, lane);
+                seq = s.b;
+                maps++;
+            }
+            if (lane == 0) {
+                auto fetch = [&](bool value, int t) {
+                    const unsigned sn = c % sh.stages;
+                    if (c >= (unsigned)sh.stages) ok = mbar_wait(&empty[sn], ((c / sh.stages) & 1u) ^ 1u, wl);
+                    if (!ok) return;
+                    const int k0 = (it.tile + t) * KT, blocks = value ? sh.nvb : sh.nkb;
+                    const bool look = value && k0 + KT > s.edge;
+                    unsigned long long* bar = look ? &raw[sn] : &full[sn];
+                    mbar_expect_tx(bar, blocks * KT * 128);
+                    if (!look) mbar_arrive(bar);
+                    for (int i = 0; i < blocks; i++)
+                        tt_load(ring + (size_t)sn * sh.stage_bytes + i * KT * 128, map + (value ? 128 : 0), i * 64, it.g, k0, bar);
+                    c++;
+                };
+                for (int t = 0; t < min(lead, it.n) && ok; t++) fetch(false, t);
+                for (int t = 0; t < it.n && ok; t++) {
+                    fetch(true, t);
+                    if (ok && t + lead < it.n) fetch(false, t + lead);
+                }
+            }
+            ok = __shfl_sync(FULL, ok ? 1 : 0, 0) != 0;
+        }
+        if (!ok && lane == 0)                        // the loads in flight write shared memory: at the most one phase of each barrier is open
+            for (unsigned k = 1; k <= (unsigned)sh.stages && k <= c; k++) {
+                (void)mbar_wait(&full[(c - k) % sh.stages], ((c - k) / sh.stages) & 1u, wl);
+            }
+    } else if (warp >= ROWS) {
+        // ---- query rows, and values that not every row sees
+        const int tid = threadIdx.x - ROWS * 32;
+        const int kp = (a.kd + 15) / 16 * 2, lanes = kp <= 8 ? 8 : kp <= 16 ? 16 : 32, qc = lane % lanes, qstep = TT_COPY / lanes;
+        unsigned c = 0, looked = 0;                  // tiles of the stretches before; phases of `raw`, a bit per stage
+        while (ok && tree_next(a, walk, it)) {
+            const TreeSeg& s = it.s;
             const int qb = both ? item & 1 : 0;
-            if (!both) flush();                      // the wait below needs what is in flight
             if (item >= (both ? 2u : 1u)) ok = wait(&q_empty[qb], ((both ? item >> 1 : item) & 1u) ^ 1u);
             if (!ok) break;
-            // query rows: a row per LANES lanes; rows that are not there keep what is there (a row's scores are its own)
+            // a row per `lanes` lanes; rows that are not there keep what is there (a row's scores are its own)
             const bf16* q = static_cast<const bf16*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
-            const int lanes = kp <= 8 ? 8 : kp <= 16 ? 16 : 32, qc = lane % lanes, qstep = TT_COPY / lanes;
             if (qc < kp)
-                for (int r = (cw * 32 + lane) / lanes; r < s.rows; r += qstep) {
+#pragma unroll 4
+                for (int r = tid / lanes; r < s.rows; r += qstep) {
                     const int row = s.r0 + r, node = (int)(row * a.per_magic >> 32), x = r & (TT_ROWS - 1);
                     const bf16* src = q + (size_t)node * a.ldq + (row - node * a.per_kv) * a.kd;
                     copy16(smem_addr(Qs + (size_t)(both ? qb : r / TT_ROWS) * sh.q_bytes) + (unsigned)((qc >> 3) * TT_ROWS * 128 + x * 128 + (((qc ^ x) & 7) << 4)),
                            qc * 8 < a.kd ? src + qc * 8 : src, qc * 8 < a.kd ? 16 : 0);
                 }
-            auto fetch = [&](bool value, int t) {
-                const unsigned sn = c % sh.stages;
-                if (c >= (unsigned)sh.stages) ok = wait(&empty[sn], ((c / sh.stages) & 1u) ^ 1u);
-                if (!ok) return;
-                const int k0 = (it.tile + t) * KT;
-                const bf16* rows = cache + (size_t)k0 * a.ld + (value ? a.kv_heads * a.kd + it.g * a.vd : it.g * a.kd);
-                // rows behind the last key: zeros for values (their weights are zero), anything for keys (their scores are masked)
-                tt_tile(smem_addr(ring + (size_t)sn * sh.stage_bytes), rows, (size_t)a.ld * 2, KT, value ? vp : kp, (value ? a.vd : a.kd) / 8,
-                        s.len + s.n - k0, value, cw, lane);
-                copies_commit();
-                copies_wait<Cfg::PEND>();
-                land(st[Cfg::PEND - 1], what[Cfg::PEND - 1]);
-#pragma unroll
-                for (int i = Cfg::PEND - 1; i > 0; i--) st[i] = st[i - 1], what[i] = what[i - 1];
-                st[0] = (int)sn;
-                what[0] = (!value && t == 0 ? 1 : 0) | (value && k0 + KT > s.len ? 2 : 0) | (int)(item << 2);
-                c++;
-            };
-            for (int t = 0; t < min(lead, it.n) && ok; t++) fetch(false, t);
-            for (int t = 0; t < it.n && ok; t++) {
-                fetch(true, t);
-                if (ok && t + lead < it.n) fetch(false, t + lead);
+            copies_wait_all();
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[qb]);
+            for (int t = max(0, s.edge / KT - it.tile); t < it.n && ok; t++) {
+                // the ring holds K .. (lead tiles), then V, K, V, K ..
+                const unsigned at = c + min(lead, it.n) + t + min(t, max(0, it.n - lead)), sn = at % sh.stages;
+                ok = wait(&raw[sn], (looked >> sn) & 1u);
+                looked ^= 1u << sn;
+                if (!ok) break;
+                if (tt_clean(ring + (size_t)sn * sh.stage_bytes, sh.nvb * KT * 128, tid)) *reinterpret_cast<volatile int*>(&odd[item & 3]) = (int)item + 1;
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[sn]);
             }
+            c += 2 * it.n;
             item++;
         }
-        flush();
     } else if (warp == PRODUCTS) {
         // ---- products
         if (lane == 0) {
@@ -462,7 +453,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 tc_fence_after();
                 if (any) {
                     const int k0 = (it.tile + (both ? 2 * j + slot : j)) * KT;
-                    const bool tree = k0 + KT > s.len;
+                    const bool tree = k0 + KT > s.edge;
                     const float mt = tree ? tt_max<KT, true>(a, s, ts, node, k0) : tt_max<KT, false>(a, s, ts, node, k0);
                     const bool grow = (mt - m) * a.scale2 > TT_GROWTH;
                     if (__any_sync(FULL, grow)) {
@@ -531,8 +522,8 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                     }
                     if (fix) {                        // warps agree on it
                         // values of attended nodes that are not finite (they entered the product as zeros)
-                        const int k0 = it.tile * KT, k1 = min(s.len + s.n, k0 + it.n * KT);
-                        for (int k = max(k0, s.len); k < k1; k++) {
+                        const int k1 = min(s.len + s.n, (it.tile + it.n) * KT);
+                        for (int k = max(it.tile, s.edge / KT) * KT; k < k1; k++) {
                             if (!(tree_seen(a, s, node, k) & 1u)) continue;
                             const bf16* val = static_cast<const bf16*>(a.seq.table[s.b].cache) + (size_t)k * a.ld + a.kv_heads * a.kd + it.g * a.vd + q;
 #pragma unroll
@@ -566,7 +557,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
     }
     __syncwarp();
     if (!ok && lane == 0) atomicExch(a.error_flag, DETB_ERR_WAIT_EXPIRED);
-    copies_wait<0>();
+    copies_wait_all();
     tc_fence_before();
     __syncthreads();
     if (warp == PRODUCTS) tmem_dealloc(tmem, 512);
@@ -579,10 +570,19 @@ void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile) {
     *tile = wide ? 64 : 128;
 }
 
+// A cache's keys or values (`size` elements a head) as [rows][heads][size], boxes of 64 elements of one head x `box` rows, zeros outside.
+// Address and rows are the first cache's that the kernel sets; here they only have to be well formed.
+static bool cache_map(CUtensorMap* map, const TreeArgs& a, int size, int box) {
+    const cuuint64_t dims[3] = {(cuuint64_t)size, (cuuint64_t)a.kv_heads, (cuuint64_t)a.cap};
+    const cuuint64_t strides[2] = {(cuuint64_t)size * 2, (cuuint64_t)a.ld * 2};
+    const cuuint32_t boxes[3] = {64, 1, (cuuint32_t)box}, estr[3] = {1, 1, 1};
+    return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, a.maps, dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int SLOTS, int KT>
 static cudaError_t launch(const TreeArgs& a, cudaStream_t q) {
     using Cfg = TtCfg<SLOTS, KT>;
-    static_assert(Cfg::PEND == 3 && KT % 32 == 0);
     TtShape sh{};
     sh.nkb = (a.kd + 63) / 64;
     sh.nvb = (a.vd + 63) / 64;
@@ -594,7 +594,9 @@ static cudaError_t launch(const TreeArgs& a, cudaStream_t q) {
     const size_t smem = fixed + (size_t)sh.stages * sh.stage_bytes;
     const cudaError_t e = cudaFuncSetAttribute(k_ftree_tc<SLOTS, KT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl_try(k_ftree_tc<SLOTS, KT>, dim3(a.ctas), dim3(Cfg::THREADS), smem, q, 1, a, sh);
+    CUtensorMap keys, values;
+    if (!cache_map(&keys, a, a.kd, KT) || !cache_map(&values, a, a.vd, KT)) return cudaErrorInvalidValue;
+    return launch_pdl_try(k_ftree_tc<SLOTS, KT>, dim3(a.ctas), dim3(Cfg::THREADS), smem, q, 1, keys, values, a, sh);
 }
 
 cudaError_t ftree_tc_launch(const TreeArgs& a, cudaStream_t q) { return a.tile == 128 ? launch<2, 128>(a, q) : launch<1, 64>(a, q); }

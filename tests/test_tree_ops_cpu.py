@@ -41,7 +41,7 @@ BAD_QK = [dict(heads=0), dict(kv_heads=-1), dict(dim=0), dict(dim=257), dict(vdi
 BAD_ATTN = [dict(heads=0), dict(heads=5), dict(kv_heads=0), dict(dim=0), dict(dim=264), dict(vdim=0), dict(cap=0), dict(dtype=-1),
             dict(scale=0.0), dict(scale=-1.0), dict(scale=NAN), dict(scale=float("inf")), dict(mask_ld=0), dict(ldo=255), dict(gate=P, ldg=3),
             dict(vrope_cos=P), dict(vrope_cos=P, vrope_sin=P), dict(vrope_cos=P, vrope_sin=P, pos=P, rope_len=0), dict(q=None), dict(out=None),
-            dict(scratch=None), dict(q=P + 4), dict(scratch=P + 8)]
+            dict(scratch=None), dict(q=P + 4), dict(scratch=P + 8), dict(scratch=P + 64)]
 BAD_KEEP = [dict(caches=-1), dict(seqs=-1), dict(cap=0), dict(max_count=-1), dict(max_count=5), dict(max_count=2000, keep_ld=2000), dict(row_bytes=0),
             dict(row_bytes=24), dict(caches=3), dict(table=None), dict(len=None), dict(keep=None), dict(count=None), dict(len_out=P)]
 BAD_REF = [dict(seqs=-1), dict(rows=-1), dict(max_len=-1), dict(max_nodes=-1), dict(seqs=70000), dict(table=None), dict(first=None), dict(len=None)]

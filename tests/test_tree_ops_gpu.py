@@ -353,6 +353,26 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_attend_them(bad, dty
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("masked", [0, 1])
+def test_values_of_the_cache_that_are_not_finite_reach_every_row(masked, dtype, gpu, libs):
+    """A cached value beside the tree (in the same tile, and far ahead of it) is attended by every row; in a run a token's value reaches
+    the tokens from it on."""
+    rng = np.random.default_rng(12)
+    for at, bad in [(149, np.inf), (3, -np.inf), (148, np.nan)]:
+        a = Attn(gpu, libs, dtype, 2, 1, 64, 64, [150], [40], masks=random_masks([40], rng) if masked else None)
+        c = a.values[0].copy()
+        c[at, 64 + 9] = bad
+        c[150 + 30, 64 + 20] = bad                             # node 30
+        a.caches[0], a.values[0] = store(gpu, c, dtype)
+        got = a.call().reshape(40, 2, 64)
+        for x in (got[:, 0], got[:, 1]):
+            assert (np.isnan(x[:, 9]) if np.isnan(bad) else x[:, 9] == bad).all()
+            hit = a.seen(0)[:, 150 + 30]
+            assert (np.isnan(x[hit, 20]) if np.isnan(bad) else x[hit, 20] == bad).all()
+            assert np.isfinite(np.delete(x, [9, 20], 1)).all() and np.isfinite(x[~hit, 20]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_gates_and_rotated_values(dtype, gpu, libs):
     rng = np.random.default_rng(2)
     for gate, vrot in [(1, 0), (0, 1), (1, 1)]:
