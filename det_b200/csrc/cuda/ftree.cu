@@ -166,8 +166,7 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
             const float sum = row_sum(l[i]);
             if (r >= s.rows) continue;
             if (!it.whole && tx == 0) {
-                piece[r] = m[i];
-                piece[RB + r] = sum;
+                reinterpret_cast<float2*>(piece)[r] = make_float2(m[i], sum);
             }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // no key seen
             const TreeOut<float> out(a, s.first + row / a.per_kv, it.g * a.per_kv + row % a.per_kv);
@@ -186,58 +185,78 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------ pieces
-constexpr int TM_THREADS = 256;
-// grid (key/value heads x pieces of a block's (row, four values) pairs, segments)
+constexpr int TM_THREADS = 512, TM_ROWS = 16;
+// grid (key/value heads x groups of 16 rows of a block, segments).  The factors of the pieces first, then a thread per (row, four
+// values).  Bound by the latency of its two rounds of loads: a merge of 18 pieces of 80 rows x 8 heads takes MERGE_US.
 template <class T>
 __global__ void __launch_bounds__(TM_THREADS) k_ftree_merge(const TreeArgs a) {
+    __shared__ float fac[TM_ROWS][TREE_CTAS];
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31, g = blockIdx.x % a.kv_heads, chunk = blockIdx.x / a.kv_heads, chunks = gridDim.x / a.kv_heads;
-    const TreeSeg s = tree_seg(a, blockIdx.y);
-    if (s.tiles <= 1) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.x % a.kv_heads, r0 = blockIdx.x / a.kv_heads * TM_ROWS;
     long long before = 0, total = 0;
+    TreeSeg s{};
     for (int i = lane; i < a.seq.seqs * a.blocks; i += 32) {
-        const int t = tree_seg(a, i).tiles;
-        total += t;
-        if (i < (int)blockIdx.y) before += t;
+        const TreeSeg x = tree_seg(a, i);
+        total += x.tiles;
+        if (i < (int)blockIdx.y) before += x.tiles;
+        if (i == (int)blockIdx.y) s = x;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
         total += __shfl_xor_sync(FULL, total, off);
         before += __shfl_xor_sync(FULL, before, off);
     }
+    const int from = (int)blockIdx.y & 31, rows = min(TM_ROWS, __shfl_sync(FULL, s.rows, from) - r0), tiles = __shfl_sync(FULL, s.tiles, from);
+    const int base_row = __shfl_sync(FULL, s.r0, from) + r0, first = __shfl_sync(FULL, s.first, from);
+    if (tiles <= 1 || rows <= 0) return;
     total *= a.kv_heads;
-    const long long share = tree_share(a, total), u0 = before * a.kv_heads + (long long)g * s.tiles, left = u0 % share;
-    const int c0 = (int)(u0 / share), n = (int)((left + s.tiles + share - 1) / share);      // the first CTA, and how many
-    if (n == 1) return;
+    const long long share = tree_share(a, total), u0 = before * a.kv_heads + (long long)g * tiles;
+    const int c0 = (int)(u0 / share);
+    const long long left = u0 - c0 * share;
+    if (left + tiles <= share) return;                        // one CTA finished it
+    const int n = (int)((left + tiles + share - 1) / share);
     const size_t size = tree_piece_floats(a.block, a.vd);
     const float* head = a.part + ((size_t)c0 * 2 + (left ? 1 : 0)) * size;    // the others are their CTAs' first pieces
-    const float* rest = a.part + (size_t)(c0 + 1) * 2 * size;
-    const int vq = a.vd / 4;
-    for (int i = chunk * TM_THREADS + threadIdx.x; i < s.rows * vq; i += chunks * TM_THREADS) {
-        const int v = i / s.rows, r = i - v * s.rows;
-        float m = head[r];
+    const float* rest = a.part + (size_t)c0 * 2 * size;
+    if (warp < rows) {
+        float m = -INFINITY, l = 0.0f;
+        float2 ml[(TREE_CTAS + 31) / 32];
+#pragma unroll
+        for (int i = 0; i < (TREE_CTAS + 31) / 32; i++) {
+            const int c = i * 32 + lane;
+            ml[i] = c < n ? reinterpret_cast<const float2*>(c ? rest + c * 2 * size : head)[r0 + warp] : make_float2(-INFINITY, 0.0f);
+            m = fmaxf(m, ml[i].x);
+        }
+        m = warp_max(m);
+        if (m == -INFINITY) m = 0.0f;                         // a row without keys
+#pragma unroll
+        for (int i = 0; i < (TREE_CTAS + 31) / 32; i++) {
+            ml[i].x = exp2f(ml[i].x - m);
+            l = fmaf(ml[i].x, ml[i].y, l);
+        }
+        l = warp_sum(l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < (TREE_CTAS + 31) / 32; i++)
+            if (i * 32 + lane < n) fac[warp][i * 32 + lane] = ml[i].x * inv;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (a.vd / 4); i += TM_THREADS) {
+        const int v = i / rows, r = i - v * rows;
+        const size_t at = 2 * a.block + ((size_t)v * a.block + r0 + r) * 4;
+        float4 o = scaled4(load4(head + at), fac[r][0]);
 #pragma unroll 8
-        for (int c = 0; c < n - 1; c++) m = fmaxf(m, rest[(size_t)c * 2 * size + r]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        const float f = exp2f(head[r] - base);
-        float l = f * head[a.block + r];
-        const size_t at = 2 * a.block + ((size_t)v * a.block + r) * 4;
-        float4 o = scaled4(load4(head + at), f);
-#pragma unroll 4
-        for (int c = 0; c < n - 1; c++) {
-            const float* p = rest + (size_t)c * 2 * size;
-            const float w = exp2f(p[r] - base);
-            const float4 x = load4(p + at);
-            l = fmaf(w, p[a.block + r], l);
+        for (int c = 1; c < n; c++) {
+            const float4 x = load4(rest + c * 2 * size + at);
+            const float w = fac[r][c];
             o.x = fmaf(w, x.x, o.x);
             o.y = fmaf(w, x.y, o.y);
             o.z = fmaf(w, x.z, o.z);
             o.w = fmaf(w, x.w, o.w);
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int row = s.r0 + r;
-        TreeOut<T>(a, s.first + row / a.per_kv, g * a.per_kv + row % a.per_kv).put4at(v * 4, scaled4(o, inv));
+        const int row = base_row + r, node = (int)(row * a.per_magic >> 32);
+        TreeOut<T>(a, first + node, g * a.per_kv + row - node * a.per_kv).put4at(v * 4, o);
     }
 }
 
@@ -255,8 +274,7 @@ static cudaError_t launch_simt_v(const TreeArgs& a, cudaStream_t q) {
 }
 template <class T>
 static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
-    const int chunks = std::max(1, std::min(16, a.block * (a.vd / 4) / TM_THREADS));
-    return launch_pdl_try(k_ftree_merge<T>, dim3(a.kv_heads * chunks, a.seq.seqs * a.blocks), dim3(TM_THREADS), 0, q, 1, a);
+    return launch_pdl_try(k_ftree_merge<T>, dim3(a.kv_heads * (a.block / TM_ROWS), a.seq.seqs * a.blocks), dim3(TM_THREADS), 0, q, 1, a);
 }
 // Rows of a block and keys of a tile.
 static void simt_shape(int rows, int* block, int* tile) {

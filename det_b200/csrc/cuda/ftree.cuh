@@ -81,7 +81,7 @@ struct TreeArgs {
 };
 constexpr int TREE_MAPS = 8;
 constexpr size_t TREE_MAP_BYTES = (size_t)TREE_CTAS * TREE_MAPS * 2 * 128;
-// A piece: m[block] | l[block] | o[vd / 4][block][4].
+// A piece: {maximum, sum}[block] | values[vd / 4][block][4].
 __host__ __device__ constexpr size_t tree_piece_floats(int block, int vd) { return (size_t)block * (2 + vd); }
 
 struct TreeSeg {

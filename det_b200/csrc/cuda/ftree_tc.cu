@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
 
     if (warp == LOADS) {
         // ---- tiles of keys and values
-        unsigned c = 0;                              // tiles issued
+        unsigned c = 0, sn = 0, phase = 0;           // tiles issued, place in the ring
         int seq = -1, maps = 0;
         unsigned char* map = nullptr;
         while (ok && tree_next(a, walk, it)) {
@@ -290,8 +290,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
             }
             if (lane == 0) {
                 auto fetch = [&](bool value, int t) {
-                    const unsigned sn = c % sh.stages;
-                    if (c >= (unsigned)sh.stages) ok = mbar_wait(&empty[sn], ((c / sh.stages) & 1u) ^ 1u, wl);
+                    if (c >= (unsigned)sh.stages) ok = mbar_wait(&empty[sn], phase ^ 1u, wl);
                     if (!ok) return;
                     const int k0 = (it.tile + t) * KT, blocks = value ? sh.nvb : sh.nkb;
                     const bool look = value && k0 + KT > s.edge;
@@ -301,6 +300,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                     for (int i = 0; i < blocks; i++)
                         tt_load(ring + (size_t)sn * sh.stage_bytes + i * KT * 128, map + (value ? 128 : 0), i * 64, it.g, k0, bar);
                     c++;
+                    if (++sn == (unsigned)sh.stages) sn = 0, phase ^= 1u;
                 };
                 for (int t = 0; t < min(lead, it.n) && ok; t++) fetch(false, t);
                 for (int t = 0; t < it.n && ok; t++) {
@@ -357,28 +357,35 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
         if (lane == 0) {
             const unsigned id_s = tt_idesc(KT, false), vn = (unsigned)(a.vd + 15) / 16 * 16, id_o = tt_idesc((int)vn, true);
             const int ksteps = (a.kd + 15) / 16;
-            unsigned c = 0, np[2] = {0, 0};          // tiles taken, weights taken per slot
+            const unsigned long long q_desc = umma_desc(Qs), k_desc = umma_desc(ring), v_desc = umma_desc_mn(ring, KT * 128);
+            unsigned c = 0, phase = 0, np[2] = {0, 0};   // place in the ring, weights taken per slot
             while (ok && tree_next(a, walk, it)) {
                 const int qb = both ? item & 1 : 0;
                 const bool second = !both && SLOTS == 2 && it.s.rows > TT_ROWS;
                 ok = mbar_wait(&q_full[qb], ((both ? item >> 1 : item) & 1u), wl);
                 if (!ok) break;
-                auto scores = [&](int slot, const uint8_t* K) {
-                    const uint8_t* Q = Qs + (size_t)(both ? qb : slot) * sh.q_bytes;
-                    for (int k = 0; k < ksteps; k++)
-                        umma_f16_ss(tmem + slot * KT, umma_desc(Q + (size_t)(k >> 2) * TT_ROWS * 128) + 2 * (k & 3),
-                                    umma_desc(K + (size_t)(k >> 2) * KT * 128) + 2 * (k & 3), id_s, k ? 1u : 0u);
+                // descriptors of neighbouring steps differ in their address (units of 16 bytes) only
+                auto scores = [&](int slot, unsigned s) {
+                    unsigned long long q = q_desc + (unsigned)(both ? qb : slot) * (unsigned)(sh.q_bytes >> 4), k = k_desc + s * (unsigned)(sh.stage_bytes >> 4);
+                    for (int e = 0; e < ksteps; e += 4) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (e + i < ksteps) umma_f16_ss(tmem + slot * KT, q + 2 * i, k + 2 * i, id_s, (e | i) ? 1u : 0u);
+                        q += TT_ROWS * 128 >> 4;
+                        k += KT * 128 >> 4;
+                    }
                     umma_commit(&s_full[slot]);
                 };
-                auto outputs = [&](int slot, const uint8_t* V, bool first) {
+                auto outputs = [&](int slot, unsigned s, bool first) {
+                    const unsigned long long v = v_desc + s * (unsigned)(sh.stage_bytes >> 4);
+#pragma unroll
                     for (int k = 0; k < KT / 16; k++)
-                        umma_f16_ts(tmem + Cfg::O_COL + slot * (256 / SLOTS), tmem + slot * KT + k * 8, umma_desc_mn(V + k * 2048, KT * 128), id_o,
-                                    first && k == 0 ? 0u : 1u);
+                        umma_f16_ts(tmem + Cfg::O_COL + slot * (256 / SLOTS), tmem + slot * KT + k * 8, v + k * 128, id_o, first && k == 0 ? 0u : 1u);
                 };
                 auto stage = [&]() {
-                    const unsigned s = c % sh.stages;
-                    ok = mbar_wait(&full[s], (c / sh.stages) & 1u, wl);
-                    c++;
+                    const unsigned s = c;
+                    ok = mbar_wait(&full[s], phase, wl);
+                    if (++c == (unsigned)sh.stages) c = 0, phase ^= 1u;
                     tc_fence_after();
                     return s;
                 };
@@ -390,15 +397,14 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 for (int t = 0; t < min(lead, it.n) && ok; t++) {
                     const unsigned s = stage();
                     if (!ok) break;
-                    scores(both ? t & 1 : 0, ring + (size_t)s * sh.stage_bytes);
-                    if (second) scores(1, ring + (size_t)s * sh.stage_bytes);
+                    scores(both ? t & 1 : 0, s);
+                    if (second) scores(1, s);
                     umma_commit(&empty[s]);
                     if (t + 1 == it.n) umma_commit(&q_empty[qb]);
                 }
                 for (int t = 0; t < it.n && ok; t++) {
                     const unsigned sv = stage();
                     if (!ok) break;
-                    const uint8_t* V = ring + (size_t)sv * sh.stage_bytes;
                     if (t == 0 && item > 0) {        // the outputs of the stretch before have been read
                         ok = mbar_wait(&o_empty, (item & 1u) ^ 1u, wl);
                         if (!ok) break;
@@ -409,19 +415,19 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                     unsigned sk = 0;
                     weights(slot);
                     if (!ok) break;
-                    outputs(slot, V, both ? t < 2 : t == 0);
+                    outputs(slot, sv, both ? t < 2 : t == 0);
                     if (!second) umma_commit(&empty[sv]);
                     if (more) {
                         sk = stage();
                         if (!ok) break;
-                        scores(slot, ring + (size_t)sk * sh.stage_bytes);
+                        scores(slot, sk);
                     }
                     if (second) {
                         weights(1);
                         if (!ok) break;
-                        outputs(1, V, t == 0);
+                        outputs(1, sv, t == 0);
                         umma_commit(&empty[sv]);
-                        if (more) scores(1, ring + (size_t)sk * sh.stage_bytes);
+                        if (more) scores(1, sk);
                     }
                     if (more) {
                         umma_commit(&empty[sk]);
@@ -545,8 +551,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                     __syncwarp();
                 }
                 if (mine && !it.whole && (!both || slot == 0)) {
-                    piece[br] = m * a.scale2;
-                    piece[a.block + br] = l;
+                    reinterpret_cast<float2*>(piece)[br] = make_float2(m * a.scale2, l);
                 }
             }
             tc_fence_before();
