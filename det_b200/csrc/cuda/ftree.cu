@@ -110,8 +110,7 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
                 unsigned seen[2] = {FULL, FULL};
                 if (tree) {
                     const int node = (s.r0 + min(r, s.rows - 1)) / a.per_kv;
-                    seen[0] = tree_seen(a, s, node, k0);
-                    seen[1] = tree_seen(a, s, node, k0 + 32);
+                    tree_seen<2>(a, s, node, k0, seen);
                 }
                 float mx = m[i];
 #pragma unroll

@@ -189,23 +189,22 @@ __device__ __forceinline__ bool tree_next(const TreeArgs& a, TreeWalk& k, TreeIt
     }
     return true;
 }
-// The 32 keys from c0 on that row r of the block sees, as bits; keys from the end of the tree on are never seen.
-__device__ __forceinline__ unsigned tree_seen(const TreeArgs& a, const TreeSeg& s, int node, int c0) {
-    const int t0 = c0 - s.len;                                 // node of the first key, negative ahead of the tree
-    if (t0 <= -32) return FULL;
-    if (t0 >= s.n) return 0;
-    const int lo = max(t0, 0);
-    unsigned w;                                                // nodes lo .. lo + 31
-    if (a.mask) {
-        const unsigned* m = a.mask + (size_t)(s.first + node) * a.mask_ld;
-        const int i = lo >> 5, last = (s.n - 1) >> 5;
-        w = __funnelshift_r(m[i], i < last ? m[i + 1] : 0u, lo & 31);
-    } else {
-        const int k = node + 1 - lo;
-        w = k >= 32 ? FULL : k <= 0 ? 0u : (1u << k) - 1u;
+// Which of the 32 * W keys from c0 on a node sees, as bits; keys from the end of the tree on are never seen.  The words of the mask are
+// asked for side by side.
+template <int W>
+__device__ __forceinline__ void tree_seen(const TreeArgs& a, const TreeSeg& s, int node, int c0, unsigned (&seen)[W]) {
+    const int t0 = c0 - s.len, w0 = t0 >> 5, sh = t0 & 31;     // node of the first key (negative ahead of the tree), its word and bit
+    unsigned m[W + 1];                                         // nodes 32 (w0 + i) ..
+    const unsigned* row = a.mask ? a.mask + (size_t)(s.first + node) * a.mask_ld : nullptr;
+    const int limit = a.mask ? s.n : min(s.n, node + 1);
+#pragma unroll
+    for (int i = 0; i <= W; i++) {
+        const int n0 = (w0 + i) * 32, left = limit - n0;       // a word ahead of the tree is seen whole
+        m[i] = n0 < 0 ? FULL : left <= 0 ? 0u : row ? row[w0 + i] : FULL;
+        if (n0 >= 0 && left > 0 && left < 32) m[i] &= (1u << left) - 1u;
     }
-    if (s.n - lo < 32) w &= (1u << (s.n - lo)) - 1u;
-    return t0 < 0 ? (w << -t0) | ((1u << -t0) - 1u) : w;
+#pragma unroll
+    for (int i = 0; i < W; i++) seen[i] = __funnelshift_r(m[i], m[i + 1], sh);
 }
 // A finished head of a row: elements v .. v + 3 are turned back, gated and stored.
 template <class T>

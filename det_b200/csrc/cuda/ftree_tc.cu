@@ -156,36 +156,41 @@ __device__ __forceinline__ void tt_load(void* dst, const void* map, int x, int h
                  "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_addr(bar))
                  : "memory");
 }
-// Values that are not finite become zeros in a staged tile (blocks of 64 columns x `rows` keys); true when there were any.
+// Values that are not finite become zeros in a staged tile; true when there were any.
 __device__ __forceinline__ bool tt_clean(uint8_t* tile, int bytes, int tid) {
     bool odd = false;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = tid * 16; i < bytes; i += TT_COPY * 16) {
         uint4* p = reinterpret_cast<uint4*>(tile + i);
         const uint4 v = *p;
+        // an exponent of ones carries into the sign's place
+        auto carry = [](unsigned w) { return (w & 0x7f807f80u) + 0x00800080u; };
+        if (!((carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & 0x80008000u)) continue;
         unsigned w[4] = {v.x, v.y, v.z, v.w};
-        bool hit = false;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, hit = true;
-            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, hit = true;
+            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u;
+            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu;
         }
-        if (hit) *p = make_uint4(w[0], w[1], w[2], w[3]);
-        odd |= hit;
+        *p = make_uint4(w[0], w[1], w[2], w[3]);
+        odd = true;
     }
     return odd;
 }
 
 // The largest of a row's scores in the KT columns from `ts` on; MASKED: of those it sees.
 template <int KT, bool MASKED>
-__device__ __forceinline__ float tt_max(const TreeArgs& a, const TreeSeg& s, unsigned ts, int node, int k0) {
+__device__ __forceinline__ float tt_max(unsigned ts, const unsigned (&words)[KT / 32]) {
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
     for (int q = 0; q < KT / 32; q++) {
         int v[32];
         tmem_ld(ts + q * 32, v);
-        const unsigned seen = MASKED ? tree_seen(a, s, node, k0 + q * 32) : FULL;
-        __syncwarp();
+        unsigned seen = FULL;
+        if (MASKED) {
+#pragma unroll
+            for (int i = 0; i < KT / 32; i++) seen = i == q ? words[i] : seen;
+        }
         tmem_landed(v);
 #pragma unroll
         for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], !MASKED || (seen >> i) & 1u ? __int_as_float(v[i]) : -INFINITY);
@@ -194,15 +199,18 @@ __device__ __forceinline__ float tt_max(const TreeArgs& a, const TreeSeg& s, uns
 }
 // The row's weights 2^(score * scale + base) in place of its scores; returns their sum.
 template <int KT, bool MASKED>
-__device__ __forceinline__ float tt_weights(const TreeArgs& a, const TreeSeg& s, unsigned ts, int node, int k0, float base) {
-    const float2 scale = make_float2(a.scale2, a.scale2), off = make_float2(base, base);
+__device__ __forceinline__ float tt_weights(unsigned ts, const unsigned (&words)[KT / 32], float scale2, float base) {
+    const float2 scale = make_float2(scale2, scale2), off = make_float2(base, base);
     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll 1
     for (int q = 0; q < KT / 32; q++) {
         int v[32];
         tmem_ld(ts + q * 32, v);
-        const unsigned seen = MASKED ? tree_seen(a, s, node, k0 + q * 32) : FULL;
-        __syncwarp();
+        unsigned seen = FULL;
+        if (MASKED) {
+#pragma unroll
+            for (int i = 0; i < KT / 32; i++) seen = i == q ? words[i] : seen;
+        }
         tmem_landed(v);
         unsigned w[16];
 #pragma unroll
@@ -454,13 +462,15 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
             const bool idle = !both && slot && s.rows <= TT_ROWS;            // the slot has no rows in this stretch
             const int jobs = idle ? 0 : both ? (it.n + 1 - slot) / 2 : it.n;
             for (int j = 0; j < jobs; j++) {
+                const int k0 = (it.tile + (both ? 2 * j + slot : j)) * KT;
+                const bool tree = k0 + KT > s.edge;
+                unsigned seen[KT / 32];
+                if (tree && any) tree_seen<KT / 32>(a, s, node, k0, seen);
                 if (ok) ok = wait(&s_full[slot], ns & 1u);
                 ns++;
                 tc_fence_after();
                 if (any) {
-                    const int k0 = (it.tile + (both ? 2 * j + slot : j)) * KT;
-                    const bool tree = k0 + KT > s.edge;
-                    const float mt = tree ? tt_max<KT, true>(a, s, ts, node, k0) : tt_max<KT, false>(a, s, ts, node, k0);
+                    const float mt = tree ? tt_max<KT, true>(ts, seen) : tt_max<KT, false>(ts, seen);
                     const bool grow = (mt - m) * a.scale2 > TT_GROWTH;
                     if (__any_sync(FULL, grow)) {
                         const float f = grow ? ex2((m - mt) * a.scale2) : 1.0f;
@@ -481,7 +491,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : -m * a.scale2;
-                    l += tree ? tt_weights<KT, true>(a, s, ts, node, k0, base) : tt_weights<KT, false>(a, s, ts, node, k0, base);
+                    l += tree ? tt_weights<KT, true>(ts, seen, a.scale2, base) : tt_weights<KT, false>(ts, seen, a.scale2, base);
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -510,43 +520,49 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 const bool fix = *reinterpret_cast<volatile int*>(&odd[item & 3]) == (int)item + 1;
                 const int orow = s.first + node, h = it.g * a.per_kv + row % a.per_kv;
                 const TreeOut<bf16> out(a, orow, h);
-                const float inv = it.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 float* piece = a.part + ((size_t)blockIdx.x * 2 + it.piece) * tree_piece_floats(a.block, a.vd);
 #pragma unroll 1
-                for (int q = both ? slot * 16 : 0; q < a.vd; q += both ? 32 : 16) {
-                    int v[16];
+                for (int q = both ? slot * 32 : 0; q < a.vd; q += both ? 64 : 32) {
+                    int v[32], w[32];
                     tmem_ld(o0 + q, v);
+                    if (other) tmem_ld(o1 + q, w);
                     tmem_landed(v);
-                    float o[16];
+                    float o[32];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = __int_as_float(v[i]) * f0;
+                    for (int i = 0; i < 32; i++) o[i] = __int_as_float(v[i]) * f0;
                     if (other) {
-                        tmem_ld(o1 + q, v);
-                        tmem_landed(v);
+                        tmem_landed(w);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = fmaf(__int_as_float(v[i]), f1, o[i]);
+                        for (int i = 0; i < 32; i++) o[i] = fmaf(__int_as_float(w[i]), f1, o[i]);
                     }
                     if (fix) {                        // warps agree on it
                         // values of attended nodes that are not finite (they entered the product as zeros)
                         const int k1 = min(s.len + s.n, (it.tile + it.n) * KT);
+#pragma unroll 1
                         for (int k = max(it.tile, s.edge / KT) * KT; k < k1; k++) {
-                            if (!(tree_seen(a, s, node, k) & 1u)) continue;
+                            unsigned sees[1];
+                            tree_seen<1>(a, s, node, k, sees);
+                            if (!(sees[0] & 1u)) continue;
                             const bf16* val = static_cast<const bf16*>(a.seq.table[s.b].cache) + (size_t)k * a.ld + a.kv_heads * a.kd + it.g * a.vd + q;
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
+                            for (int i = 0; i < 32; i++) {
                                 const float x = q + i < a.vd ? to_f(val[i]) : 0.0f;
                                 if (!isfinite(x)) o[i] += x;
                             }
                         }
                     }
                     if (mine) {
+                        if (it.whole) {
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4)
-                            if (q + i < a.vd) {
-                                const float4 x = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
-                                if (it.whole) out.put4at(q + i, x);
-                                else put4(piece + 2 * a.block + ((size_t)((q + i) / 4) * a.block + br) * 4, x);
-                            }
+                            for (int i = 0; i < 32; i += 4)
+                                if (q + i < a.vd) out.put4at(q + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
+                        } else {
+                            float* to4 = piece + 2 * a.block + ((size_t)(q / 4) * a.block + br) * 4;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4, to4 += a.block * 4)
+                                if (q + i < a.vd) put4(to4, make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                        }
                     }
                     __syncwarp();
                 }
