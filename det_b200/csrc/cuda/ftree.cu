@@ -44,8 +44,8 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
     float* V = K + TS_KEYS * ldk;                // [64][ldv]
     float* P = V + TS_KEYS * ldv;                // [RB][68]
     constexpr int LDP = TS_KEYS + 4;
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();                               // behind the wait: what k_ftree_merge reads ahead of its own is then there
     if (tid < 32) {
         const TreeShare w = tree_start(a, blockIdx.x, tid);
         if (tid == 0) share = w;
@@ -184,21 +184,22 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------ pieces
-constexpr int TM_THREADS = 512, TM_ROWS = 16;
+constexpr int TM_THREADS = 256, TM_ROWS = 8;
 // grid (key/value heads x groups of 16 rows of a block, segments).  The factors of the pieces first, then a thread per (row, four
 // values).  Bound by the latency of its two rounds of loads: a merge of 18 pieces of 80 rows x 8 heads takes MERGE_US.
 template <class T>
 __global__ void __launch_bounds__(TM_THREADS) k_ftree_merge(const TreeArgs a) {
     __shared__ float fac[TM_ROWS][TREE_CTAS];
     pdl_trigger();
-    pdl_wait();
+    // Where the pieces are follows from what the attention kernel has waited for before it let this one start.
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.x % a.kv_heads, r0 = blockIdx.x / a.kv_heads * TM_ROWS;
     long long before = 0, total = 0;
     TreeSeg s{};
     for (int i = lane; i < a.seq.seqs * a.blocks; i += 32) {
         const TreeSeg x = tree_seg(a, i);
-        total += x.tiles;
-        if (i < (int)blockIdx.y) before += x.tiles;
+        const int places = tree_places(a, x.tiles);
+        total += places;
+        if (i < (int)blockIdx.y) before += places;
         if (i == (int)blockIdx.y) s = x;
     }
 #pragma unroll
@@ -208,15 +209,22 @@ __global__ void __launch_bounds__(TM_THREADS) k_ftree_merge(const TreeArgs a) {
     }
     const int from = (int)blockIdx.y & 31, rows = min(TM_ROWS, __shfl_sync(FULL, s.rows, from) - r0), tiles = __shfl_sync(FULL, s.tiles, from);
     const int base_row = __shfl_sync(FULL, s.r0, from) + r0, first = __shfl_sync(FULL, s.first, from);
-    if (tiles <= 1 || rows <= 0) return;
     total *= a.kv_heads;
-    const long long share = tree_share(a, total), u0 = before * a.kv_heads + (long long)g * tiles;
-    const int c0 = (int)(u0 / share);
-    const long long left = u0 - c0 * share;
-    if (left + tiles <= share) return;                        // one CTA finished it
-    const int n = (int)((left + tiles + share - 1) / share);
+    const long long share = tree_share(a, total), begin = before * a.kv_heads + (long long)g * (tiles + a.turn), u0 = begin + a.turn;   // of its tiles
+    int c0, n;                                                // the first CTA and how many
+    bool second;                                              // the first CTA had tiles of the segment before
+    if (total < 1ll << 31) {
+        c0 = (int)((unsigned)u0 / (unsigned)share);
+        n = (int)((unsigned)(u0 + tiles - 1) / (unsigned)share) - c0 + 1;
+    } else {
+        c0 = (int)(u0 / share);
+        n = (int)((u0 + tiles - 1) / share) - c0 + 1;
+    }
+    second = c0 * share < begin;
+    pdl_wait();
+    if (tiles <= 1 || rows <= 0 || n == 1) return;
     const size_t size = tree_piece_floats(a.block, a.vd);
-    const float* head = a.part + ((size_t)c0 * 2 + (left ? 1 : 0)) * size;    // the others are their CTAs' first pieces
+    const float* head = a.part + ((size_t)c0 * 2 + (second ? 1 : 0)) * size;    // the others are their CTAs' first pieces
     const float* rest = a.part + (size_t)c0 * 2 * size;
     if (warp < rows) {
         float m = -INFINITY, l = 0.0f;
@@ -276,9 +284,10 @@ static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
     return launch_pdl_try(k_ftree_merge<T>, dim3(a.kv_heads * (a.block / TM_ROWS), a.seq.seqs * a.blocks), dim3(TM_THREADS), 0, q, 1, a);
 }
 // Rows of a block and keys of a tile.
-static void simt_shape(int rows, int* block, int* tile) {
+static void simt_shape(int rows, int* block, int* tile, int* turn) {
     *block = rows <= 16 ? 16 : 64;
     *tile = TS_KEYS;
+    *turn = 1;
 }
 
 }  // namespace detb
@@ -290,9 +299,9 @@ extern "C" {
 size_t det_f_tree_scratch_bytes(int heads, int kv_heads, int vdim, int max_nodes) {
     if (heads <= 0 || kv_heads <= 0 || vdim <= 0 || max_nodes <= 0) return 16;
     const int rows = (int)std::min((long long)max_nodes * (heads / kv_heads), 1ll << 24), vd = round8(vdim);
-    int block = 0, other = 0, tile = 0;
-    simt_shape(rows, &block, &tile);
-    ftree_tc_shape(rows, 8, vd, &other, &tile);      // the smallest keys have the largest blocks
+    int block = 0, other = 0, tile = 0, turn = 0;
+    simt_shape(rows, &block, &tile, &turn);
+    ftree_tc_shape(rows, 8, vd, &other, &tile, &turn);      // the smallest keys have the largest blocks
     block = std::max(block, other);
     return TREE_MAP_BYTES + TREE_CTAS * 2 * tree_piece_floats(block, vd) * sizeof(float);
 }
@@ -316,8 +325,8 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
               "q, out or scratch is NULL or misaligned");
     TreeArgs a{};
     a.kd = round8(op->dim); a.vd = round8(op->vdim);
-    if (op->dtype == DET_BF16) ftree_tc_shape((int)rows, a.kd, a.vd, &a.block, &a.tile);
-    else simt_shape((int)rows, &a.block, &a.tile);
+    if (op->dtype == DET_BF16) ftree_tc_shape((int)rows, a.kd, a.vd, &a.block, &a.tile, &a.turn);
+    else simt_shape((int)rows, &a.block, &a.tile, &a.turn);
     const long long blocks = (rows + a.block - 1) / a.block;
     DETB_TAKE(blocks * op->seq.seqs <= 65535, "too many rows");
     DETB_TAKE(runtime_ready(), "no usable device");

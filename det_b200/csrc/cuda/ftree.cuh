@@ -52,7 +52,9 @@ __device__ __forceinline__ TreePlace tree_place(const det_tree_ref& s, int row, 
 // its keys come in tiles.  The tiles of all (sequence, row block, key/value head) segments, in that order, are dealt out evenly: CTA
 // c takes `share` tiles from c * share on, whatever segments they belong to, so unequal lengths leave no CTA idle.  A segment that
 // falls to one CTA is finished there; of the others every CTA leaves a piece (maximum, sum, values per row) in scratch, and the
-// merge kernel adds the pieces in order of the keys.  A CTA has at most two such pieces, of its first and of its last segment.
+// merge kernel adds the pieces in order of the keys.  A CTA has at most two such pieces, of its first and of its last stretch.  A CTA that
+// passes from one segment to the next drains its pipeline in between: a segment counts for `turn` tiles more than it has, at its
+// beginning, so that such CTAs get fewer.
 constexpr int TREE_CTAS = 148;
 constexpr int TREE_SHARE = 2;      // tiles of a CTA at least, if there are enough
 
@@ -76,7 +78,7 @@ struct TreeArgs {
     void* maps;                    // [CTA][TREE_MAPS][2] tensor maps
     int* error_flag;
     int block, tile, blocks;       // rows of a block, keys of a tile, row blocks of the largest tree
-    int ctas;
+    int ctas, turn;
     det_tree_ref seq;
 };
 constexpr int TREE_MAPS = 8;
@@ -108,23 +110,26 @@ __device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, int seg) {
     s.tiles = s.rows > 0 ? (s.keys + a.tile - 1) / a.tile : 0;
     return s;
 }
-// Tiles of a CTA.
+// Places of a segment in the deal, for one key/value head.
+__device__ __forceinline__ int tree_places(const TreeArgs& a, int tiles) { return tiles > 0 ? tiles + a.turn : 0; }
+// Places of a CTA.
 __device__ __forceinline__ long long tree_share(const TreeArgs& a, long long total) {
-    return max((long long)TREE_SHARE, (total + a.ctas - 1) / a.ctas);
+    if (total < 1ll << 31) return max(TREE_SHARE, (int)(((unsigned)total + a.ctas - 1) / (unsigned)a.ctas));
+    return (total + a.ctas - 1) / a.ctas;
 }
 // Where a CTA's share begins and how long it is.  tree_start is called by a whole warp; every lane gets the result.
 struct TreeShare {
-    int seg, g, tile;              // segment, key/value head, tile within them
-    long long left;                // tiles of the share
+    int seg, g, place;             // segment, key/value head, place within them
+    long long left;                // places of the share
 };
 __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int lane) {
     const int segs = a.seq.seqs * a.blocks;
     long long total = 0;
-    int mine = 0;                                             // tiles of the lane's last segment
+    int mine = 0;                                             // places of the lane's last segment
     bool bad = false;
     for (int i = lane; i < segs; i += 32) {
         const TreeSeg s = tree_seg(a, i);
-        total += mine = s.tiles;
+        total += mine = tree_places(a, s.tiles);
         bad |= s.bad;
     }
     if (cta == 0 && bad) report_size(a.error_flag);
@@ -135,10 +140,10 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
     TreeShare w{0, 0, 0, 0};
     if (u0 >= total) return w;
     w.left = min(share, total - u0);
-    long long base = 0;                                       // tiles ahead of this round's segments
+    long long base = 0;                                       // places ahead of this round's segments
     for (int i = lane;; i += 32) {
-        const int tiles = i >= segs ? 0 : segs <= 32 ? mine : tree_seg(a, i).tiles;
-        long long sum = (long long)tiles * a.kv_heads;
+        const int places = i >= segs ? 0 : segs <= 32 ? mine : tree_places(a, tree_seg(a, i).tiles);
+        long long sum = (long long)places * a.kv_heads;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const long long v = __shfl_up_sync(FULL, sum, off);
@@ -146,12 +151,12 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
         }
         const unsigned holds = __ballot_sync(FULL, base + sum > u0);
         if (holds) {
-            const int src = __ffs(holds) - 1, per = __shfl_sync(FULL, tiles, src);
-            // tiles of the segment ahead of the share: below kv_heads * per, which fits 31 bits (per < 2^19, kv_heads <= 2^12)
-            const unsigned in = (unsigned)(u0 - __shfl_sync(FULL, base + sum - (long long)tiles * a.kv_heads, src));
+            const int src = __ffs(holds) - 1, per = __shfl_sync(FULL, places, src);
+            // places of the segment ahead of the share: below kv_heads * per, which fits 31 bits (per < 2^19, kv_heads <= 2^12)
+            const unsigned in = (unsigned)(u0 - __shfl_sync(FULL, base + sum - (long long)places * a.kv_heads, src));
             w.seg = i - lane + src;
             w.g = (int)(in / (unsigned)per);
-            w.tile = (int)(in % (unsigned)per);
+            w.place = (int)(in % (unsigned)per);
             return w;
         }
         base += __shfl_sync(FULL, sum, 31);
@@ -169,24 +174,27 @@ struct TreeWalk {
     bool begun;
 };
 __device__ __forceinline__ bool tree_next(const TreeArgs& a, TreeWalk& k, TreeItem& it) {
-    if (k.w.left <= 0) return false;
-    it.s = tree_seg(a, k.w.seg);
-    while (it.s.tiles == 0) {                                  // only segments behind the first can be empty
-        k.w.seg++;
+    do {
+        if (k.w.left <= 0) return false;
         it.s = tree_seg(a, k.w.seg);
-    }
-    it.g = k.w.g;
-    it.tile = k.w.tile;
-    it.n = (int)min((long long)(it.s.tiles - it.tile), k.w.left);
+        while (it.s.tiles == 0) {                              // only segments behind the first can be empty
+            k.w.seg++;
+            it.s = tree_seg(a, k.w.seg);
+        }
+        const int from = k.w.place, n = (int)min((long long)(it.s.tiles + a.turn - from), k.w.left);
+        it.g = k.w.g;
+        it.tile = max(0, from - a.turn);
+        it.n = max(0, from + n - a.turn) - it.tile;
+        k.w.left -= n;
+        k.w.place = 0;
+        if (++k.w.g == a.kv_heads) {
+            k.w.g = 0;
+            k.w.seg++;
+        }
+    } while (it.n == 0);                                       // the share ended ahead of the first tile
     it.whole = it.n == it.s.tiles;
     it.piece = k.begun ? 1 : 0;
     k.begun = true;
-    k.w.left -= it.n;
-    k.w.tile = 0;
-    if (++k.w.g == a.kv_heads) {
-        k.w.g = 0;
-        k.w.seg++;
-    }
     return true;
 }
 // Which of the 32 * W keys from c0 on a node sees, as bits; keys from the end of the tree on are never seen.  The words of the mask are
@@ -250,8 +258,8 @@ struct TreeOut {
 };
 __device__ __forceinline__ float4 scaled4(float4 v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
 
-// ftree_tc.cu: bfloat16 activations.  Rows of a block and keys of a tile are the kernel's.
-void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile);
+// ftree_tc.cu: bfloat16 activations.  Rows of a block, keys of a tile and the tiles that a turn costs are the kernel's.
+void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile, int* turn);
 cudaError_t ftree_tc_launch(const TreeArgs& a, cudaStream_t q);
 
 }  // namespace detb

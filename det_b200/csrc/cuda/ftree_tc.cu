@@ -197,6 +197,31 @@ __device__ __forceinline__ float tt_max(unsigned ts, const unsigned (&words)[KT 
     }
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
+// Weights of scores that are not masked in one pass: 2^(score * scale + base) into w, bfloat16 pairs, and their sum; returns the largest
+// score.
+template <int KT>
+__device__ __forceinline__ float tt_one_pass(unsigned ts, float scale2, float base, unsigned (&w)[KT / 2], float& total) {
+    const float2 scale = make_float2(scale2, scale2), off = make_float2(base, base);
+    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int q = 0; q < KT / 32; q++) {
+        int v[32];
+        tmem_ld(ts + q * 32, v);
+        tmem_landed(v);
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float a = __int_as_float(v[i]), b = __int_as_float(v[i + 1]);
+            asm("max.f32 %0, %0, %1, %2;" : "+f"(top[(i >> 1) & 1]) : "f"(a), "f"(b));
+            const float2 x = fma2(make_float2(a, b), scale, off);
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], p);
+            w[q * 16 + i / 2] = pack_bf(p.x, p.y);
+        }
+    }
+    total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    return fmaxf(top[0], top[1]);
+}
 // The row's weights 2^(score * scale + base) in place of its scores; returns their sum.
 template <int KT, bool MASKED>
 __device__ __forceinline__ float tt_weights(unsigned ts, const unsigned (&words)[KT / 32], float scale2, float base) {
@@ -240,9 +265,9 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
     auto &odd = tb.odd;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long wl = wait_limit(a.error_flag);
-    pdl_trigger();
     if (smem_addr(Qs) & 1023) {                      // the layout of the operands needs it
         pdl_wait();
+        pdl_trigger();
         if (threadIdx.x == 0) report_size(a.error_flag);
         return;
     }
@@ -265,6 +290,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
     }
     if (warp == PRODUCTS) tmem_alloc(&tb.tmem_slot, 512);
     pdl_wait();
+    pdl_trigger();                                   // behind the wait: what k_ftree_merge reads ahead of its own is then there
     if (warp == 0) {
         const TreeShare w = tree_start(a, blockIdx.x, lane);
         if (lane == 0) tb.share = w;
@@ -470,28 +496,50 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 ns++;
                 tc_fence_after();
                 if (any) {
-                    const float mt = tree ? tt_max<KT, true>(ts, seen) : tt_max<KT, false>(ts, seen);
-                    const bool grow = (mt - m) * a.scale2 > TT_GROWTH;
-                    if (__any_sync(FULL, grow)) {
-                        const float f = grow ? ex2((m - mt) * a.scale2) : 1.0f;
-                        if (grow) m = mt;
-                        l *= f;
-                        __syncwarp();
-                        if (j > 0) {
-#pragma unroll 1
-                            for (int q = 0; q < a.vd; q += 16) {
-                                int v[16];
-                                tmem_ld(to + q, v);
-                                tmem_landed(v);
-                                unsigned w[16];
+                    // as a rule the reference holds: weights in one pass, stored when the tile's maximum is known not to have outgrown it
+                    float mt;
+                    bool done = false;
+                    if (!tree && j > 0) {
+                        unsigned w[KT / 2];
+                        float sum;
+                        mt = tt_one_pass<KT>(ts, a.scale2, m == -INFINITY ? 0.0f : -m * a.scale2, w, sum);
+                        done = !__any_sync(FULL, (mt - m) * a.scale2 > TT_GROWTH);
+                        if (done) {
+                            l += sum;
 #pragma unroll
-                                for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__int_as_float(v[i]) * f);
-                                tmem_st(to + q, w);
+                            for (int q = 0; q < KT / 32; q++) {
+                                unsigned x[16];
+#pragma unroll
+                                for (int i = 0; i < 16; i++) x[i] = w[q * 16 + i];
+                                tmem_st(ts + q * 16, x);
                             }
                         }
+                    } else {
+                        mt = tree ? tt_max<KT, true>(ts, seen) : tt_max<KT, false>(ts, seen);
                     }
-                    const float base = m == -INFINITY ? 0.0f : -m * a.scale2;
-                    l += tree ? tt_weights<KT, true>(ts, seen, a.scale2, base) : tt_weights<KT, false>(ts, seen, a.scale2, base);
+                    if (!done) {
+                        const bool grow = (mt - m) * a.scale2 > TT_GROWTH;
+                        if (__any_sync(FULL, grow)) {
+                            const float f = grow ? ex2((m - mt) * a.scale2) : 1.0f;
+                            if (grow) m = mt;
+                            l *= f;
+                            __syncwarp();
+                            if (j > 0) {
+#pragma unroll 1
+                                for (int q = 0; q < a.vd; q += 16) {
+                                    int v[16];
+                                    tmem_ld(to + q, v);
+                                    tmem_landed(v);
+                                    unsigned w[16];
+#pragma unroll
+                                    for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__int_as_float(v[i]) * f);
+                                    tmem_st(to + q, w);
+                                }
+                            }
+                        }
+                        const float base = m == -INFINITY ? 0.0f : -m * a.scale2;
+                        l += tree ? tt_weights<KT, true>(ts, seen, a.scale2, base) : tt_weights<KT, false>(ts, seen, a.scale2, base);
+                    }
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -585,10 +633,11 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
 }
 
 // ------------------------------------------------------------------------------------------------------ host side
-void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile) {
+void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile, int* turn) {
     const bool wide = kd > 128 || vd > 128;
     *block = wide || rows <= TT_ROWS ? TT_ROWS : 2 * TT_ROWS;
     *tile = wide ? 64 : 128;
+    *turn = *block == TT_ROWS ? 4 : 2;
 }
 
 // A cache's keys or values (`size` elements a head) as [rows][heads][size], boxes of 64 elements of one head x `box` rows, zeros outside.
