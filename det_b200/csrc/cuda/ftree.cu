@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
                 if (it.whole) {
                     out.put4at(c, scaled4(o[i][j], inv));
                 } else {
-                    put4(piece + 2 * RB + ((size_t)(c / 4) * RB + r) * 4, o[i][j]);
+                    put4(piece + 2 * RB + (size_t)r * a.vd + c, o[i][j]);
                 }
             }
         }
@@ -184,86 +184,98 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------ pieces
-constexpr int TM_THREADS = 256, TM_ROWS = 8;
-// grid (key/value heads x groups of 16 rows of a block, segments).  The factors of the pieces first, then a thread per (row, four
-// values).  Bound by the latency of its two rounds of loads: a merge of 18 pieces of 80 rows x 8 heads takes MERGE_US.
-template <class T>
-__global__ void __launch_bounds__(TM_THREADS) k_ftree_merge(const TreeArgs a) {
-    __shared__ float fac[TM_ROWS][TREE_CTAS];
+constexpr int TM_WARPS = 8, TM_ML = (TREE_CTAS + 31) / 32;
+__device__ __forceinline__ void add4(float4& o, float f, float4 x) {
+    o.x = fmaf(f, x.x, o.x);
+    o.y = fmaf(f, x.y, o.y);
+    o.z = fmaf(f, x.z, o.z);
+    o.w = fmaf(f, x.w, o.w);
+}
+// grid (X, groups of `per` rows).  With few segments X counts them; else block x looks at the border between the shares of CTAs x and
+// x + 1, and when it is the first border inside a segment, the block adds that segment's pieces.  WIDE: the warps of a block share the
+// pieces of one row after the other (few rows); else a warp has rows of its own.  Bound by the latency of two rounds of loads; where the
+// pieces are follows from what the attention kernel has waited for before it let this one start.
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs a, int per, int by_segment) {
+    __shared__ float4 sum[WIDE ? TM_WARPS : 1][64];
+    __shared__ float fac[TM_WARPS][TM_ML * 32];
     pdl_trigger();
-    // Where the pieces are follows from what the attention kernel has waited for before it let this one start.
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.x % a.kv_heads, r0 = blockIdx.x / a.kv_heads * TM_ROWS;
-    long long before = 0, total = 0;
-    TreeSeg s{};
-    for (int i = lane; i < a.seq.seqs * a.blocks; i += 32) {
-        const TreeSeg x = tree_seg(a, i);
-        const int places = tree_places(a, x.tiles);
-        total += places;
-        if (i < (int)blockIdx.y) before += places;
-        if (i == (int)blockIdx.y) s = x;
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        total += __shfl_xor_sync(FULL, total, off);
-        before += __shfl_xor_sync(FULL, before, off);
-    }
-    const int from = (int)blockIdx.y & 31, rows = min(TM_ROWS, __shfl_sync(FULL, s.rows, from) - r0), tiles = __shfl_sync(FULL, s.tiles, from);
-    const int base_row = __shfl_sync(FULL, s.r0, from) + r0, first = __shfl_sync(FULL, s.first, from);
-    total *= a.kv_heads;
-    const long long share = tree_share(a, total), begin = before * a.kv_heads + (long long)g * (tiles + a.turn), u0 = begin + a.turn;   // of its tiles
-    int c0, n;                                                // the first CTA and how many
-    bool second;                                              // the first CTA had tiles of the segment before
-    if (total < 1ll << 31) {
-        c0 = (int)((unsigned)u0 / (unsigned)share);
-        n = (int)((unsigned)(u0 + tiles - 1) / (unsigned)share) - c0 + 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long share;
+    int cta = blockIdx.x;                                     // the CTA ahead of the border
+    TreeShare w;
+    if (by_segment) {
+        w = tree_start(a, -1, lane, &share, blockIdx.x);
+        cta = w.cta;
     } else {
-        c0 = (int)(u0 / share);
-        n = (int)((u0 + tiles - 1) / share) - c0 + 1;
+        w = tree_start(a, cta + 1, lane, &share);
     }
-    second = c0 * share < begin;
+    const TreeSeg s = tree_seg(a, w.seg);
+    // in places from the beginning of the segment: the border lies at w.place, the tiles at turn .. turn + tiles - 1
+    const int r0 = blockIdx.y * per, r1 = min(s.rows, r0 + per);
+    const bool mine = w.left > 0 && w.place > a.turn && w.place - share <= a.turn;
     pdl_wait();
-    if (tiles <= 1 || rows <= 0 || n == 1) return;
+    if (!mine || r0 >= r1) return;
+    const int n = 1 + (int)(share < (1 << 30) ? (unsigned)(s.tiles + a.turn - w.place + (int)share - 1) / (unsigned)share : 1);   // pieces
     const size_t size = tree_piece_floats(a.block, a.vd);
-    const float* head = a.part + ((size_t)c0 * 2 + (second ? 1 : 0)) * size;    // the others are their CTAs' first pieces
-    const float* rest = a.part + (size_t)c0 * 2 * size;
-    if (warp < rows) {
+    // the CTA ahead of the border had tiles of the segment before when its share began ahead of this one
+    const float* head = a.part + ((size_t)cta * 2 + (w.place < share ? 1 : 0)) * size;
+    const float* rest = a.part + (size_t)cta * 2 * size;                      // the others are their CTAs' first pieces
+    const int vq = a.vd / 4;
+    for (int r = WIDE ? r0 : r0 + warp; r < r1; r += WIDE ? 1 : TM_WARPS) {
+        float2 ml[TM_ML];
         float m = -INFINITY, l = 0.0f;
-        float2 ml[(TREE_CTAS + 31) / 32];
 #pragma unroll
-        for (int i = 0; i < (TREE_CTAS + 31) / 32; i++) {
+        for (int i = 0; i < TM_ML; i++) {
             const int c = i * 32 + lane;
-            ml[i] = c < n ? reinterpret_cast<const float2*>(c ? rest + c * 2 * size : head)[r0 + warp] : make_float2(-INFINITY, 0.0f);
-            m = fmaxf(m, ml[i].x);
+            ml[i] = c < n ? reinterpret_cast<const float2*>(c ? rest + c * 2 * size : head)[r] : make_float2(-INFINITY, 0.0f);
         }
+#pragma unroll
+        for (int i = 0; i < TM_ML; i++) m = fmaxf(m, ml[i].x);
         m = warp_max(m);
         if (m == -INFINITY) m = 0.0f;                         // a row without keys
+        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < (TREE_CTAS + 31) / 32; i++) {
-            ml[i].x = exp2f(ml[i].x - m);
-            l = fmaf(ml[i].x, ml[i].y, l);
+        for (int i = 0; i < TM_ML; i++) {
+            const float f = exp2f(ml[i].x - m);
+            fac[warp][i * 32 + lane] = f;
+            l = fmaf(f, ml[i].y, l);
         }
         l = warp_sum(l);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-        for (int i = 0; i < (TREE_CTAS + 31) / 32; i++)
-            if (i * 32 + lane < n) fac[warp][i * 32 + lane] = ml[i].x * inv;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * (a.vd / 4); i += TM_THREADS) {
-        const int v = i / rows, r = i - v * rows;
-        const size_t at = 2 * a.block + ((size_t)v * a.block + r0 + r) * 4;
-        float4 o = scaled4(load4(head + at), fac[r][0]);
-#pragma unroll 8
-        for (int c = 1; c < n; c++) {
-            const float4 x = load4(rest + c * 2 * size + at);
-            const float w = fac[r][c];
-            o.x = fmaf(w, x.x, o.x);
-            o.y = fmaf(w, x.y, o.y);
-            o.z = fmaf(w, x.z, o.z);
-            o.w = fmaf(w, x.w, o.w);
+        __syncwarp();
+        const size_t at = 2 * a.block + (size_t)r * a.vd + lane * 4;
+        const bool lo = lane < vq, hi = 32 + lane < vq;
+        float4 o0 = make_float4(0, 0, 0, 0), o1 = o0;
+        int c = WIDE ? warp : 0;
+        if (c == 0) {
+            if (lo) o0 = scaled4(load4(head + at), fac[warp][0]);
+            if (hi) o1 = scaled4(load4(head + at + 128), fac[warp][0]);
+            c += WIDE ? TM_WARPS : 1;
         }
-        const int row = base_row + r, node = (int)(row * a.per_magic >> 32);
-        TreeOut<T>(a, first + node, g * a.per_kv + row - node * a.per_kv).put4at(v * 4, o);
+#pragma unroll 4
+        for (; c < n; c += WIDE ? TM_WARPS : 1) {
+            const float* p = rest + c * 2 * size + at;
+            if (lo) add4(o0, fac[warp][c], load4(p));
+            if (hi) add4(o1, fac[warp][c], load4(p + 128));
+        }
+        const int row = s.r0 + r, node = (int)(row * a.per_magic >> 32), h = w.g * a.per_kv + row - node * a.per_kv;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (!WIDE) {
+            const TreeOut<T> out(a, s.first + node, h);
+            if (lo) out.put4at(lane * 4, scaled4(o0, inv));
+            if (hi) out.put4at(128 + lane * 4, scaled4(o1, inv));
+            continue;
+        }
+        __syncthreads();
+        sum[warp][lane] = o0;
+        sum[warp][32 + lane] = o1;
+        __syncthreads();
+        if ((int)threadIdx.x < vq) {
+            float4 x = sum[0][threadIdx.x];
+#pragma unroll
+            for (int i = 1; i < (WIDE ? TM_WARPS : 1); i++) add4(x, 1.0f, sum[i][threadIdx.x]);
+            TreeOut<T>(a, s.first + node, h).put4at(threadIdx.x * 4, scaled4(x, inv));
+        }
     }
 }
 
@@ -281,7 +293,13 @@ static cudaError_t launch_simt_v(const TreeArgs& a, cudaStream_t q) {
 }
 template <class T>
 static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
-    return launch_pdl_try(k_ftree_merge<T>, dim3(a.kv_heads * (a.block / TM_ROWS), a.seq.seqs * a.blocks), dim3(TM_THREADS), 0, q, 1, a);
+    if (a.ctas == 1) return cudaSuccess;
+    const long long segs = (long long)a.seq.seqs * a.blocks * a.kv_heads;
+    const int by_segment = segs < a.ctas - 1, x = by_segment ? (int)segs : a.ctas - 1, rows = std::min(a.block, a.seq.max_nodes * a.per_kv);
+    if (rows * x <= 4 * TREE_CTAS)                             // a row per block, about four blocks on an SM
+        return launch_pdl_try(k_ftree_merge<T, true>, dim3(x, rows), dim3(TM_WARPS * 32), 0, q, 1, a, 1, by_segment);
+    const int per = TM_WARPS * std::max(1, rows * x / (TM_WARPS * 4 * TREE_CTAS));
+    return launch_pdl_try(k_ftree_merge<T, false>, dim3(x, (rows + per - 1) / per), dim3(TM_WARPS * 32), 0, q, 1, a, per, by_segment);
 }
 // Rows of a block and keys of a tile.
 static void simt_shape(int rows, int* block, int* tile, int* turn) {

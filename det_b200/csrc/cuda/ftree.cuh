@@ -83,7 +83,7 @@ struct TreeArgs {
 };
 constexpr int TREE_MAPS = 8;
 constexpr size_t TREE_MAP_BYTES = (size_t)TREE_CTAS * TREE_MAPS * 2 * 128;
-// A piece: {maximum, sum}[block] | values[vd / 4][block][4].
+// A piece: {maximum, sum}[block] | values[block][vd].
 __host__ __device__ constexpr size_t tree_piece_floats(int block, int vd) { return (size_t)block * (2 + vd); }
 
 struct TreeSeg {
@@ -121,8 +121,10 @@ __device__ __forceinline__ long long tree_share(const TreeArgs& a, long long tot
 struct TreeShare {
     int seg, g, place;             // segment, key/value head, place within them
     long long left;                // places of the share
+    int cta;                       // whose share it is
 };
-__device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int lane) {
+// With `segment` >= 0 it finds the share that begins first inside that segment (counted with the key/value heads) behind its first tile.
+__device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int lane, long long* share_out = nullptr, int segment = -1) {
     const int segs = a.seq.seqs * a.blocks;
     long long total = 0;
     int mine = 0;                                             // places of the lane's last segment
@@ -136,10 +138,29 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(FULL, total, off);
     total *= a.kv_heads;
-    const long long share = tree_share(a, total), u0 = cta * share;
-    TreeShare w{0, 0, 0, 0};
+    const long long share = tree_share(a, total);
+    if (share_out) *share_out = share;
+    TreeShare w{0, 0, 0, 0, 0};
+    if (segment >= 0) {
+        w.seg = segment / a.kv_heads;
+        w.g = segment - w.seg * a.kv_heads;
+        long long before = 0;
+        for (int i = lane; i < w.seg; i += 32) before += tree_places(a, tree_seg(a, i).tiles);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) before += __shfl_xor_sync(FULL, before, off);
+        const int places = tree_places(a, tree_seg(a, w.seg).tiles);
+        const long long begin = before * a.kv_heads + (long long)w.g * places, first = begin + a.turn;   // its first tile
+        if (places == 0) return w;
+        w.cta = first + places < 1ll << 31 ? (int)((unsigned)first / (unsigned)share) : (int)(first / share);
+        const long long border = (w.cta + 1) * share;
+        w.place = (int)(border - begin);
+        w.left = border < begin + places ? 1 : 0;
+        return w;
+    }
+    const long long u0 = cta * share;
     if (u0 >= total) return w;
     w.left = min(share, total - u0);
+    w.cta = cta;
     long long base = 0;                                       // places ahead of this round's segments
     for (int i = lane;; i += 32) {
         const int places = i >= segs ? 0 : segs <= 32 ? mine : tree_places(a, tree_seg(a, i).tiles);

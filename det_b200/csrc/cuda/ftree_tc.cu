@@ -151,9 +151,10 @@ __device__ __forceinline__ void tt_maps(const CUtensorMap& mk, const CUtensorMap
 #pragma unroll
     for (int i = 0; i < 2; i++) asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(to + i * 128) : "memory");
 }
-__device__ __forceinline__ void tt_load(void* dst, const void* map, int x, int head, int row, unsigned long long* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
-                 "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_addr(bar))
+__device__ __forceinline__ void tt_load(void* dst, const void* map, int x, int head, int row, unsigned long long* bar, unsigned long long policy) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(
+                     smem_addr(dst)),
+                 "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_addr(bar)), "l"(policy)
                  : "memory");
 }
 // Values that are not finite become zeros in a staged tile; true when there were any.
@@ -312,6 +313,10 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
         unsigned c = 0, sn = 0, phase = 0;           // tiles issued, place in the ring
         int seq = -1, maps = 0;
         unsigned char* map = nullptr;
+        // keys that one row block reads are read once: they leave the L2 cache to the pieces and to the next kernels
+        unsigned long long policy;
+        if (a.blocks == 1) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+        else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
         while (ok && tree_next(a, walk, it)) {
             const TreeSeg& s = it.s;
             if (s.b != seq) {
@@ -332,7 +337,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                     mbar_expect_tx(bar, blocks * KT * 128);
                     if (!look) mbar_arrive(bar);
                     for (int i = 0; i < blocks; i++)
-                        tt_load(ring + (size_t)sn * sh.stage_bytes + i * KT * 128, map + (value ? 128 : 0), i * 64, it.g, k0, bar);
+                        tt_load(ring + (size_t)sn * sh.stage_bytes + i * KT * 128, map + (value ? 128 : 0), i * 64, it.g, k0, bar, policy);
                     c++;
                     if (++sn == (unsigned)sh.stages) sn = 0, phase ^= 1u;
                 };
@@ -606,10 +611,10 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                             for (int i = 0; i < 32; i += 4)
                                 if (q + i < a.vd) out.put4at(q + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
                         } else {
-                            float* to4 = piece + 2 * a.block + ((size_t)(q / 4) * a.block + br) * 4;
+                            float* to4 = piece + 2 * a.block + (size_t)br * a.vd + q;
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4, to4 += a.block * 4)
-                                if (q + i < a.vd) put4(to4, make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                            for (int i = 0; i < 32; i += 4)
+                                if (q + i < a.vd) put4(to4 + i, make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
                         }
                     }
                     __syncwarp();
