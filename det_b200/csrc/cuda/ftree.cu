@@ -1,9 +1,9 @@
 // Attention of a step of drafted tokens (include/det_b200.h, det_ftree_op): one pass over the keys with the running maximum and sum of
 // the softmax, in 32-bit.  ftree.cuh says how the work is dealt out.
 //
+//   k_ftree_few    bfloat16, up to 16 rows per key/value head: ftree_few.cu.
 //   k_ftree_tc     bfloat16: ftree_tc.cu.
-//   k_ftree_simt   32-bit products on the CUDA cores: 256 threads over a tile of query rows x 64 keys, keys and values staged in
-//                  shared memory.
+//   k_ftree_simt   fp32: products on the CUDA cores, 256 threads over a tile of query rows x 64 keys.
 //   k_ftree_merge  adds the pieces of the segments that several CTAs shared.
 #include "ftree.cuh"
 #include <algorithm>
@@ -13,8 +13,8 @@ namespace detb {
 
 constexpr int TS_KEYS = 64, TS_THREADS = 256;
 
-static size_t simt_smem(int block, int kd, int vd) {
-    return ((size_t)(block + TS_KEYS) * (kd + 4) + (size_t)TS_KEYS * (vd + 4) + (size_t)block * (TS_KEYS + 4)) * sizeof(float);
+static size_t simt_smem(int block, int kd, int vd, int stages) {
+    return ((size_t)block * (kd + 4) + (size_t)stages * TS_KEYS * (kd + vd + 8) + (size_t)block * (TS_KEYS + 4)) * sizeof(float);
 }
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
@@ -31,19 +31,37 @@ __device__ __forceinline__ float row_sum(float v) {
     for (int off = 8; off > 0; off >>= 1) v += __shfl_xor_sync(FULL, v, off);
     return v;
 }
+__device__ __forceinline__ void copy16(float* dst, const float* src, int bytes) {      // what is missing of 16 bytes becomes zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
+}
+// `rows` rows of n floats (a multiple of 4), `ld` apart, into rows of n + 4; rows past `have` become zeros
+__device__ __forceinline__ void copy_rows(float* dst, const float* src, size_t ld, int n, int rows, int have) {
+    const int pieces = n / 4, dr = TS_THREADS / pieces, dc = TS_THREADS - dr * pieces;
+    int r = threadIdx.x / pieces, c = threadIdx.x - r * pieces;
+    while (r < rows) {
+        copy16(dst + r * (n + 4) + c * 4, r < have ? src + r * ld + c * 4 : src, r < have ? 16 : 0);
+        r += dr;
+        c += dc;
+        if (c >= pieces) {
+            c -= pieces;
+            r++;
+        }
+    }
+}
 
-// Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.
+// Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.  With two stages the next tile's copies run
+// beside the products of this one.  Bound by the fp32 multiply-adds (a key costs all rows of the block, 16 TR, whatever is in them).
 template <int TR, int VJ>
-__global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
+__global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int stages) {
     extern __shared__ __align__(16) float tsm[];
     __shared__ TreeShare share;
-    constexpr int RB = 16 * TR;
+    __shared__ int odd;                          // a staged value that not every row sees was not finite
+    constexpr int RB = 16 * TR, LDP = TS_KEYS + 4;
     const int ldk = a.kd + 4, ldv = a.vd + 4, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     float* Q = tsm;                              // [RB][ldk]
-    float* K = Q + RB * ldk;                     // [64][ldk]
-    float* V = K + TS_KEYS * ldk;                // [64][ldv]
-    float* P = V + TS_KEYS * ldv;                // [RB][68]
-    constexpr int LDP = TS_KEYS + 4;
+    float* P = Q + RB * ldk;                     // [RB][LDP]
+    float* KV = P + RB * LDP;                    // [stage] K [64][ldk] | V [64][ldv]
+    const int stage_floats = TS_KEYS * (ldk + ldv);
     pdl_wait();
     pdl_trigger();                               // behind the wait: what k_ftree_merge reads ahead of its own is then there
     if (tid < 32) {
@@ -57,12 +75,23 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
         const TreeSeg& s = it.s;
         const float* cache = static_cast<const float*>(a.seq.table[s.b].cache);
         const float* q = static_cast<const float*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
+        auto fetch = [&](int t, int stage) {
+            if (t < it.tile + it.n) {
+                const int k0 = t * TS_KEYS, have = s.len + s.n - k0;
+                const float* rows = cache + (size_t)k0 * a.ld;
+                copy_rows(KV + stage * stage_floats, rows + it.g * a.kd, a.ld, a.kd, TS_KEYS, have);
+                copy_rows(KV + stage * stage_floats + TS_KEYS * ldk, rows + a.kv_heads * a.kd + it.g * a.vd, a.ld, a.vd, TS_KEYS, have);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
         __syncthreads();
+        if (tid == 0) odd = 0;
+        fetch(it.tile, 0);
         for (int i = tid; i < RB * (a.kd / 4); i += TS_THREADS) {
-            const int r = i / (a.kd / 4), e = (i - r * (a.kd / 4)) * 4, row = s.r0 + r;
+            const int r = i / (a.kd / 4), e = (i - r * (a.kd / 4)) * 4, row = s.r0 + r, node = (int)(row * a.per_magic >> 32);
             float4 v = make_float4(0, 0, 0, 0);
-            if (r < s.rows) v = load4(q + (size_t)(row / a.per_kv) * a.ldq + (row % a.per_kv) * a.kd + e);
-            *reinterpret_cast<float4*>(Q + r * ldk + e) = v;
+            if (r < s.rows) v = load4(q + (size_t)node * a.ldq + (row - node * a.per_kv) * a.kd + e);
+            put4(Q + r * ldk + e, v);
         }
         float m[TR], l[TR];
         float4 o[TR][VJ];
@@ -73,26 +102,30 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
 #pragma unroll
             for (int j = 0; j < VJ; j++) o[i][j] = make_float4(0, 0, 0, 0);
         }
-        for (int t = it.tile; t < it.tile + it.n; t++) {
-            const int k0 = t * TS_KEYS, last = s.len + s.n;
+        for (int t = it.tile, stage = 0; t < it.tile + it.n; t++) {
+            const int k0 = t * TS_KEYS;
             const bool tree = k0 + TS_KEYS > s.edge;
-            __syncthreads();
-            const float* kp = cache + (size_t)k0 * a.ld + it.g * a.kd;
-            for (int i = tid; i < TS_KEYS * (a.kd / 4); i += TS_THREADS) {
-                const int k = i / (a.kd / 4), e = (i - k * (a.kd / 4)) * 4;
-                *reinterpret_cast<float4*>(K + k * ldk + e) = k0 + k < last ? load4(kp + (size_t)k * a.ld + e) : make_float4(0, 0, 0, 0);
-            }
-            const float* vp = cache + (size_t)k0 * a.ld + a.kv_heads * a.kd + it.g * a.vd;
-            for (int i = tid; i < TS_KEYS * (a.vd / 4); i += TS_THREADS) {
-                const int k = i / (a.vd / 4), e = (i - k * (a.vd / 4)) * 4;
-                *reinterpret_cast<float4*>(V + k * ldv + e) = k0 + k < last ? load4(vp + (size_t)k * a.ld + e) : make_float4(0, 0, 0, 0);
+            float* K = KV + stage * stage_floats;
+            float* V = K + TS_KEYS * ldk;
+            if (stages == 2) {
+                fetch(t + 1, stage ^ 1);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
             __syncthreads();
+            if (tree) {                          // a weight of zero does not undo a value that is not finite
+                for (int i = tid; i < TS_KEYS * a.vd; i += TS_THREADS) {
+                    float* p = V + i / a.vd * ldv + i % a.vd;
+                    if (!isfinite(*p)) *p = 0.0f, odd = 1;
+                }
+            }
             float sc[TR][4];
 #pragma unroll
             for (int i = 0; i < TR; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) sc[i][j] = 0.0f;
+#pragma unroll 2
             for (int e = 0; e < a.kd; e += 4) {
                 float4 kv[4];
 #pragma unroll
@@ -109,8 +142,8 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
                 const int r = ty + 16 * i;
                 unsigned seen[2] = {FULL, FULL};
                 if (tree) {
-                    const int node = (s.r0 + min(r, s.rows - 1)) / a.per_kv;
-                    tree_seen<2>(a, s, node, k0, seen);
+                    const int row = s.r0 + min(r, s.rows - 1);
+                    tree_seen<2>(a, s, (int)(row * a.per_magic >> 32), k0, seen);
                 }
                 float mx = m[i];
 #pragma unroll
@@ -123,12 +156,7 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
                 m[i] = mx;
                 l[i] *= f;
 #pragma unroll
-                for (int j = 0; j < VJ; j++) {
-                    o[i][j].x *= f;
-                    o[i][j].y *= f;
-                    o[i][j].z *= f;
-                    o[i][j].w *= f;
-                }
+                for (int j = 0; j < VJ; j++) o[i][j] = scaled4(o[i][j], f);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float p = exp2f(sc[i][j] - base);
@@ -137,47 +165,65 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
                 }
             }
             __syncthreads();
-            for (int k = 0; k < TS_KEYS; k++) {
-                float4 v[VJ];
+            for (int k = 0; k < TS_KEYS; k += 4) {
+                float4 p[TR];
+#pragma unroll
+                for (int i = 0; i < TR; i++) p[i] = load4(P + (ty + 16 * i) * LDP + k);
 #pragma unroll
                 for (int j = 0; j < VJ; j++) {
                     const int c = 4 * tx + 64 * j;
-                    v[j] = c < a.vd ? load4(V + k * ldv + c) : make_float4(0, 0, 0, 0);
-                }
+                    if (c >= a.vd) continue;
+                    const float4 v0 = load4(V + k * ldv + c), v1 = load4(V + (k + 1) * ldv + c), v2 = load4(V + (k + 2) * ldv + c),
+                                 v3 = load4(V + (k + 3) * ldv + c);
 #pragma unroll
-                for (int i = 0; i < TR; i++) {
-                    const float p = P[(ty + 16 * i) * LDP + k];
-                    if (tree && p == 0.0f) continue;          // a masked node's value may be anything
-#pragma unroll
-                    for (int j = 0; j < VJ; j++) {
-                        o[i][j].x = fmaf(p, v[j].x, o[i][j].x);
-                        o[i][j].y = fmaf(p, v[j].y, o[i][j].y);
-                        o[i][j].z = fmaf(p, v[j].z, o[i][j].z);
-                        o[i][j].w = fmaf(p, v[j].w, o[i][j].w);
+                    for (int i = 0; i < TR; i++) {
+                        add4(o[i][j], p[i].x, v0);
+                        add4(o[i][j], p[i].y, v1);
+                        add4(o[i][j], p[i].z, v2);
+                        add4(o[i][j], p[i].w, v3);
                     }
                 }
             }
+            if (stages == 2) {
+                stage ^= 1;
+            } else {
+                __syncthreads();
+                fetch(t + 1, 0);
+            }
+            if (stages == 2) __syncthreads();    // the stage that the next round fills has been read
         }
         float* piece = a.part + ((size_t)blockIdx.x * 2 + it.piece) * tree_piece_floats(RB, a.vd);
+        const bool fix = odd != 0;
 #pragma unroll
         for (int i = 0; i < TR; i++) {
-            const int r = ty + 16 * i, row = s.r0 + r;
+            const int r = ty + 16 * i, row = s.r0 + min(r, s.rows - 1), node = (int)(row * a.per_magic >> 32);
             const float sum = row_sum(l[i]);
             if (r >= s.rows) continue;
-            if (!it.whole && tx == 0) {
-                reinterpret_cast<float2*>(piece)[r] = make_float2(m[i], sum);
-            }
+            if (fix)                             // values of attended keys that are not finite (they entered the product as zeros)
+                for (int k = max(it.tile, s.edge / TS_KEYS) * TS_KEYS; k < min(s.len + s.n, (it.tile + it.n) * TS_KEYS); k++) {
+                    unsigned sees[1];
+                    tree_seen<1>(a, s, node, k, sees);
+                    if (!(sees[0] & 1u)) continue;
+#pragma unroll
+                    for (int j = 0; j < VJ; j++) {
+                        const int c = 4 * tx + 64 * j;
+                        if (c >= a.vd) continue;
+                        const float4 x = load4(cache + (size_t)k * a.ld + a.kv_heads * a.kd + it.g * a.vd + c);
+                        if (!isfinite(x.x)) o[i][j].x += x.x;
+                        if (!isfinite(x.y)) o[i][j].y += x.y;
+                        if (!isfinite(x.z)) o[i][j].z += x.z;
+                        if (!isfinite(x.w)) o[i][j].w += x.w;
+                    }
+                }
+            if (!it.whole && tx == 0) reinterpret_cast<float2*>(piece)[r] = make_float2(m[i], sum);
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // no key seen
-            const TreeOut<float> out(a, s.first + row / a.per_kv, it.g * a.per_kv + row % a.per_kv);
+            const TreeOut<float> out(a, s.first + node, it.g * a.per_kv + row - node * a.per_kv);
 #pragma unroll
             for (int j = 0; j < VJ; j++) {
                 const int c = 4 * tx + 64 * j;
                 if (c >= a.vd) continue;
-                if (it.whole) {
-                    out.put4at(c, scaled4(o[i][j], inv));
-                } else {
-                    put4(piece + 2 * RB + (size_t)r * a.vd + c, o[i][j]);
-                }
+                if (it.whole) out.put4at(c, scaled4(o[i][j], inv));
+                else put4(piece + 2 * RB + (size_t)r * a.vd + c, o[i][j]);
             }
         }
     }
@@ -185,12 +231,6 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a) {
 
 // ------------------------------------------------------------------------------------------------------ pieces
 constexpr int TM_WARPS = 8, TM_ML = (TREE_CTAS + 31) / 32;
-__device__ __forceinline__ void add4(float4& o, float f, float4 x) {
-    o.x = fmaf(f, x.x, o.x);
-    o.y = fmaf(f, x.y, o.y);
-    o.z = fmaf(f, x.z, o.z);
-    o.w = fmaf(f, x.w, o.w);
-}
 // grid (X, groups of `per` rows).  With few segments X counts them; else block x looks at the border between the shares of CTAs x and
 // x + 1, and when it is the first border inside a segment, the block adds that segment's pieces.  WIDE: the warps of a block share the
 // pieces of one row after the other (few rows); else a warp has rows of its own.  Bound by the latency of two rounds of loads; where the
@@ -282,14 +322,23 @@ __global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs
 // ------------------------------------------------------------------------------------------------------ host side
 template <int TR, int VJ>
 static cudaError_t launch_simt(const TreeArgs& a, cudaStream_t q) {
-    const size_t smem = simt_smem(a.block, a.kd, a.vd);
+    const int stages = simt_smem(a.block, a.kd, a.vd, 2) <= 220 * 1024 ? 2 : 1;
+    const size_t smem = simt_smem(a.block, a.kd, a.vd, stages);
     const cudaError_t e = cudaFuncSetAttribute(k_ftree_simt<TR, VJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl_try(k_ftree_simt<TR, VJ>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a);
+    return launch_pdl_try(k_ftree_simt<TR, VJ>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a, stages);
 }
 template <int TR>
 static cudaError_t launch_simt_v(const TreeArgs& a, cudaStream_t q) {
     return a.vd <= 64 ? launch_simt<TR, 1>(a, q) : a.vd <= 128 ? launch_simt<TR, 2>(a, q) : launch_simt<TR, 4>(a, q);
+}
+static cudaError_t launch_simt_r(const TreeArgs& a, cudaStream_t q) {
+    switch (a.block) {
+        case 16: return launch_simt_v<1>(a, q);
+        case 32: return launch_simt_v<2>(a, q);
+        case 48: return launch_simt_v<3>(a, q);
+        default: return launch_simt_v<4>(a, q);
+    }
 }
 template <class T>
 static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
@@ -301,9 +350,11 @@ static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
     const int per = TM_WARPS * std::max(1, rows * x / (TM_WARPS * 4 * TREE_CTAS));
     return launch_pdl_try(k_ftree_merge<T, false>, dim3(x, (rows + per - 1) / per), dim3(TM_WARPS * 32), 0, q, 1, a, per, by_segment);
 }
-// Rows of a block and keys of a tile.
+// Rows of a block (of 16, 32, 48 or 64 the size that leaves the fewest rows empty), keys of a tile, tiles that a turn costs.
 static void simt_shape(int rows, int* block, int* tile, int* turn) {
-    *block = rows <= 16 ? 16 : 64;
+    *block = 64;
+    for (int b = 48; b >= 16; b -= 16)
+        if ((rows + b - 1) / b * b < (rows + *block - 1) / *block * *block) *block = b;
     *tile = TS_KEYS;
     *turn = 1;
 }
@@ -342,16 +393,19 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     DETB_TAKE(op->q && op->out && op->scratch && aligned16(op->q) && reinterpret_cast<uintptr_t>(op->scratch) % 128 == 0,
               "q, out or scratch is NULL or misaligned");
     TreeArgs a{};
+    a.heads = op->heads; a.kv_heads = op->kv_heads; a.per_kv = op->heads / op->kv_heads; a.dim = op->dim; a.vdim = op->vdim;
+    a.per_magic = ((1ull << 32) + a.per_kv - 1) / a.per_kv;
     a.kd = round8(op->dim); a.vd = round8(op->vdim);
-    if (op->dtype == DET_BF16) ftree_tc_shape((int)rows, a.kd, a.vd, &a.block, &a.tile, &a.turn);
+    a.ld = det_f_attn_ld(op->kv_heads, op->dim, op->vdim);
+    a.ldq = det_f_attn_q_ld(op->heads, op->dim);
+    a.seq = op->seq;
+    const bool few = op->dtype == DET_BF16 && ftree_few_takes(a, (int)rows);
+    if (few) ftree_few_shape(&a.block, &a.tile);
+    else if (op->dtype == DET_BF16) ftree_tc_shape((int)rows, a.kd, a.vd, &a.block, &a.tile, &a.turn);
     else simt_shape((int)rows, &a.block, &a.tile, &a.turn);
     const long long blocks = (rows + a.block - 1) / a.block;
     DETB_TAKE(blocks * op->seq.seqs <= 65535, "too many rows");
     DETB_TAKE(runtime_ready(), "no usable device");
-    a.heads = op->heads; a.kv_heads = op->kv_heads; a.per_kv = op->heads / op->kv_heads;
-    a.per_magic = ((1ull << 32) + a.per_kv - 1) / a.per_kv; a.dim = op->dim; a.vdim = op->vdim;
-    a.ld = det_f_attn_ld(op->kv_heads, op->dim, op->vdim);
-    a.ldq = det_f_attn_q_ld(op->heads, op->dim);
     a.scale2 = op->scale * 1.4426950408889634f;
     a.cap = op->cap; a.q = op->q; a.mask = op->mask; a.mask_ld = op->mask_ld; a.gate = op->gate; a.ldg = op->ldg; a.pos = op->pos;
     a.rope_len = op->rope_len; a.vcs = op->vrope_cos; a.vsn = op->vrope_sin; a.out = op->out; a.ldo = op->ldo;
@@ -359,14 +413,14 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     a.part = reinterpret_cast<float*>(static_cast<char*>(op->scratch) + TREE_MAP_BYTES);
     a.error_flag = error_word();
     a.blocks = (int)blocks;
-    a.seq = op->seq;
     a.ctas = std::min(TREE_CTAS, sm_count());
     cudaStream_t q = queue_of(st);
+    if (few) return launched(name, ftree_few_launch(a, q));
     if (op->dtype == DET_BF16) {
         if (int rc = launched(name, ftree_tc_launch(a, q))) return rc;
         return launched(name, launch_merge<bf16>(a, q));
     }
-    if (int rc = launched(name, a.block == 16 ? launch_simt_v<1>(a, q) : launch_simt_v<4>(a, q))) return rc;
+    if (int rc = launched(name, launch_simt_r(a, q))) return rc;
     return launched(name, launch_merge<float>(a, q));
 }
 

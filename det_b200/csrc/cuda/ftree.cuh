@@ -279,6 +279,17 @@ struct TreeOut {
 };
 __device__ __forceinline__ float4 scaled4(float4 v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
 
+__device__ __forceinline__ void add4(float4& o, float f, float4 x) {
+    o.x = fmaf(f, x.x, o.x);
+    o.y = fmaf(f, x.y, o.y);
+    o.z = fmaf(f, x.z, o.z);
+    o.w = fmaf(f, x.w, o.w);
+}
+
+// ftree_few.cu: bfloat16 activations, few rows.
+bool ftree_few_takes(const TreeArgs& a, int rows);
+void ftree_few_shape(int* block, int* tile);
+cudaError_t ftree_few_launch(const TreeArgs& a, cudaStream_t q);
 // ftree_tc.cu: bfloat16 activations.  Rows of a block, keys of a tile and the tiles that a turn costs are the kernel's.
 void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile, int* turn);
 cudaError_t ftree_tc_launch(const TreeArgs& a, cudaStream_t q);
