@@ -2,7 +2,7 @@
 // norms, rotates and caches the rows of a step.
 //
 //   k_frope_table   a thread owns up to four neighbouring columns and walks down the positions.
-//   k_fqk_rope      one head of a row per group of 8 to 32 lanes.
+//   k_fqk_rope      a warp takes some heads of a row, one per 8 to 32 lanes at a time.
 #include "ftree.cuh"
 #include <algorithm>
 #include <cmath>
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256) k_frope_table(const RopeArgs a) {
 
 // ------------------------------------------------------------------------------------------------------ norm and rotation
 struct QkArgs {
-    int heads, kv_heads, dim, vdim, rot, half, kd, vd, ld, ldq, cap, ldy, q_off, k_off, v_off, rope_len, lanes;
+    int heads, kv_heads, dim, vdim, rot, half, kd, vd, ld, ldq, cap, ldy, q_off, k_off, v_off, rope_len;
     float eps;
     const float* q_norm;
     const float* k_norm;
@@ -83,97 +83,153 @@ struct QkArgs {
     int* error_flag;
     det_tree_ref seq;
 };
+// n elements from e on (8 of them, zeros past the end).
 template <bool VEC>
-__device__ __forceinline__ float4 load4(const float* p, int e, int n) {
-    if (VEC) return e < n ? *reinterpret_cast<const float4*>(p + e) : make_float4(0, 0, 0, 0);
-    return make_float4(e < n ? p[e] : 0.0f, e + 1 < n ? p[e + 1] : 0.0f, e + 2 < n ? p[e + 2] : 0.0f, e + 3 < n ? p[e + 3] : 0.0f);
+__device__ __forceinline__ void load8(const float* p, int e, int n, float (&v)[8]) {
+    if (VEC) {
+        const float4 a = e < n ? *reinterpret_cast<const float4*>(p + e) : make_float4(0, 0, 0, 0);
+        const float4 b = e < n ? *reinterpret_cast<const float4*>(p + e + 4) : make_float4(0, 0, 0, 0);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = e + i < n ? p[e + i] : 0.0f;
+    }
+}
+__device__ __forceinline__ void put8(float* p, const float (&v)[8]) {
+    put4(p, make_float4(v[0], v[1], v[2], v[3]));
+    put4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
+}
+__device__ __forceinline__ void put8(bf16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf(v[0], v[1]), pack_bf(v[2], v[3]), pack_bf(v[4], v[5]), pack_bf(v[6], v[7]));
 }
 
+// A warp takes a part of a row's heads, 32 / LPH at a time, eight neighbouring elements a lane; the row's place and its cosines and sines
+// are fetched once.  VEC: heads are multiples of 8 elements, everything is 16-byte aligned and the halves of a rotated head are whole
+// lanes apart, so that a lane gets its partners by a shuffle.  Bound by HBM in long runs (it has 130 instructions to spend on a head of
+// 128 then), by latency for few rows.
 constexpr int QK_THREADS = 256;
-// grid (rows, pieces of a row's heads); `lanes` lanes per head, four neighbouring elements each, CH times.
-template <class T, bool VEC, int CH>
-__global__ void __launch_bounds__(QK_THREADS) k_fqk_rope(const QkArgs a) {
+template <class T, bool VEC, int LPH>
+__global__ void __launch_bounds__(QK_THREADS) k_fqk_rope(const QkArgs a, int parts) {
     pdl_trigger();
+    constexpr int HEADS = 32 / LPH;
+    const int lane = threadIdx.x & 31, sub = lane / LPH, e = lane % LPH * 8, units = a.heads + 2 * a.kv_heads, groups = (units + HEADS - 1) / HEADS;
+    const int task = (int)(((long long)blockIdx.x * QK_THREADS + threadIdx.x) >> 5), row = task / parts, part = task - row * parts;
     pdl_wait();
-    const int row = blockIdx.x, lane = threadIdx.x & 31;
+    if (row >= a.seq.rows) return;
     const TreePlace at = tree_place(a.seq, row, lane);
     if (at.b < 0) return;
     const int pos = a.pos ? a.pos[row] : at.slot;
     void* base = a.seq.table[at.b].cache;
     if (at.node < 0 || at.node >= a.seq.max_nodes || at.slot < at.node || at.slot >= a.cap || !usable_cache(base) ||
         ((a.rot || a.vcs) && (pos < 0 || pos >= a.rope_len))) {
-        if (threadIdx.x == 0) report_size(a.error_flag);
+        if (lane == 0) report_size(a.error_flag);
         return;
     }
-    const int u = (blockIdx.y * QK_THREADS + threadIdx.x) / a.lanes, l = threadIdx.x % a.lanes;
-    const int units = a.heads + 2 * a.kv_heads;
-    const bool value = u >= a.heads + a.kv_heads, key = !value && u >= a.heads;
-    const int h = value ? u - a.heads - a.kv_heads : key ? u - a.heads : u;
-    const int n = value ? a.vdim : a.dim, nd = value ? a.vd : a.kd;
-    const float* x = a.y + (size_t)row * a.ldy + (value ? a.v_off : key ? a.k_off : a.q_off) + (size_t)h * n;
-    const float* w = value ? nullptr : key ? a.k_norm : a.q_norm;
-    float4 v[CH];
-    float sum = 0.0f;
+    // cosines and sines of the lane's elements: four pairs, or eight elements of a half
+    const int hr = a.rot / 2, i0 = a.half ? (e < hr ? e : e - hr) : e / 2;
+    float co[8], si[8];
+    if (e < a.rot) {
+        const float* c = a.cs + (size_t)pos * hr;
+        const float* s = a.sn + (size_t)pos * hr;
+        if (a.half && VEC) {
+            load8<VEC>(c, i0, hr, co);
+            load8<VEC>(s, i0, hr, si);
+        } else if (!a.half) {
 #pragma unroll
-    for (int c = 0; c < CH; c++) {
-        v[c] = u < units ? load4<VEC>(x, (c * 32 + l) * 4, n) : make_float4(0, 0, 0, 0);
-        sum = fmaf(v[c].x, v[c].x, fmaf(v[c].y, v[c].y, fmaf(v[c].z, v[c].z, fmaf(v[c].w, v[c].w, sum))));
-    }
-    for (int off = a.lanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(FULL, sum, off);
-    if (u >= units) return;
-    const float r = w ? 1.0f / sqrtf(sum / (float)n + a.eps) : 1.0f;
-    const int rot = value ? (a.vcs ? a.vdim : 0) : a.rot, half = value ? 0 : a.half, hr = rot / 2;
-    const float* cs = (value ? a.vcs : a.cs) + (size_t)pos * hr;
-    const float* sn = (value ? a.vsn : a.sn) + (size_t)pos * hr;
-    T* to;
-    if (value || key) {
-        T* cache = static_cast<T*>(base) + (size_t)at.slot * a.ld;
-        to = cache + (value ? a.kv_heads * a.kd + h * a.vd : h * a.kd);
-    } else {
-        to = static_cast<T*>(a.q) + (size_t)row * a.ldq + h * a.kd;
-    }
-#pragma unroll
-    for (int c = 0; c < CH; c++) {
-        const int e = (c * 32 + l) * 4;
-        if (e >= nd) break;
-        float z[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-        if (w) {
-            const float4 g = load4<VEC>(w, e, n);
-            z[0] *= r * g.x;
-            z[1] *= r * g.y;
-            z[2] *= r * g.z;
-            z[3] *= r * g.w;
-        }
-        if (e < rot) {
-            if (!half) {
-#pragma unroll
-                for (int j = 0; j < 4; j += 2)
-                    if (e + j < rot) {
-                        const float co = cs[(e + j) / 2], si = sn[(e + j) / 2], p = z[j];
-                        z[j] = fmaf(p, co, -(z[j + 1] * si));
-                        z[j + 1] = fmaf(z[j + 1], co, p * si);
-                    }
-            } else {
-                // the other half of the pairs comes from memory again (the lines are in L1) and is normed here too
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (e + j >= rot) break;
-                    const bool first = e + j < hr;
-                    const int i = first ? e + j : e + j - hr, o = first ? e + j + hr : i;
-                    float p = x[o];
-                    if (w) p *= r * w[o];
-                    z[j] = first ? fmaf(z[j], cs[i], -(p * sn[i])) : fmaf(z[j], cs[i], p * sn[i]);
-                }
+            for (int i = 0; i < 4; i++) {
+                const bool in = i0 + i < hr;
+                co[i] = in ? c[i0 + i] : 1.0f;
+                si[i] = in ? s[i0 + i] : 0.0f;
             }
         }
-        put4(to + e, make_float4(z[0], z[1], z[2], z[3]));
+    }
+    const float* y = a.y + (size_t)row * a.ldy;
+    T* cache = static_cast<T*>(base) + (size_t)at.slot * a.ld;
+    T* query = static_cast<T*>(a.q) + (size_t)row * a.ldq;
+    const float inv_dim = 1.0f / (float)a.dim;
+#pragma unroll 2
+    for (int grp = part; grp < groups; grp += parts) {
+        const int u = grp * HEADS + sub;
+        const bool real = u < units, value = u >= a.heads + a.kv_heads, key = !value && u >= a.heads;
+        const int h = value ? u - a.heads - a.kv_heads : key ? u - a.heads : u, n = value ? a.vdim : a.dim;
+        const float* x = y + (value ? a.v_off : key ? a.k_off : a.q_off) + (size_t)h * n;
+        const float* w = value ? nullptr : key ? a.k_norm : a.q_norm;
+        float z[8];
+        load8<VEC>(x, e, real ? n : 0, z);
+        float r = 1.0f;
+        if (a.q_norm || a.k_norm) {
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                s0 = fmaf(z[i], z[i], s0);
+                s1 = fmaf(z[i + 1], z[i + 1], s1);
+            }
+            s0 += s1;
+#pragma unroll
+            for (int off = LPH / 2; off > 0; off >>= 1) s0 += __shfl_xor_sync(FULL, s0, off);
+            r = rsqrtf(fmaf(s0, inv_dim, a.eps));
+            if (w && real) {
+                float g[8];
+                load8<VEC>(w, e, n, g);
+#pragma unroll
+                for (int i = 0; i < 8; i++) z[i] *= r * g[i];
+            }
+        }
+        if (a.half) {
+            if (VEC) {
+                const bool first = e < hr, turned = !value && e < a.rot;
+                const int from = sub * LPH + ((lane % LPH + (first ? hr / 8 : LPH - hr / 8)) & (LPH - 1));
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float p = __shfl_sync(FULL, z[i], from);
+                    if (turned) z[i] = fmaf(z[i], co[i], (first ? -p : p) * si[i]);
+                }
+            } else if (real && !value) {
+                // the other half of the pairs comes from memory again (the lines are in L1) and is normed here too
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (e + i >= a.rot) break;
+                    const bool first = e + i < hr;
+                    const int k = first ? e + i : e + i - hr, o = first ? e + i + hr : k;
+                    float p = x[o];
+                    if (w) p *= r * w[o];
+                    z[i] = fmaf(z[i], a.cs[(size_t)pos * hr + k], (first ? -p : p) * a.sn[(size_t)pos * hr + k]);
+                }
+            }
+        } else if (!value) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (e + 2 * i < a.rot) {
+                    const float p = z[2 * i];
+                    z[2 * i] = fmaf(p, co[i], -(z[2 * i + 1] * si[i]));
+                    z[2 * i + 1] = fmaf(z[2 * i + 1], co[i], p * si[i]);
+                }
+        }
+        if (a.vcs && value && real) {
+            const float* c = a.vcs + (size_t)pos * (a.vdim / 2);
+            const float* s = a.vsn + (size_t)pos * (a.vdim / 2);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (e + 2 * i < a.vdim) {
+                    const float ci = c[e / 2 + i], sj = s[e / 2 + i], p = z[2 * i];
+                    z[2 * i] = fmaf(p, ci, -(z[2 * i + 1] * sj));
+                    z[2 * i + 1] = fmaf(z[2 * i + 1], ci, p * sj);
+                }
+        }
+        if (real && e < (value ? a.vd : a.kd)) put8(value ? cache + a.kv_heads * a.kd + h * a.vd + e : (key ? cache : query) + h * a.kd + e, z);
     }
 }
 
 template <class T, bool VEC>
-static cudaError_t launch_qk(const QkArgs& a, dim3 grid, cudaStream_t q) {
-    return std::max(a.kd, a.vd) <= 128 ? launch_pdl_try(k_fqk_rope<T, VEC, 1>, grid, dim3(QK_THREADS), 0, q, 1, a)
-                                       : launch_pdl_try(k_fqk_rope<T, VEC, 2>, grid, dim3(QK_THREADS), 0, q, 1, a);
+static cudaError_t launch_qk(const QkArgs& a, cudaStream_t q) {
+    const int most = std::max(a.kd, a.vd), lph = most <= 64 ? 8 : most <= 128 ? 16 : 32, groups = (a.heads + 2 * a.kv_heads + 32 / lph - 1) / (32 / lph);
+    // a group per warp while that leaves SMs idle, seven in long runs
+    const int parts = (int)std::max<long long>((groups + 6) / 7, std::min<long long>(groups, 32ll * sm_count() / a.seq.rows));
+    const long long warps = (long long)a.seq.rows * parts;
+    const dim3 grid((unsigned)((warps + QK_THREADS / 32 - 1) / (QK_THREADS / 32))), block(QK_THREADS);
+    return lph == 8    ? launch_pdl_try(k_fqk_rope<T, VEC, 8>, grid, block, 0, q, 1, a, parts)
+           : lph == 16 ? launch_pdl_try(k_fqk_rope<T, VEC, 16>, grid, block, 0, q, 1, a, parts)
+                       : launch_pdl_try(k_fqk_rope<T, VEC, 32>, grid, block, 0, q, 1, a, parts);
 }
 
 }  // namespace detb
@@ -251,16 +307,14 @@ int det_f_qk_rope(const det_fqk_op* op, cudaStream_t st) {
     a.eps = op->eps; a.q_norm = op->q_norm; a.k_norm = op->k_norm; a.y = op->y;
     a.cs = op->rope_cos; a.sn = op->rope_sin; a.vcs = op->vrope_cos; a.vsn = op->vrope_sin;
     a.pos = op->pos; a.q = op->q; a.error_flag = error_word(); a.seq = op->seq;
-    a.lanes = 8;
-    while (a.lanes < 32 && a.lanes * 4 < std::max(a.kd, a.vd)) a.lanes *= 2;
-    const int per = QK_THREADS / a.lanes, units = a.heads + 2 * a.kv_heads;
-    const dim3 grid(op->seq.rows, (units + per - 1) / per);
-    const bool vec = aligned16(op->y) && op->ldy % 4 == 0 && op->q_off % 4 == 0 && op->k_off % 4 == 0 && op->v_off % 4 == 0 && op->dim % 4 == 0 &&
-                     op->vdim % 4 == 0 && aligned16(op->q_norm) && aligned16(op->k_norm);
+    DETB_TAKE((long long)op->seq.rows * (a.heads + 2 * a.kv_heads) < 1ll << 31, "too many rows");
+    const bool vec = aligned16(op->y) && op->ldy % 4 == 0 && op->q_off % 4 == 0 && op->k_off % 4 == 0 && op->v_off % 4 == 0 && op->dim % 8 == 0 &&
+                     op->vdim % 8 == 0 && aligned16(op->q_norm) && aligned16(op->k_norm) && op->rot_dims % 16 == 0 && aligned16(op->rope_cos) &&
+                     aligned16(op->rope_sin);
     cudaStream_t q = queue_of(st);
     cudaError_t e;
-    if (op->dtype == DET_BF16) e = vec ? launch_qk<bf16, true>(a, grid, q) : launch_qk<bf16, false>(a, grid, q);
-    else e = vec ? launch_qk<float, true>(a, grid, q) : launch_qk<float, false>(a, grid, q);
+    if (op->dtype == DET_BF16) e = vec ? launch_qk<bf16, true>(a, q) : launch_qk<bf16, false>(a, q);
+    else e = vec ? launch_qk<float, true>(a, q) : launch_qk<float, false>(a, q);
     return launched(name, e);
 }
 

@@ -34,19 +34,30 @@ __device__ __forceinline__ float row_sum(float v) {
 __device__ __forceinline__ void copy16(float* dst, const float* src, int bytes) {      // what is missing of 16 bytes becomes zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
 }
-// `rows` rows of n floats (a multiple of 4), `ld` apart, into rows of n + 4; rows past `have` become zeros
-__device__ __forceinline__ void copy_rows(float* dst, const float* src, size_t ld, int n, int rows, int have) {
-    const int pieces = n / 4, dr = TS_THREADS / pieces, dc = TS_THREADS - dr * pieces;
-    int r = threadIdx.x / pieces, c = threadIdx.x - r * pieces;
-    while (r < rows) {
-        copy16(dst + r * (n + 4) + c * 4, r < have ? src + r * ld + c * 4 : src, r < have ? 16 : 0);
-        r += dr;
-        c += dc;
-        if (c >= pieces) {
-            c -= pieces;
-            r++;
-        }
+// The 64 rows of a tile, n floats (a multiple of 4) each, `ld` apart, into rows of n + 4; rows past `have` become zeros.  LANES threads take
+// the 16-byte pieces of a row, so an address is one addition.
+template <int LANES>
+__device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t ld, int n, int have) {
+    constexpr int STEP = TS_THREADS / LANES;
+    const int c = (threadIdx.x % LANES) * 4, r0 = threadIdx.x / LANES;
+    if (c >= n) return;
+    const float* first = src + c;
+    src += r0 * ld + c;
+    dst += r0 * (n + 4) + c;
+    const size_t step = STEP * ld;
+    const int to = STEP * (n + 4);
+    if (have >= TS_KEYS) {
+#pragma unroll
+        for (int i = 0; i < TS_KEYS / STEP; i++, src += step, dst += to) copy16(dst, src, 16);
+    } else {
+        for (int r = r0; r < TS_KEYS; r += STEP, src += step, dst += to) copy16(dst, r < have ? src : first, r < have ? 16 : 0);
     }
+}
+__device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t ld, int n, int have) {
+    if (n <= 32) copy_tile<8>(dst, src, ld, n, have);
+    else if (n <= 64) copy_tile<16>(dst, src, ld, n, have);
+    else if (n <= 128) copy_tile<32>(dst, src, ld, n, have);
+    else copy_tile<64>(dst, src, ld, n, have);
 }
 
 // Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.  With two stages the next tile's copies run
@@ -79,8 +90,8 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int
             if (t < it.tile + it.n) {
                 const int k0 = t * TS_KEYS, have = s.len + s.n - k0;
                 const float* rows = cache + (size_t)k0 * a.ld;
-                copy_rows(KV + stage * stage_floats, rows + it.g * a.kd, a.ld, a.kd, TS_KEYS, have);
-                copy_rows(KV + stage * stage_floats + TS_KEYS * ldk, rows + a.kv_heads * a.kd + it.g * a.vd, a.ld, a.vd, TS_KEYS, have);
+                copy_tile(KV + stage * stage_floats, rows + it.g * a.kd, a.ld, a.kd, have);
+                copy_tile(KV + stage * stage_floats + TS_KEYS * ldk, rows + a.kv_heads * a.kd + it.g * a.vd, a.ld, a.vd, have);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -350,11 +361,13 @@ static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
     const int per = TM_WARPS * std::max(1, rows * x / (TM_WARPS * 4 * TREE_CTAS));
     return launch_pdl_try(k_ftree_merge<T, false>, dim3(x, (rows + per - 1) / per), dim3(TM_WARPS * 32), 0, q, 1, a, per, by_segment);
 }
-// Rows of a block (of 16, 32, 48 or 64 the size that leaves the fewest rows empty), keys of a tile, tiles that a turn costs.
+// Rows of a block, keys of a tile, tiles that a turn costs.  A tile takes about as long for its copies, waits and softmax as for the
+// products of 48 rows.
 static void simt_shape(int rows, int* block, int* tile, int* turn) {
+    auto cost = [&](int b) { return (long long)((rows + b - 1) / b) * (48 + b); };
     *block = 64;
     for (int b = 48; b >= 16; b -= 16)
-        if ((rows + b - 1) / b * b < (rows + *block - 1) / *block * *block) *block = b;
+        if (cost(b) < cost(*block)) *block = b;
     *tile = TS_KEYS;
     *turn = 1;
 }
