@@ -29,30 +29,46 @@ __device__ __forceinline__ double turns_of(const RopeArgs& a, int i) {
     }
     return t;
 }
-// cos and sin of 2 pi x: whole turns leave in binary64, what is left is taken in two fp32 parts, the small one to first order.
-__device__ __forceinline__ float2 turn(double x, float m) {
-    const double r = 2.0 * (x - rint(x));
-    const float hi = (float)r, lo = (float)(r - (double)hi) * 3.14159265f;
-    float s, c;
-    sincospif(hi, &s, &c);
-    return make_float2(fmaf(-lo, s, c) * m, fmaf(lo, c, s) * m);
+// cos and sin of `phase` / 2^32 turns.  The quadrant is an integer, what is left (an eighth of a turn either way) goes through the Taylor
+// series of both functions, r^11 and r^12 the first terms left out (4e-9 and 1e-10 of the result).
+__device__ __forceinline__ float2 turn(unsigned phase, float m) {
+    const unsigned q = (phase + 0x20000000u) >> 30;
+    const float r = (float)(int)(phase - (q << 30)) * 1.46291807926715968e-9f, x = r * r;      // 2 pi / 2^32
+    float s = fmaf(x, 2.75573192e-6f, -1.98412698e-4f);
+    s = fmaf(s, x, 8.33333333e-3f);
+    s = fmaf(s, x, -1.66666667e-1f);
+    s = fmaf(s * x, r, r);
+    float c = fmaf(x, -2.75573192e-7f, 2.48015873e-5f);
+    c = fmaf(c, x, -1.38888889e-3f);
+    c = fmaf(c, x, 4.16666667e-2f);
+    c = fmaf(c, x, -0.5f);
+    c = fmaf(c, x, 1.0f);
+    const float u = q & 1 ? s : c, v = q & 1 ? c : s;
+    // cos: - in quadrants 1 and 2; sin: - in quadrants 2 and 3
+    return make_float2(__uint_as_float(__float_as_uint(u) ^ ((q + 1) >> 1 << 31)) * m, __uint_as_float(__float_as_uint(v) ^ (q >> 1 << 31)) * m);
 }
+// One more turn is no turn: a column's turns per position are kept as 64 bits behind the point, and a position's phase is the product's
+// low 64 bits, of which the upper half is used (2^-33 turns).  The products of binary64 it replaces are what the call took longest
+// over (262144 x 64 pairs: 38.4 us with them, TABLE_US now, 134 MB written).
 template <int V>
 __global__ void __launch_bounds__(256) k_frope_table(const RopeArgs a) {
     pdl_trigger();
     const int groups = a.cols / V, g = blockIdx.x * blockDim.x + threadIdx.x;
-    double t[V];
+    unsigned long long t[V];
     if (g < groups)
 #pragma unroll
-        for (int j = 0; j < V; j++) t[j] = turns_of(a, g * V + j);
+        for (int j = 0; j < V; j++) {
+            const double x = turns_of(a, g * V + j);
+            t[j] = __double2ull_rn((x - floor(x)) * 18446744073709551616.0);
+        }
     pdl_wait();
     if (g >= groups) return;
     for (int p = blockIdx.y * blockDim.y + threadIdx.y; p < a.n; p += gridDim.y * blockDim.y) {
-        const double at = (double)a.pos0 + (double)p;
+        const unsigned at = (unsigned)(a.pos0 + p);
         float c[V], s[V];
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const float2 v = turn(at * t[j], a.mscale);
+            const float2 v = turn((unsigned)(at * t[j] >> 32), a.mscale);
             c[j] = v.x;
             s[j] = v.y;
         }
@@ -103,17 +119,115 @@ __device__ __forceinline__ void put8(bf16* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf(v[0], v[1]), pack_bf(v[2], v[3]), pack_bf(v[4], v[5]), pack_bf(v[6], v[7]));
 }
 
-// A warp takes a part of a row's heads, 32 / LPH at a time, eight neighbouring elements a lane; the row's place and its cosines and sines
-// are fetched once.  VEC: heads are multiples of 8 elements, everything is 16-byte aligned and the halves of a rotated head are whole
-// lanes apart, so that a lane gets its partners by a shuffle.  Bound by HBM in long runs (it has 130 instructions to spend on a head of
-// 128 then), by latency for few rows.
+// A warp takes a part of a row's heads, 32 / LPH at a time, eight neighbouring elements a lane; the row's place, its cosines and sines and
+// the norm's weights are fetched once.  VEC: heads are multiples of 8 elements, everything is 16-byte aligned and the halves of a
+// rotated head are whole lanes apart, so that a lane gets its partners by a shuffle.
 constexpr int QK_THREADS = 256;
+struct QkLane {
+    int e, first, from;            // element, in the first half of the pairs, the lane with the partners
+    float co[8], si[8];            // of four pairs, or of eight elements of a half (si with the sign of its product)
+};
+// `count` heads of n elements from x on, results to `to`: normed by w (or NULL), rotated in the first `rot` elements (or 0).
 template <class T, bool VEC, int LPH>
-__global__ void __launch_bounds__(QK_THREADS) k_fqk_rope(const QkArgs a, int parts) {
-    pdl_trigger();
+__device__ __forceinline__ void qk_heads(const QkArgs& a, const QkLane& k, const float* x, T* to, int count, int n, int nd, const float* w, int rot, bool half,
+                                         size_t pos, int part, int parts) {
     constexpr int HEADS = 32 / LPH;
-    const int lane = threadIdx.x & 31, sub = lane / LPH, e = lane % LPH * 8, units = a.heads + 2 * a.kv_heads, groups = (units + HEADS - 1) / HEADS;
-    const int task = (int)(((long long)blockIdx.x * QK_THREADS + threadIdx.x) >> 5), row = task / parts, part = task - row * parts;
+    const int lane = threadIdx.x & 31, hr = rot / 2;
+    float g[8];
+    if (w) load8<VEC>(w, k.e, n, g);
+    const float inv_n = 1.0f / (float)n;
+    int h = part * HEADS + lane / LPH;
+    x += h * n;
+    to += h * nd + k.e;
+    const int left = (count - part * HEADS + parts * HEADS - 1) / (parts * HEADS);       // rounds of the warp
+    float ahead[8];
+    load8<VEC>(x, k.e, h < count ? n : 0, ahead);
+    for (int i = 0; i < left; i++) {
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) z[j] = ahead[j];
+        const float* mine = x;
+        const bool real = h < count;
+        h += parts * HEADS;
+        x += parts * HEADS * n;
+        if (i + 1 < left) load8<VEC>(x, k.e, h < count ? n : 0, ahead);
+        float r = 1.0f;
+        if (w) {
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                s0 = fmaf(z[j], z[j], s0);
+                s1 = fmaf(z[j + 1], z[j + 1], s1);
+            }
+            s0 += s1;
+#pragma unroll
+            for (int off = LPH / 2; off > 0; off >>= 1) s0 += __shfl_xor_sync(FULL, s0, off);
+            r = rsqrtf(fmaf(s0, inv_n, a.eps));
+#pragma unroll
+            for (int j = 0; j < 8; j++) z[j] *= r * g[j];
+        }
+        if (rot && half && VEC) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float p = __shfl_sync(FULL, z[j], k.from);
+                if (k.e < rot) z[j] = fmaf(z[j], k.co[j], p * k.si[j]);
+            }
+        } else if (rot && half) {
+            // the other half of the pairs comes from memory again (the lines are in L1) and is normed here too
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (real && k.e + j < rot) {
+                    const bool first = k.e + j < hr;
+                    const int i0 = first ? k.e + j : k.e + j - hr, o = first ? k.e + j + hr : i0;
+                    float p = mine[o];
+                    if (w) p *= r * w[o];
+                    z[j] = fmaf(z[j], a.cs[pos * hr + i0], (first ? -p : p) * a.sn[pos * hr + i0]);
+                }
+        } else if (rot) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (k.e + 2 * j < rot) {
+                    const float p = z[2 * j];
+                    z[2 * j] = fmaf(p, k.co[j], -(z[2 * j + 1] * k.si[j]));
+                    z[2 * j + 1] = fmaf(z[2 * j + 1], k.co[j], p * k.si[j]);
+                }
+        }
+        if (real && k.e < nd) put8(to, z);
+        to += parts * HEADS * nd;
+    }
+}
+template <bool VEC, int LPH>
+__device__ __forceinline__ QkLane qk_lane(const float* cs, const float* sn, size_t pos, int rot, bool half) {
+    QkLane k;
+    const int lane = threadIdx.x & 31, l = lane % LPH, hr = rot / 2;
+    k.e = l * 8;
+    k.first = k.e < hr;
+    k.from = lane - l + ((l + (k.first ? hr / 8 : LPH - hr / 8)) & (LPH - 1));
+#pragma unroll
+    for (int i = 0; i < 8; i++) k.co[i] = 1.0f, k.si[i] = 0.0f;
+    if (k.e >= rot) return k;
+    cs += pos * hr;
+    sn += pos * hr;
+    if (half && VEC) {
+        load8<VEC>(cs, k.first ? k.e : k.e - hr, hr, k.co);
+        load8<VEC>(sn, k.first ? k.e : k.e - hr, hr, k.si);
+        if (k.first)
+#pragma unroll
+            for (int i = 0; i < 8; i++) k.si[i] = -k.si[i];
+    } else if (!half) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (k.e / 2 + i < hr) {
+                k.co[i] = cs[k.e / 2 + i];
+                k.si[i] = sn[k.e / 2 + i];
+            }
+    }
+    return k;
+}
+template <class T, bool VEC, int LPH>
+__global__ void __launch_bounds__(QK_THREADS, 4) k_fqk_rope(const QkArgs a, int parts) {
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, task = (int)(((long long)blockIdx.x * QK_THREADS + threadIdx.x) >> 5), row = task / parts, part = task - row * parts;
     pdl_wait();
     if (row >= a.seq.rows) return;
     const TreePlace at = tree_place(a.seq, row, lane);
@@ -125,99 +239,20 @@ __global__ void __launch_bounds__(QK_THREADS) k_fqk_rope(const QkArgs a, int par
         if (lane == 0) report_size(a.error_flag);
         return;
     }
-    // cosines and sines of the lane's elements: four pairs, or eight elements of a half
-    const int hr = a.rot / 2, i0 = a.half ? (e < hr ? e : e - hr) : e / 2;
-    float co[8], si[8];
-    if (e < a.rot) {
-        const float* c = a.cs + (size_t)pos * hr;
-        const float* s = a.sn + (size_t)pos * hr;
-        if (a.half && VEC) {
-            load8<VEC>(c, i0, hr, co);
-            load8<VEC>(s, i0, hr, si);
-        } else if (!a.half) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool in = i0 + i < hr;
-                co[i] = in ? c[i0 + i] : 1.0f;
-                si[i] = in ? s[i0 + i] : 0.0f;
-            }
-        }
-    }
     const float* y = a.y + (size_t)row * a.ldy;
     T* cache = static_cast<T*>(base) + (size_t)at.slot * a.ld;
-    T* query = static_cast<T*>(a.q) + (size_t)row * a.ldq;
-    const float inv_dim = 1.0f / (float)a.dim;
-#pragma unroll 2
-    for (int grp = part; grp < groups; grp += parts) {
-        const int u = grp * HEADS + sub;
-        const bool real = u < units, value = u >= a.heads + a.kv_heads, key = !value && u >= a.heads;
-        const int h = value ? u - a.heads - a.kv_heads : key ? u - a.heads : u, n = value ? a.vdim : a.dim;
-        const float* x = y + (value ? a.v_off : key ? a.k_off : a.q_off) + (size_t)h * n;
-        const float* w = value ? nullptr : key ? a.k_norm : a.q_norm;
-        float z[8];
-        load8<VEC>(x, e, real ? n : 0, z);
-        float r = 1.0f;
-        if (a.q_norm || a.k_norm) {
-            float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                s0 = fmaf(z[i], z[i], s0);
-                s1 = fmaf(z[i + 1], z[i + 1], s1);
-            }
-            s0 += s1;
-#pragma unroll
-            for (int off = LPH / 2; off > 0; off >>= 1) s0 += __shfl_xor_sync(FULL, s0, off);
-            r = rsqrtf(fmaf(s0, inv_dim, a.eps));
-            if (w && real) {
-                float g[8];
-                load8<VEC>(w, e, n, g);
-#pragma unroll
-                for (int i = 0; i < 8; i++) z[i] *= r * g[i];
-            }
-        }
-        if (a.half) {
-            if (VEC) {
-                const bool first = e < hr, turned = !value && e < a.rot;
-                const int from = sub * LPH + ((lane % LPH + (first ? hr / 8 : LPH - hr / 8)) & (LPH - 1));
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float p = __shfl_sync(FULL, z[i], from);
-                    if (turned) z[i] = fmaf(z[i], co[i], (first ? -p : p) * si[i]);
-                }
-            } else if (real && !value) {
-                // the other half of the pairs comes from memory again (the lines are in L1) and is normed here too
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (e + i >= a.rot) break;
-                    const bool first = e + i < hr;
-                    const int k = first ? e + i : e + i - hr, o = first ? e + i + hr : k;
-                    float p = x[o];
-                    if (w) p *= r * w[o];
-                    z[i] = fmaf(z[i], a.cs[(size_t)pos * hr + k], (first ? -p : p) * a.sn[(size_t)pos * hr + k]);
-                }
-            }
-        } else if (!value) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (e + 2 * i < a.rot) {
-                    const float p = z[2 * i];
-                    z[2 * i] = fmaf(p, co[i], -(z[2 * i + 1] * si[i]));
-                    z[2 * i + 1] = fmaf(z[2 * i + 1], co[i], p * si[i]);
-                }
-        }
-        if (a.vcs && value && real) {
-            const float* c = a.vcs + (size_t)pos * (a.vdim / 2);
-            const float* s = a.vsn + (size_t)pos * (a.vdim / 2);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (e + 2 * i < a.vdim) {
-                    const float ci = c[e / 2 + i], sj = s[e / 2 + i], p = z[2 * i];
-                    z[2 * i] = fmaf(p, ci, -(z[2 * i + 1] * sj));
-                    z[2 * i + 1] = fmaf(z[2 * i + 1], ci, p * sj);
-                }
-        }
-        if (real && e < (value ? a.vd : a.kd)) put8(value ? cache + a.kv_heads * a.kd + h * a.vd + e : (key ? cache : query) + h * a.kd + e, z);
-    }
+    // a group of heads after the other goes round the warps of the row: queries, then keys, then values
+    constexpr int HEADS = 32 / LPH;
+    const int gq = (a.heads + HEADS - 1) / HEADS, gk = (a.kv_heads + HEADS - 1) / HEADS;
+    const int pk = (part + parts - gq % parts) % parts, pv = (pk + parts - gk % parts) % parts;
+    const QkLane k = qk_lane<VEC, LPH>(a.cs, a.sn, pos, a.rot, a.half);
+    qk_heads<T, VEC, LPH>(a, k, y + a.q_off, static_cast<T*>(a.q) + (size_t)row * a.ldq, a.heads, a.dim, a.kd, a.q_norm, a.rot, a.half, pos, part, parts);
+    qk_heads<T, VEC, LPH>(a, k, y + a.k_off, cache, a.kv_heads, a.dim, a.kd, a.k_norm, a.rot, a.half, pos, pk, parts);
+    cache += a.kv_heads * a.kd;
+    if (a.vcs)
+        qk_heads<T, VEC, LPH>(a, qk_lane<VEC, LPH>(a.vcs, a.vsn, pos, a.vdim, false), y + a.v_off, cache, a.kv_heads, a.vdim, a.vd, nullptr, a.vdim, false, pos, pv,
+                              parts);
+    else qk_heads<T, VEC, LPH>(a, k, y + a.v_off, cache, a.kv_heads, a.vdim, a.vd, nullptr, 0, false, pos, pv, parts);
 }
 
 template <class T, bool VEC>
