@@ -244,11 +244,12 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int
 constexpr int TM_WARPS = 8, TM_ML = (TREE_CTAS + 31) / 32;
 // grid (X, groups of `per` rows).  With few segments X counts them; else block x looks at the border between the shares of CTAs x and
 // x + 1, and when it is the first border inside a segment, the block adds that segment's pieces.  WIDE: the warps of a block share the
-// pieces of one row after the other (few rows); else a warp has rows of its own.  Bound by the latency of two rounds of loads; where the
-// pieces are follows from what the attention kernel has waited for before it let this one start.
-template <class T, bool WIDE>
+// pieces of one row after the other (few rows); else a warp has rows of its own.  HI: values above 128.  Bound by the latency of the
+// loads, so what can be is asked for side by side; where the pieces are follows from what the attention kernel has waited for before it
+// let this one start.
+template <class T, bool WIDE, bool HI>
 __global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs a, int per, int by_segment) {
-    __shared__ float4 sum[WIDE ? TM_WARPS : 1][64];
+    __shared__ float4 sum[WIDE ? TM_WARPS : 1][HI ? 64 : 32];
     __shared__ float fac[TM_WARPS][TM_ML * 32];
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -273,18 +274,53 @@ __global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs
     const float* head = a.part + ((size_t)cta * 2 + (w.place < share ? 1 : 0)) * size;
     const float* rest = a.part + (size_t)cta * 2 * size;                      // the others are their CTAs' first pieces
     const int vq = a.vd / 4;
+    const bool lo = lane < vq, hi = HI && 32 + lane < vq;
+    auto piece = [&](int c) { return c ? rest + c * 2 * size : head; };
+    auto finish = [&](int r, float4 o0, float4 o1) {
+        const int row = s.r0 + r, node = (int)(row * a.per_magic >> 32);
+        const TreeOut<T> out(a, s.first + node, w.g * a.per_kv + row - node * a.per_kv);
+        if (lo) out.put4at(lane * 4, o0);
+        if (hi) out.put4at(128 + lane * 4, o1);
+    };
+    if (!WIDE && n <= 4) {                                    // every lane takes all factors of its row
+        for (int r = r0 + warp; r < r1; r += TM_WARPS) {
+            float2 ml[4];
+            float4 x[4], y[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const float* p = piece(min(c, n - 1));
+                const float* v = p + 2 * a.block + (size_t)r * a.vd + lane * 4;
+                ml[c] = c < n ? reinterpret_cast<const float2*>(p)[r] : make_float2(-INFINITY, 0.0f);
+                x[c] = lo && c < n ? load4(v) : make_float4(0, 0, 0, 0);
+                y[c] = hi && c < n ? load4(v + 128) : make_float4(0, 0, 0, 0);
+            }
+            float m = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), l = 0.0f;
+            if (m == -INFINITY) m = 0.0f;                     // a row without keys
+            float4 o0 = make_float4(0, 0, 0, 0), o1 = o0;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const float f = exp2f(ml[c].x - m);
+                l = fmaf(f, ml[c].y, l);
+                add4(o0, f, x[c]);
+                add4(o1, f, y[c]);
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            finish(r, scaled4(o0, inv), scaled4(o1, inv));
+        }
+        return;
+    }
     for (int r = WIDE ? r0 : r0 + warp; r < r1; r += WIDE ? 1 : TM_WARPS) {
         float2 ml[TM_ML];
         float m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int i = 0; i < TM_ML; i++) {
             const int c = i * 32 + lane;
-            ml[i] = c < n ? reinterpret_cast<const float2*>(c ? rest + c * 2 * size : head)[r] : make_float2(-INFINITY, 0.0f);
+            ml[i] = c < n ? reinterpret_cast<const float2*>(piece(c))[r] : make_float2(-INFINITY, 0.0f);
         }
 #pragma unroll
         for (int i = 0; i < TM_ML; i++) m = fmaxf(m, ml[i].x);
         m = warp_max(m);
-        if (m == -INFINITY) m = 0.0f;                         // a row without keys
+        if (m == -INFINITY) m = 0.0f;
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < TM_ML; i++) {
@@ -295,37 +331,42 @@ __global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs
         l = warp_sum(l);
         __syncwarp();
         const size_t at = 2 * a.block + (size_t)r * a.vd + lane * 4;
-        const bool lo = lane < vq, hi = 32 + lane < vq;
         float4 o0 = make_float4(0, 0, 0, 0), o1 = o0;
-        int c = WIDE ? warp : 0;
-        if (c == 0) {
-            if (lo) o0 = scaled4(load4(head + at), fac[warp][0]);
-            if (hi) o1 = scaled4(load4(head + at + 128), fac[warp][0]);
-            c += WIDE ? TM_WARPS : 1;
+        constexpr int RUN = WIDE || HI ? 4 : 8, STEP = WIDE ? TM_WARPS : 1;
+        for (int c0 = WIDE ? warp : 0; c0 < n; c0 += RUN * STEP) {
+            float4 x[RUN], y[RUN];
+#pragma unroll
+            for (int k = 0; k < RUN; k++) {
+                const int c = c0 + k * STEP;
+                const float* p = piece(c) + at;
+                x[k] = lo && c < n ? load4(p) : make_float4(0, 0, 0, 0);
+                y[k] = hi && c < n ? load4(p + 128) : make_float4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < RUN; k++) {
+                const int c = c0 + k * STEP;
+                const float f = c < n ? fac[warp][c] : 0.0f;
+                add4(o0, f, x[k]);
+                add4(o1, f, y[k]);
+            }
         }
-#pragma unroll 4
-        for (; c < n; c += WIDE ? TM_WARPS : 1) {
-            const float* p = rest + c * 2 * size + at;
-            if (lo) add4(o0, fac[warp][c], load4(p));
-            if (hi) add4(o1, fac[warp][c], load4(p + 128));
-        }
-        const int row = s.r0 + r, node = (int)(row * a.per_magic >> 32), h = w.g * a.per_kv + row - node * a.per_kv;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         if (!WIDE) {
-            const TreeOut<T> out(a, s.first + node, h);
-            if (lo) out.put4at(lane * 4, scaled4(o0, inv));
-            if (hi) out.put4at(128 + lane * 4, scaled4(o1, inv));
+            finish(r, scaled4(o0, inv), scaled4(o1, inv));
             continue;
         }
         __syncthreads();
-        sum[warp][lane] = o0;
-        sum[warp][32 + lane] = o1;
+        sum[WIDE ? warp : 0][lane] = o0;
+        if (HI) sum[WIDE ? warp : 0][HI ? 32 + lane : 0] = o1;
         __syncthreads();
-        if ((int)threadIdx.x < vq) {
-            float4 x = sum[0][threadIdx.x];
+        if (warp == 0) {
+            o0 = o1 = make_float4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 1; i < (WIDE ? TM_WARPS : 1); i++) add4(x, 1.0f, sum[i][threadIdx.x]);
-            TreeOut<T>(a, s.first + node, h).put4at(threadIdx.x * 4, scaled4(x, inv));
+            for (int i = 0; i < (WIDE ? TM_WARPS : 1); i++) {
+                add4(o0, inv, sum[i][lane]);
+                if (HI) add4(o1, inv, sum[i][HI ? 32 + lane : 0]);
+            }
+            finish(r, o0, o1);
         }
     }
 }
@@ -356,10 +397,14 @@ static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
     if (a.ctas == 1) return cudaSuccess;
     const long long segs = (long long)a.seq.seqs * a.blocks * a.kv_heads;
     const int by_segment = segs < a.ctas - 1, x = by_segment ? (int)segs : a.ctas - 1, rows = std::min(a.block, a.seq.max_nodes * a.per_kv);
-    if (rows * x <= 4 * TREE_CTAS)                             // a row per block, about four blocks on an SM
-        return launch_pdl_try(k_ftree_merge<T, true>, dim3(x, rows), dim3(TM_WARPS * 32), 0, q, 1, a, 1, by_segment);
-    const int per = TM_WARPS * std::max(1, rows * x / (TM_WARPS * 4 * TREE_CTAS));
-    return launch_pdl_try(k_ftree_merge<T, false>, dim3(x, (rows + per - 1) / per), dim3(TM_WARPS * 32), 0, q, 1, a, per, by_segment);
+    const bool wide = rows * x <= 4 * TREE_CTAS;              // a row per block, about four blocks on an SM
+    const int per = wide ? 1 : TM_WARPS * std::max(1, rows * x / (TM_WARPS * 4 * TREE_CTAS));
+    const dim3 grid(x, (rows + per - 1) / per), block(TM_WARPS * 32);
+    if (a.vd <= 128)
+        return wide ? launch_pdl_try(k_ftree_merge<T, true, false>, grid, block, 0, q, 1, a, per, by_segment)
+                    : launch_pdl_try(k_ftree_merge<T, false, false>, grid, block, 0, q, 1, a, per, by_segment);
+    return wide ? launch_pdl_try(k_ftree_merge<T, true, true>, grid, block, 0, q, 1, a, per, by_segment)
+                : launch_pdl_try(k_ftree_merge<T, false, true>, grid, block, 0, q, 1, a, per, by_segment);
 }
 // Rows of a block, keys of a tile, tiles that a turn costs.  A tile takes about as long for its copies, waits and softmax as for the
 // products of 48 rows.
