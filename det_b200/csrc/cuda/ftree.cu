@@ -263,12 +263,12 @@ __global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs
         w = tree_start(a, cta + 1, lane, &share);
     }
     const TreeSeg s = tree_seg(a, w.seg);
-    // in places from the beginning of the segment: the border lies at w.place, the tiles at turn .. turn + tiles - 1
+    // the border lies at place w.place of the segment
     const int r0 = blockIdx.y * per, r1 = min(s.rows, r0 + per);
-    const bool mine = w.left > 0 && w.place > a.turn && w.place - share <= a.turn;
+    const bool mine = w.left > 0 && tree_tiles(a, s, w.place) > 0 && tree_tiles(a, s, w.place - share) == 0;
     pdl_wait();
     if (!mine || r0 >= r1) return;
-    const int n = 1 + (int)(share < (1 << 30) ? (unsigned)(s.tiles + a.turn - w.place + (int)share - 1) / (unsigned)share : 1);   // pieces
+    const int behind = tree_places(a, s) - 1 - w.place, n = 2 + (share <= behind ? (int)((unsigned)behind / (unsigned)share) : 0);   // pieces
     const size_t size = tree_piece_floats(a.block, a.vd);
     // the CTA ahead of the border had tiles of the segment before when its share began ahead of this one
     const float* head = a.part + ((size_t)cta * 2 + (w.place < share ? 1 : 0)) * size;

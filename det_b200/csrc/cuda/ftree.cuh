@@ -110,8 +110,13 @@ __device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, int seg) {
     s.tiles = s.rows > 0 ? (s.keys + a.tile - 1) / a.tile : 0;
     return s;
 }
-// Places of a segment in the deal, for one key/value head.
-__device__ __forceinline__ int tree_places(const TreeArgs& a, int tiles) { return tiles > 0 ? tiles + a.turn : 0; }
+// Places of a segment in the deal, for one key/value head: `turn`, then one for a tile, or two where it meets more than 128 rows (two
+// slots of k_ftree_tc).  A tile goes to the CTA that has its last place.
+__device__ __forceinline__ int tree_double(const TreeSeg& s) { return s.rows > 128 ? 1 : 0; }
+__device__ __forceinline__ int tree_places(const TreeArgs& a, const TreeSeg& s) { return s.tiles > 0 ? (s.tiles << tree_double(s)) + a.turn : 0; }
+__device__ __forceinline__ int tree_tiles(const TreeArgs& a, const TreeSeg& s, long long places) {      // of the segment's first places
+    return (int)(max(0ll, places - a.turn) >> tree_double(s));
+}
 // Places of a CTA.
 __device__ __forceinline__ long long tree_share(const TreeArgs& a, long long total) {
     if (total < 1ll << 31) return max(TREE_SHARE, (int)(((unsigned)total + a.ctas - 1) / (unsigned)a.ctas));
@@ -131,7 +136,7 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
     bool bad = false;
     for (int i = lane; i < segs; i += 32) {
         const TreeSeg s = tree_seg(a, i);
-        total += mine = tree_places(a, s.tiles);
+        total += mine = tree_places(a, s);
         bad |= s.bad;
     }
     if (cta == 0 && bad) report_size(a.error_flag);
@@ -145,11 +150,12 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
         w.seg = segment / a.kv_heads;
         w.g = segment - w.seg * a.kv_heads;
         long long before = 0;
-        for (int i = lane; i < w.seg; i += 32) before += tree_places(a, tree_seg(a, i).tiles);
+        for (int i = lane; i < w.seg; i += 32) before += tree_places(a, tree_seg(a, i));
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) before += __shfl_xor_sync(FULL, before, off);
-        const int places = tree_places(a, tree_seg(a, w.seg).tiles);
-        const long long begin = before * a.kv_heads + (long long)w.g * places, first = begin + a.turn;   // its first tile
+        const TreeSeg s = tree_seg(a, w.seg);
+        const int places = tree_places(a, s);
+        const long long begin = before * a.kv_heads + (long long)w.g * places, first = begin + a.turn + tree_double(s);   // where its first tile goes
         if (places == 0) return w;
         w.cta = first + places < 1ll << 31 ? (int)((unsigned)first / (unsigned)share) : (int)(first / share);
         const long long border = (w.cta + 1) * share;
@@ -163,7 +169,7 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
     w.cta = cta;
     long long base = 0;                                       // places ahead of this round's segments
     for (int i = lane;; i += 32) {
-        const int places = i >= segs ? 0 : segs <= 32 ? mine : tree_places(a, tree_seg(a, i).tiles);
+        const int places = i >= segs ? 0 : segs <= 32 ? mine : tree_places(a, tree_seg(a, i));
         long long sum = (long long)places * a.kv_heads;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -202,10 +208,10 @@ __device__ __forceinline__ bool tree_next(const TreeArgs& a, TreeWalk& k, TreeIt
             k.w.seg++;
             it.s = tree_seg(a, k.w.seg);
         }
-        const int from = k.w.place, n = (int)min((long long)(it.s.tiles + a.turn - from), k.w.left);
+        const int from = k.w.place, n = (int)min((long long)(tree_places(a, it.s) - from), k.w.left);
         it.g = k.w.g;
-        it.tile = max(0, from - a.turn);
-        it.n = max(0, from + n - a.turn) - it.tile;
+        it.tile = tree_tiles(a, it.s, from);
+        it.n = tree_tiles(a, it.s, from + n) - it.tile;
         k.w.left -= n;
         k.w.place = 0;
         if (++k.w.g == a.kv_heads) {

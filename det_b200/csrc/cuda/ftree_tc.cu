@@ -38,7 +38,7 @@ struct TtCfg {
 struct TtShape {
     int nkb, nvb;                                   // 64-element blocks of a key, of a value
     int stages, stage_bytes;
-    int both;                                       // the slots hold the same rows
+    int twice;                                      // blocks of 128 rows: one slot's room holds the next stretch's rows
     int q_bytes;                                    // of one slot's rows
 };
 
@@ -304,8 +304,10 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
     TreeItem it;
     bool ok = true;
     auto wait = [&](unsigned long long* bar, unsigned parity) { return __all_sync(FULL, mbar_wait(bar, parity, wl)) != 0; };   // by whole warps
-    const bool both = SLOTS == 2 && sh.both;         // the slots take every other tile of the same rows
-    const int lead = both ? 2 : 1;                   // tiles whose scores are asked for ahead
+    const bool twice = sh.twice != 0;
+    // the slots take every other tile of the same rows; tiles whose scores are asked for ahead
+    auto both_of = [](const TreeItem& x) { return SLOTS == 2 && x.s.rows <= TT_ROWS; };
+    auto lead_of = [&](const TreeItem& x) { return both_of(x) ? 2 : 1; };
     unsigned item = 0;                               // stretches so far
 
     if (warp == LOADS) {
@@ -327,6 +329,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 seq = s.b;
                 maps++;
             }
+            const int lead = lead_of(it);
             if (lane == 0) {
                 auto fetch = [&](bool value, int t) {
                     if (c >= (unsigned)sh.stages) ok = mbar_wait(&empty[sn], phase ^ 1u, wl);
@@ -360,8 +363,8 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
         unsigned c = 0, looked = 0;                  // tiles of the stretches before; phases of `raw`, a bit per stage
         while (ok && tree_next(a, walk, it)) {
             const TreeSeg& s = it.s;
-            const int qb = both ? item & 1 : 0;
-            if (item >= (both ? 2u : 1u)) ok = wait(&q_empty[qb], ((both ? item >> 1 : item) & 1u) ^ 1u);
+            const int qb = twice ? item & 1 : 0, lead = lead_of(it);
+            if (item >= (twice ? 2u : 1u)) ok = wait(&q_empty[qb], ((twice ? item >> 1 : item) & 1u) ^ 1u);
             if (!ok) break;
             // a row per `lanes` lanes; rows that are not there keep what is there (a row's scores are its own)
             const bf16* q = static_cast<const bf16*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 for (int r = tid / lanes; r < s.rows; r += qstep) {
                     const int row = s.r0 + r, node = (int)(row * a.per_magic >> 32), x = r & (TT_ROWS - 1);
                     const bf16* src = q + (size_t)node * a.ldq + (row - node * a.per_kv) * a.kd;
-                    copy16(smem_addr(Qs + (size_t)(both ? qb : r / TT_ROWS) * sh.q_bytes) + (unsigned)((qc >> 3) * TT_ROWS * 128 + x * 128 + (((qc ^ x) & 7) << 4)),
+                    copy16(smem_addr(Qs + (size_t)(twice ? qb : r / TT_ROWS) * sh.q_bytes) + (unsigned)((qc >> 3) * TT_ROWS * 128 + x * 128 + (((qc ^ x) & 7) << 4)),
                            qc * 8 < a.kd ? src + qc * 8 : src, qc * 8 < a.kd ? 16 : 0);
                 }
             copies_wait_all();
@@ -399,13 +402,13 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
             const unsigned long long q_desc = umma_desc(Qs), k_desc = umma_desc(ring), v_desc = umma_desc_mn(ring, KT * 128);
             unsigned c = 0, phase = 0, np[2] = {0, 0};   // place in the ring, weights taken per slot
             while (ok && tree_next(a, walk, it)) {
-                const int qb = both ? item & 1 : 0;
-                const bool second = !both && SLOTS == 2 && it.s.rows > TT_ROWS;
-                ok = mbar_wait(&q_full[qb], ((both ? item >> 1 : item) & 1u), wl);
+                const int qb = twice ? item & 1 : 0, lead = lead_of(it);
+                const bool both = both_of(it), second = it.s.rows > TT_ROWS;
+                ok = mbar_wait(&q_full[qb], ((twice ? item >> 1 : item) & 1u), wl);
                 if (!ok) break;
                 // descriptors of neighbouring steps differ in their address (units of 16 bytes) only
                 auto scores = [&](int slot, unsigned s) {
-                    unsigned long long q = q_desc + (unsigned)(both ? qb : slot) * (unsigned)(sh.q_bytes >> 4), k = k_desc + s * (unsigned)(sh.stage_bytes >> 4);
+                    unsigned long long q = q_desc + (unsigned)(twice ? qb : both ? 0 : slot) * (unsigned)(sh.q_bytes >> 4), k = k_desc + s * (unsigned)(sh.stage_bytes >> 4);
                     for (int e = 0; e < ksteps; e += 4) {
 #pragma unroll
                         for (int i = 0; i < 4; i++)
@@ -486,12 +489,12 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
         // after an expired wait the stretches are gone through without waiting, so that all warps meet at the barrier below
         while (tree_next(a, walk, it)) {
             const TreeSeg& s = it.s;
+            const bool both = both_of(it);
             const int br = both ? r : slot * TT_ROWS + r;                     // row of the block
             const bool mine = br < s.rows, any = (both ? quarter * 32 : slot * TT_ROWS + quarter * 32) < s.rows;
             const int row = s.r0 + min(br, s.rows - 1), node = row / a.per_kv;
             float m = -INFINITY, l = 0.0f;
-            const bool idle = !both && slot && s.rows <= TT_ROWS;            // the slot has no rows in this stretch
-            const int jobs = idle ? 0 : both ? (it.n + 1 - slot) / 2 : it.n;
+            const int jobs = both ? (it.n + 1 - slot) / 2 : it.n;
             for (int j = 0; j < jobs; j++) {
                 const int k0 = (it.tile + (both ? 2 * j + slot : j)) * KT;
                 const bool tree = k0 + KT > s.edge;
@@ -568,7 +571,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 f1 = ex2((y.x - b) * a.scale2);
                 l = f0 * x.y + f1 * y.y;
             }
-            if (any && !idle) {
+            if (any) {
                 const unsigned o0 = tmem + lanes + Cfg::O_COL + (both ? 0 : slot * (256 / SLOTS)), o1 = o0 + 256 / SLOTS;
                 const bool fix = *reinterpret_cast<volatile int*>(&odd[item & 3]) == (int)item + 1;
                 const int orow = s.first + node, h = it.g * a.per_kv + row % a.per_kv;
@@ -642,7 +645,7 @@ void ftree_tc_shape(int rows, int kd, int vd, int* block, int* tile, int* turn) 
     const bool wide = kd > 128 || vd > 128;
     *block = wide || rows <= TT_ROWS ? TT_ROWS : 2 * TT_ROWS;
     *tile = wide ? 64 : 128;
-    *turn = *block == TT_ROWS ? 4 : 2;
+    *turn = 4;
 }
 
 // A cache's keys or values (`size` elements a head) as [rows][heads][size], boxes of 64 elements of one head x `box` rows, zeros outside.
@@ -663,7 +666,7 @@ static cudaError_t launch(const TreeArgs& a, cudaStream_t q) {
     sh.nvb = (a.vd + 63) / 64;
     sh.q_bytes = sh.nkb * TT_ROWS * 128;
     sh.stage_bytes = std::max(sh.nkb, sh.nvb) * KT * 128;
-    sh.both = SLOTS == 2 && a.block == TT_ROWS;
+    sh.twice = SLOTS == 2 && a.block == TT_ROWS;
     const size_t fixed = (size_t)SLOTS * sh.q_bytes + sizeof(TtTables);
     sh.stages = (int)std::min<size_t>(TT_STAGES, (TT_SMEM - fixed) / sh.stage_bytes);
     const size_t smem = fixed + (size_t)sh.stages * sh.stage_bytes;
