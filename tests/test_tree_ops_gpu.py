@@ -464,6 +464,119 @@ def test_a_run_equals_the_attention_op_of_the_models(gpu, libs):
         assert np.abs(got - want).max() <= tol
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nodes", [1, 3, 20, 70])
+def test_scores_that_rise_and_fall_along_the_keys(nodes, dtype, gpu, libs):
+    """The running maximum moves far from tile to tile, by little, or not at all: the reference of the weights follows it."""
+    n = 900
+    for low, high in [(-40.0, 60.0), (60.0, -40.0), (0.0, 4.0), (-300.0, 300.0), (5.0, 5.0)]:
+        a = Attn(gpu, libs, dtype, 4, 1, 64, 64, [n], [nodes], masks=[to.tree_mask(list(range(-1, nodes - 1)))], seed=nodes)
+        c = a.values[0].copy()
+        ramp = np.linspace(low, high, n + nodes)
+        c[:n + nodes, :64] *= 0.1
+        c[:n + nodes, 0] = ramp                                # the first element carries the trend (q's is 8: scale * 8 = 1)
+        a.caches[0], a.values[0] = store(gpu, c, dtype)
+        q = a.q.copy()
+        q[..., 0] = 8.0
+        a.qp, a.q = store(gpu, q, dtype)
+        a.check(a.call())
+    assert size_error(gpu) == 0
+
+
+def test_rows_behind_the_fourth_gigabyte(gpu, libs):
+    """Byte offsets inside one cache pass 32 bits: rows are written, moved and attended there by every kernel."""
+    H, G, d = 8, 8, 128
+    for dtype, esize in (("bf16", 2), ("f32", 4)):
+        ld = gpu.d.det_f_attn_ld(G, d, d)
+        at = (1 << 32) // (ld * esize) + 1000
+        cap = at + 300
+        cache = gpu.d.det_malloc(cap * ld * esize)
+        assert cache
+        rng = np.random.default_rng(5)
+        for nodes in (2, 40, 200):
+            s = Step(gpu, libs, [at], [nodes])
+            ref = s.ref([cache])
+            y = np.float32(rng.standard_normal((nodes, (H + 2 * G) * d)))
+            y[:, H * d:(H + G) * d] = 0.0                      # keys of zero: a row's weights are even over everything it sees
+            y[:, :H * d] *= 0.1
+            q, out = gpu.space(4 * nodes * H * d), gpu.space(4 * nodes * H * d)
+            qk = libs.FQkOp(heads=H, kv_heads=G, dim=d, vdim=d, rot_dims=0, half=0, eps=0.0, cap=cap, dtype=code(libs, dtype), y=gpu.f32(y), ldy=y.shape[1],
+                            q_off=0, k_off=H * d, v_off=(H + G) * d, q=q, seq=ref)
+            assert gpu.d.det_f_qk_rope(C.byref(qk), None) == 0
+            m = to.tree_mask([-1] * nodes)                     # every node by itself
+            ta = libs.FTreeOp(heads=H, kv_heads=G, dim=d, vdim=d, scale=1.0, cap=cap, dtype=code(libs, dtype), q=q, mask=gpu.put(to.bits(m, 7)), mask_ld=7,
+                              out=out, ldo=H * d, scratch=gpu.space(gpu.d.det_f_tree_scratch_bytes(H, G, d, nodes)), seq=ref)
+            assert gpu.d.det_f_tree_attn(C.byref(ta), None) == 0
+            got = load(gpu, out, (nodes, H * d), dtype)
+            v = y[:, (H + G) * d:].astype(float)
+            if dtype == "bf16":
+                v = ho.bf16_values(ho.bf16_bits(np.float32(v))).astype(float)
+            # all other keys and values are zero: the weight is 1 / (at + 1), known to 2 u_act and the sum of `at` terms in fp32
+            want = v / (at + 1)
+            tol = np.abs(want) * (4 * to.UNIT[dtype] + (at / 16 + 100) * U32) + 1e-12
+            assert (np.abs(got - want) <= tol).all(), np.abs(got / np.where(want == 0, 1, want) - 1).max()
+            kept = [1, nodes - 1] if nodes > 2 else [1]
+            op = libs.FKeepOp(caches=1, seqs=1, cap=cap, row_bytes=ld * esize, table=ref.table, len=s.len_p, keep=ints(gpu, kept), keep_ld=2,
+                              count=ints(gpu, [len(kept)]), max_count=2)
+            assert gpu.d.det_f_tree_keep(C.byref(op), None) == 0
+            rows = np.zeros((len(kept), ld), np.uint16 if esize == 2 else np.float32)
+            gpu.d.det_memcpy(rows.ctypes.data, cache + at * ld * esize, rows.nbytes, None)
+            gpu.d.det_sync()
+            rows = ho.bf16_values(rows).astype(float) if esize == 2 else rows.astype(float)
+            assert np.array_equal(rows[:, G * d:], v[kept])
+            gpu.d.det_memset(cache + at * ld * esize, 0, 250 * ld * esize, None)
+        gpu.d.det_free(cache)
+    assert size_error(gpu) == 0
+
+
+def test_calls_on_two_streams_and_replays_of_two_graphs(gpu, libs):
+    """Calls with scratch of their own overlap on two streams; two captured calls that share scratch are replayed in turn, with other
+    lengths."""
+    rt = C.CDLL("libcudart.so.12")
+    streams = [C.c_void_p() for _ in range(2)]
+    for s in streams:
+        assert rt.cudaStreamCreateWithFlags(C.byref(s), 1) == 0
+    rng = np.random.default_rng(11)
+    cases = [Attn(gpu, libs, "bf16", 16, 2, 128, 128, [6000, 40], [30, 5], masks=random_masks([30, 5], rng), seed=i) for i in range(2)]
+    ops = [a.op() for a in cases]
+    gpu.d.det_sync()
+    for _ in range(20):
+        for op, s in zip(ops, streams):
+            assert gpu.d.det_f_tree_attn(C.byref(op), s) == 0
+    gpu.d.det_sync()
+    for a in cases:
+        a.check(load(gpu, a.out, (a.s.rows, a.ldo), "bf16"))
+    for s in streams:
+        assert rt.cudaStreamDestroy(s) == 0
+    graphs = []
+    for op in ops:
+        op.scratch = ops[0].scratch
+        gpu.d.det_graph_begin()
+        assert gpu.d.det_f_tree_attn(C.byref(op), None) == 0
+        graphs.append(gpu.d.det_graph_end())
+        assert graphs[-1]
+    for lens in ([6000, 40], [77, 3000], [0, 129], [6000, 40]):
+        for a in cases:
+            fits = [min(x, a.cap - n) for x, n in zip(lens, a.s.nodes)]
+            b = np.array(fits, np.int32)
+            gpu.d.det_memcpy(a.s.len_p, b.ctypes.data, 8, None)
+            gpu.d.det_sync()
+            a.s.lens = fits
+            for i, (n, first) in enumerate(zip(a.s.nodes, fits)):   # every row of the cache holds something
+                c = np.nan_to_num(a.values[i], nan=0.5)
+                a.values[i] = c
+                bits = ho.bf16_bits(np.float32(c))
+                gpu.d.det_memcpy(a.caches[i], bits.ctypes.data, bits.nbytes, None)
+                gpu.d.det_sync()
+        for g in (graphs[0], graphs[1], graphs[1], graphs[0]):
+            gpu.d.det_graph_launch(g)
+        gpu.d.det_sync()
+        for a in cases:
+            a.check(load(gpu, a.out, (a.s.rows, a.ldo), "bf16"))
+    for g in graphs:
+        gpu.d.det_graph_free(g)
+
+
 # ------------------------------------------------------------------------------------------------------------------ kept rows
 @pytest.mark.parametrize("row_bytes", [16, 48, 4096, 4112])
 def test_kept_rows_move_up(row_bytes, gpu, libs):
