@@ -1,7 +1,7 @@
 // Attention of a step of drafted tokens (include/det_b200.h, det_ftree_op): one pass over the keys with the running maximum and sum of
 // the softmax, in 32-bit.  ftree.cuh says how the work is dealt out.
 //
-//   k_ftree_few    bfloat16, up to 16 rows per key/value head: ftree_few.cu.
+//   k_ftree_few    bfloat16, few rows or short caches: ftree_few.cu.
 //   k_ftree_tc     bfloat16: ftree_tc.cu.
 //   k_ftree_simt   fp32: products on the CUDA cores, 256 threads over a tile of query rows x 64 keys.
 //   k_ftree_merge  adds the pieces of the segments that several CTAs shared.

@@ -1,7 +1,7 @@
-// Tree attention over bfloat16 caches with at most 16 query rows per key/value head (decoded tokens, small trees): the rows are one MMA
-// tile, so a key costs 16 rows of products whatever their number, and what bounds the call is the cache's bytes or, for short caches,
-// latency.  One launch: a cluster of CTAs shares the keys of a (sequence, key/value head), each of its warps walks 16-key tiles through
-// a ring of its own, and the cluster adds its pieces over distributed shared memory.
+// Tree attention over bfloat16 caches for decoded tokens and small trees: 16 query rows of a key/value head are one MMA tile, so a key
+// costs 16 rows of products whatever their number, and what bounds the call is the cache's bytes or, for short caches, latency.  One
+// launch: a cluster of CTAs shares the keys of a (sequence, key/value head, block of 16 rows), each of its warps walks 16-key tiles
+// through a ring of its own, and the cluster adds its pieces over distributed shared memory.
 #include "flash.cuh"
 #include "ftree.cuh"
 #include <algorithm>
@@ -33,7 +33,7 @@ __device__ __forceinline__ float2 far2(unsigned addr) {
     return v;
 }
 
-// grid (CTAs of a cluster, key/value heads, sequences)
+// grid (CTAs of a cluster, key/value heads x row blocks, sequences)
 template <int DV>
 __global__ void __launch_bounds__(TF_WARPS * 32) k_ftree_few(const TreeArgs a) {
     extern __shared__ __align__(16) uint8_t tfs[];
@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(TF_WARPS * 32) k_ftree_few(const TreeArgs a) {
     const int dqp = (a.kd + 15) & ~15, ldk = dqp + 8;
     constexpr int LDV = DV + 8;
     bf16* Q = reinterpret_cast<bf16*>(tfs);                   // [16][ldk]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x, ranks = gridDim.x, g = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x, ranks = gridDim.x, g = blockIdx.y / a.blocks, rb = blockIdx.y % a.blocks;
     bf16* Kt = Q + TF_ROWS * ldk + (size_t)warp * TF_STAGES * TF_KEYS * (ldk + LDV);   // this warp's [stage][16][ldk]
     bf16* Vt = Kt + TF_STAGES * TF_KEYS * ldk;                // ... and [stage][16][LDV]
     pdl_trigger();
@@ -49,8 +49,8 @@ __global__ void __launch_bounds__(TF_WARPS * 32) k_ftree_few(const TreeArgs a) {
     if (dqp != a.kd)                                          // what the copies leave unwritten enters products
         for (int i = lane; i < TF_STAGES * TF_KEYS; i += 32) *reinterpret_cast<uint4*>(Kt + i * ldk + a.kd) = make_uint4(0, 0, 0, 0);
     pdl_wait();
-    const TreeSeg s = tree_seg(a, blockIdx.z);
-    if (s.bad && rank == 0 && g == 0 && threadIdx.x == 0) report_size(a.error_flag);
+    const TreeSeg s = tree_seg(a, blockIdx.z * a.blocks + rb);
+    if (s.bad && rank == 0 && blockIdx.y == 0 && threadIdx.x == 0) report_size(a.error_flag);
     if (s.tiles == 0) return;                                 // the whole cluster
     const int per = (s.tiles + ranks - 1) / ranks, t1 = min(s.tiles, (rank + 1) * per);
     const int last = s.len + s.n - 1;
@@ -73,9 +73,9 @@ __global__ void __launch_bounds__(TF_WARPS * 32) k_ftree_few(const TreeArgs a) {
     for (int i = 0; i < TF_STAGES - 1; i++) fetch(t + i * TF_WARPS, i);
     const bf16* q = static_cast<const bf16*>(a.q) + (size_t)s.first * a.ldq + (size_t)g * a.per_kv * a.kd;
     for (int i = threadIdx.x; i < TF_ROWS * (dqp / 8); i += TF_WARPS * 32) {
-        const int r = i / (dqp / 8), v = i - r * (dqp / 8), node = (int)(r * a.per_magic >> 32);
+        const int r = i / (dqp / 8), v = i - r * (dqp / 8), row = s.r0 + r, node = (int)(row * a.per_magic >> 32);
         uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < s.rows && v < kvec) x = *reinterpret_cast<const uint4*>(q + (size_t)node * a.ldq + (r - node * a.per_kv) * a.kd + v * 8);
+        if (r < s.rows && v < kvec) x = *reinterpret_cast<const uint4*>(q + (size_t)node * a.ldq + (row - node * a.per_kv) * a.kd + v * 8);
         *reinterpret_cast<uint4*>(Q + r * ldk + v * 8) = x;
     }
     __syncthreads();
@@ -126,8 +126,8 @@ __global__ void __launch_bounds__(TF_WARPS * 32) k_ftree_few(const TreeArgs a) {
             unsigned seen[2][1];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int r = min((lane >> 2) + i * 8, s.rows - 1);
-                tree_seen<1>(a, s, (int)(r * a.per_magic >> 32), k0, seen[i]);
+                const int row = s.r0 + min((lane >> 2) + i * 8, s.rows - 1);
+                tree_seen<1>(a, s, (int)(row * a.per_magic >> 32), k0, seen[i]);
             }
 #pragma unroll
             for (int n = 0; n < 2; n++)
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(TF_WARPS * 32) k_ftree_few(const TreeArgs a) {
             asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(any) : "r"(in_cta(far_odd, c)) : "memory");
             fix |= any != 0;
         }
-        const int node = (int)(r * a.per_magic >> 32);
+        const int row = s.r0 + r, node = (int)(row * a.per_magic >> 32);
         y = scaled4(y, l == 0.0f ? 0.0f : 1.0f / l);
         if (fix) {                                            // values of attended keys that are not finite (they entered the product as zeros)
             float z[4] = {y.x, y.y, y.z, y.w};
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(TF_WARPS * 32) k_ftree_few(const TreeArgs a) {
             }
             y = make_float4(z[0], z[1], z[2], z[3]);
         }
-        TreeOut<bf16>(a, s.first + node, g * a.per_kv + r - node * a.per_kv).put4at(v, y);
+        TreeOut<bf16>(a, s.first + node, g * a.per_kv + row - node * a.per_kv).put4at(v, y);
     }
     __syncwarp();
     cluster_sync();                                           // nobody leaves while its pieces are read
@@ -234,35 +234,40 @@ static cudaError_t launch(const TreeArgs& a, int ranks, cudaStream_t q) {
     cudaError_t e = cudaFuncSetAttribute(k_ftree_few<DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_ftree_few<DV>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    return launch_pdl_try(k_ftree_few<DV>, dim3(ranks, a.kv_heads, a.seq.seqs), dim3(TF_WARPS * 32), smem, q, ranks, a);
+    return launch_pdl_try(k_ftree_few<DV>, dim3(ranks, a.kv_heads * a.blocks, a.seq.seqs), dim3(TF_WARPS * 32), smem, q, ranks, a);
 }
 
 // CTAs of a cluster: a power of two, so that all clusters fill the device about twice over, and no more than there are tiles for the
-// warps.
-static int few_ranks(int kv_heads, int seqs, int max_len) {
-    const long long clusters = (long long)seqs * kv_heads;
+// warps.  Clusters of 16 find room eight at a time (16 of them took two rounds: 20.4 us where 24 clusters of 8 took 11.1).
+static int few_ranks(long long clusters, int max_len) {
     const int tiles = max_len / TF_KEYS + 1;
     int ranks = 1;
-    while (ranks < 16 && clusters * ranks * 2 <= 2 * TREE_CTAS && ranks * TF_WARPS < tiles) ranks *= 2;
+    while (ranks < (clusters <= 8 ? 16 : 8) && clusters * ranks * 2 <= 2 * TREE_CTAS && ranks * TF_WARPS < tiles) ranks *= 2;
     return ranks;
 }
-// Against k_ftree_tc, which any number of rows can take: a CTA here moves about 24 GB/s of cache with keys and values of 128 (its copies
-// in flight), so few clusters of a long cache leave HBM idle, where the other kernel reaches 5.5 TB/s at any split; but that one needs
-// about 8 us more for its larger start and its second launch.  Measured, 8 key/value heads of 128, this kernel against the other: 11.9 /
-// 17.1 us at 2048 keys, 19.3 / 22.7 at 8192, 88 / 68 at 65536; one head of 32768 keys 37 / 23; 32 sequences of 4096 keys 100 / 108.
+// This kernel or k_ftree_tc, by what both were measured to take (in us, 8 key/value heads of 128, this one / the other):
+//   here   8.5 for every round of CTAs, and the cache's bytes once per 16 rows at 24 GB/s a CTA (keys and values of 128 in its ring), 5.2 TB/s
+//          together: 11.0 / 16.3 at 5 rows of 512 keys, 14.3 / 19.9 at 40 rows of 2048, 30.4 / 25.0 at 40 rows of 8192, 88 / 68 at 5 rows
+//          of 65536; 32.3 / 43.7 for 16 sequences of 2048 keys and 5 rows, 98 / 49 with 40 rows
+//   there  15 for its start and its second launch, 5 for a turn, the larger of the bytes at 6 TB/s and 1.45 for a tile of 128 x 128
 bool ftree_few_takes(const TreeArgs& a, int rows) {
-    if (rows > TF_ROWS || a.kv_heads > 65535 || a.seq.seqs > 65535) return false;
-    const int ranks = few_ranks(a.kv_heads, a.seq.seqs, a.seq.max_len), dv = a.vd <= 64 ? 64 : a.vd <= 128 ? 128 : 256;
-    const double row = 2.0 * (a.kd + a.vd), bytes = row * a.kv_heads * a.seq.seqs * a.seq.max_len;
-    const double at_once = std::min((double)a.seq.seqs * a.kv_heads * ranks, (few_smem(a.kd, dv) <= 113 * 1024 ? 2.0 : 1.0) * TREE_CTAS);
-    return bytes / std::min(at_once * 24e9 * row / 512, 5.5e12) <= bytes / 5.5e12 + 8e-6;
+    const int blocks = (rows + TF_ROWS - 1) / TF_ROWS, len = a.seq.max_len + a.seq.max_nodes;
+    const long long clusters = (long long)a.seq.seqs * a.kv_heads * blocks;
+    if (blocks > 16 || (long long)a.kv_heads * blocks > 65535) return false;
+    const int dv = a.vd <= 64 ? 64 : a.vd <= 128 ? 128 : 256;
+    const double row = 2.0 * (a.kd + a.vd), heads = (double)a.kv_heads * a.seq.seqs, bytes = row * heads * len;
+    const double slots = (few_smem(a.kd, dv) <= 113 * 1024 ? 2.0 : 1.0) * TREE_CTAS, ctas = (double)clusters * few_ranks(clusters, a.seq.max_len);
+    const double here = 8.5e-6 * (double)((long long)(ctas / slots + 0.999)) + bytes * blocks / std::min(std::min(ctas, slots) * 24e9 * row / 512, 5.2e12);
+    const double tiles = heads * (len / 128 + 1) * ((rows + 127) / 128);
+    const double there = 15e-6 + heads / TREE_CTAS * 5e-6 + std::max(bytes / 6e12, tiles / TREE_CTAS * 1.45e-6);
+    return here <= there;
 }
 void ftree_few_shape(int* block, int* tile) {
     *block = TF_ROWS;
     *tile = TF_KEYS;
 }
 cudaError_t ftree_few_launch(const TreeArgs& a, cudaStream_t q) {
-    const int ranks = few_ranks(a.kv_heads, a.seq.seqs, a.seq.max_len);
+    const int ranks = few_ranks((long long)a.seq.seqs * a.kv_heads * a.blocks, a.seq.max_len);
     return a.vd <= 64 ? launch<64>(a, ranks, q) : a.vd <= 128 ? launch<128>(a, ranks, q) : launch<256>(a, ranks, q);
 }
 
