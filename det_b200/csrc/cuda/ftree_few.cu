@@ -253,7 +253,8 @@ static int few_ranks(long long clusters, int max_len) {
 bool ftree_few_takes(const TreeArgs& a, int rows) {
     const int blocks = (rows + TF_ROWS - 1) / TF_ROWS, len = a.seq.max_len + a.seq.max_nodes;
     const long long clusters = (long long)a.seq.seqs * a.kv_heads * blocks;
-    if (blocks > 16 || (long long)a.kv_heads * blocks > 65535) return false;
+    if (blocks > 16 || (long long)a.kv_heads * blocks > 65535 || (float_flags() & 16)) return false;
+    if (float_flags() & 32) return true;
     const int dv = a.vd <= 64 ? 64 : a.vd <= 128 ? 128 : 256;
     const double row = 2.0 * (a.kd + a.vd), heads = (double)a.kv_heads * a.seq.seqs, bytes = row * heads * len;
     const double slots = (few_smem(a.kd, dv) <= 113 * 1024 ? 2.0 : 1.0) * TREE_CTAS, ctas = (double)clusters * few_ranks(clusters, a.seq.max_len);

@@ -787,7 +787,8 @@ typedef struct {
 int det_f_tree_keep(const det_fkeep_op* op, cudaStream_t st);
 
 /* Measurement switches of the floating-point ops (results agree up to rounding): bit 0 no norm in the GEMV's prologue, bit 1 no
- * GEMV, bit 2 no split of K in the tensor-core GEMM, bit 3 no tensor-core attention.                                   */
+ * GEMV, bit 2 no split of K in the tensor-core GEMM, bit 3 no tensor-core attention; tree attention in bfloat16: bit 4 never, bit 5
+ * always (up to 256 rows per key/value head) the kernel for few rows.                                                      */
 void det_debug_set_float(int flags);
 
 #ifdef __cplusplus

@@ -221,8 +221,9 @@ class Attn:
         self.mask_ld = words
         self.mask_p = None
         if masks is not None:
-            w = np.concatenate([to.bits(m, words) for m in masks] + [np.full((extra, words), 0xffffffff, np.uint32)])
-            w[:, self.s.max_nodes // 32 + 1:] = 0xffffffff     # words behind the tree are not looked at
+            def wide(m):                                       # bits behind the tree are not looked at
+                return to.bits(np.concatenate([m, np.ones((len(m), words * 32 - m.shape[1]), bool)], 1), words)
+            w = np.concatenate([wide(m) for m in masks] + [np.full((extra, words), 0xffffffff, np.uint32)])
             self.mask_p = gpu.put(w)
         self.gate = np.float32(rng.standard_normal((self.s.rows, heads + 1))) if gate else None
         self.vt = rope_tables(gpu, v, 64, 50.0) if vrot else None
@@ -238,10 +239,23 @@ class Attn:
                                  vrope_cos=self.vt[0] if self.vt else None, vrope_sin=self.vt[1] if self.vt else None, out=self.out, ldo=self.ldo,
                                  scratch=self.scratch, seq=self.s.ref(self.caches))
 
-    def call(self):
+    def call(self, flags=0):
+        self.out, _ = store(self.gpu, np.full((self.s.rows, self.ldo), 7.0), self.dtype)
         op = self.op()
-        assert self.gpu.d.det_f_tree_attn(C.byref(op), None) == 0
+        self.gpu.d.det_debug_set_float(flags)
+        try:
+            assert self.gpu.d.det_f_tree_attn(C.byref(op), None) == 0
+        finally:
+            self.gpu.d.det_debug_set_float(0)
         return load(self.gpu, self.out, (self.s.rows, self.ldo), self.dtype)
+
+    def call_each(self):
+        """The outputs of every kernel of the type (bfloat16: the one for many rows, the one for few)."""
+        return [self.call(f) for f in ((0,) if self.dtype == "f32" else (16, 32))]
+
+    def check_each(self):
+        for got in self.call_each():
+            self.check(got)
 
     def seen(self, b):
         a, n = self.s.lens[b], self.s.nodes[b]
@@ -297,7 +311,7 @@ def test_attention_of_trees(heads, dtype, gpu, libs):
     rng = np.random.default_rng(sum(heads))
     for lens, nodes, extra in [([0], [1], 0), ([1], [1], 0), ([130], [7], 0), ([0, 63, 64, 65, 200, 5], [3, 1, 16, 0, 33, 2], 2), ([700], [64], 1)]:
         a = Attn(gpu, libs, dtype, *heads, lens, nodes, masks=random_masks(nodes, rng), extra=extra, seed=len(nodes))
-        a.check(a.call())
+        a.check_each()
     assert size_error(gpu) == 0
 
 
@@ -307,7 +321,7 @@ def test_attention_of_runs(heads, dtype, gpu, libs):
     """No mask: prompts and single tokens, at the edges of the tiles."""
     for lens, nodes in [([0], [1]), ([127], [1]), ([128], [1]), ([0], [200]), ([61, 0, 300], [70, 129, 1]), ([5], [333])]:
         a = Attn(gpu, libs, dtype, *heads, lens, nodes, seed=lens[0], ldo=heads[0] * heads[3] + 5)
-        a.check(a.call())
+        a.check_each()
     assert size_error(gpu) == 0
 
 
@@ -320,9 +334,9 @@ def test_rows_that_attend_nothing(dtype, gpu, libs):
         masks = random_masks(nodes, rng, empty=0.4)
         masks[0][:] = False
         a = Attn(gpu, libs, dtype, 4, 2, 64, 64, lens, nodes, masks=masks)
-        got = a.call()
-        a.check(got)
-        assert (got[:9] == 0).all()
+        for got in a.call_each():
+            a.check(got)
+            assert (got[:9] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -338,18 +352,18 @@ def test_values_that_are_not_finite_stay_with_the_rows_that_attend_them(bad, dty
     c[a0 + node, 2 * 64 + col] = bad                           # one element of key/value head 0
     c[a0 + 9, :64] = np.nan                                    # the key of another node, in the same head
     a.caches[0], a.values[0] = store(gpu, c, dtype)
-    got = a.call()
     hit, lost = m[:, node], m[:, 9]
-    for h in range(4):
-        x = got[:, h * 64:(h + 1) * 64]
-        if h >= 2:
-            assert np.isfinite(x).all()
-            continue
-        assert np.isnan(x[lost]).all()
-        assert np.isfinite(np.delete(x[~lost], col, 1)).all()
-        assert np.isfinite(x[~lost & ~hit]).all()
-        one = x[hit & ~lost, col]
-        assert (np.isnan(one) if np.isnan(bad) else one == bad).all()
+    for got in a.call_each():
+        for h in range(4):
+            x = got[:, h * 64:(h + 1) * 64]
+            if h >= 2:
+                assert np.isfinite(x).all()
+                continue
+            assert np.isnan(x[lost]).all()
+            assert np.isfinite(np.delete(x[~lost], col, 1)).all()
+            assert np.isfinite(x[~lost & ~hit]).all()
+            one = x[hit & ~lost, col]
+            assert (np.isnan(one) if np.isnan(bad) else one == bad).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -364,12 +378,12 @@ def test_values_of_the_cache_that_are_not_finite_reach_every_row(masked, dtype, 
         c[at, 64 + 9] = bad
         c[150 + 30, 64 + 20] = bad                             # node 30
         a.caches[0], a.values[0] = store(gpu, c, dtype)
-        got = a.call().reshape(40, 2, 64)
-        for x in (got[:, 0], got[:, 1]):
-            assert (np.isnan(x[:, 9]) if np.isnan(bad) else x[:, 9] == bad).all()
-            hit = a.seen(0)[:, 150 + 30]
-            assert (np.isnan(x[hit, 20]) if np.isnan(bad) else x[hit, 20] == bad).all()
-            assert np.isfinite(np.delete(x, [9, 20], 1)).all() and np.isfinite(x[~hit, 20]).all()
+        hit = a.seen(0)[:, 150 + 30]
+        for got in a.call_each():
+            for x in np.moveaxis(got.reshape(40, 2, 64), 1, 0):
+                assert (np.isnan(x[:, 9]) if np.isnan(bad) else x[:, 9] == bad).all()
+                assert (np.isnan(x[hit, 20]) if np.isnan(bad) else x[hit, 20] == bad).all()
+                assert np.isfinite(np.delete(x, [9, 20], 1)).all() and np.isfinite(x[~hit, 20]).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -378,7 +392,7 @@ def test_gates_and_rotated_values(dtype, gpu, libs):
     for gate, vrot in [(1, 0), (0, 1), (1, 1)]:
         for heads, lens, nodes in [((6, 2, 40, 24), [5, 300], [4, 13]), ((8, 2, 128, 128), [2000, 64], [20, 1]), ((2, 1, 64, 256), [100], [90])]:
             a = Attn(gpu, libs, dtype, *heads, lens, nodes, masks=random_masks(nodes, rng), gate=gate, vrot=vrot)
-            a.check(a.call())
+            a.check_each()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -388,10 +402,10 @@ def test_long_unequal_contexts_are_shared_out(dtype, gpu, libs):
     lens = [9000, 3, 0, 517, 4100, 64, 2049]
     nodes = [5, 1, 2, 17, 64, 30, 1]
     a = Attn(gpu, libs, dtype, 10, 2, 128, 128, lens, nodes, masks=random_masks(nodes, rng), sharp=4.0)
-    a.check(a.call())
+    a.check_each()
     b = Attn(gpu, libs, dtype, 4, 1, 64, 64, [20000], [1], sharp=3.0)
-    b.check(b.call())
-    b.check(b.call())                                          # the scratch as the first call left it
+    b.check_each()
+    b.check_each()                                          # the scratch as the first call left it
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -400,7 +414,7 @@ def test_many_small_sequences(dtype, gpu, libs):
     nodes = [int(n) for n in rng.integers(0, 4, 300)]
     lens = [int(n) for n in rng.integers(0, 150, 300)]
     a = Attn(gpu, libs, dtype, 4, 2, 32, 32, lens, nodes, masks=random_masks(nodes, rng), extra=4)
-    a.check(a.call())
+    a.check_each()
 
 
 def test_results_repeat_and_do_not_depend_on_the_bounds(gpu, libs):
@@ -408,12 +422,12 @@ def test_results_repeat_and_do_not_depend_on_the_bounds(gpu, libs):
     nodes, lens = [6, 3, 1], [3000, 17, 800]
     masks = random_masks(nodes, rng)
     a = Attn(gpu, libs, "bf16", 8, 2, 128, 128, lens, nodes, masks=masks)
-    first = a.call()
-    assert np.array_equal(first, a.call())
-    a.s.max_len = 0
-    a.check(a.call())
-    a.s.max_len = 100000
-    a.check(a.call())
+    for flags in (0, 16, 32):
+        assert np.array_equal(a.call(flags), a.call(flags))
+    for bound in (0, 100000):
+        a.s.max_len = bound
+        a.check(a.call())
+        a.check_each()
 
 
 def test_sequences_that_do_not_fit_are_left_out(gpu, libs):
@@ -426,9 +440,12 @@ def test_sequences_that_do_not_fit_are_left_out(gpu, libs):
             op = a.op()
             op.cap, op.seq.len = cap, ints(gpu, lens)
             # the caches keep 70 rows: a smaller cap only narrows what may be read
-            assert gpu.d.det_f_tree_attn(C.byref(op), None) == 0
-            assert size_error(gpu) == SIZE_ERROR
-            a.check(load(gpu, a.out, (a.s.rows, a.ldo), dtype), rows={1 - bad})
+            for flags in (16, 32):
+                gpu.d.det_debug_set_float(flags)
+                assert gpu.d.det_f_tree_attn(C.byref(op), None) == 0
+                gpu.d.det_debug_set_float(0)
+                assert size_error(gpu) == SIZE_ERROR
+                a.check(load(gpu, a.out, (a.s.rows, a.ldo), dtype), rows={1 - bad})
 
 
 def test_a_run_equals_the_attention_op_of_the_models(gpu, libs):
@@ -479,7 +496,7 @@ def test_scores_that_rise_and_fall_along_the_keys(nodes, dtype, gpu, libs):
         q = a.q.copy()
         q[..., 0] = 8.0
         a.qp, a.q = store(gpu, q, dtype)
-        a.check(a.call())
+        a.check_each()
     assert size_error(gpu) == 0
 
 
