@@ -165,6 +165,17 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
     }
     const long long u0 = cta * share;
     if (u0 >= total) return w;
+    if (segs <= 32 && total < 1ll << 31) {                     // the usual case in 32 bits
+        int sum = mine * a.kv_heads;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int v = __shfl_up_sync(FULL, sum, off);
+            if (lane >= off) sum += v;
+        }
+        const int src = __ffs(__ballot_sync(FULL, sum > (int)u0)) - 1, per = __shfl_sync(FULL, mine, src);
+        const unsigned in = (unsigned)((int)u0 - __shfl_sync(FULL, sum - mine * a.kv_heads, src));
+        return {src, (int)(in / (unsigned)per), (int)(in % (unsigned)per), min(share, total - u0), cta};
+    }
     w.left = min(share, total - u0);
     w.cta = cta;
     long long base = 0;                                       // places ahead of this round's segments

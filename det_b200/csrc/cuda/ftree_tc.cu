@@ -144,12 +144,13 @@ __device__ __forceinline__ void tt_maps(const CUtensorMap& mk, const CUtensorMap
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-        asm volatile("tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned [%0], [%1], 128;" ::"l"(to + i * 128),
-                     "r"(smem_addr(sm[i]))
-                     : "memory");
+    for (int i = 0; i < 2; i++) reinterpret_cast<unsigned*>(to + i * 128)[lane] = reinterpret_cast<const unsigned*>(sm[i])[lane];
+    __syncwarp();
+    if (lane == 0) {                                 // the lane that names them: one release for both
+        asm volatile("fence.proxy.tensormap::generic.release.gpu;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 2; i++) asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(to + i * 128) : "memory");
+        for (int i = 0; i < 2; i++) asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(to + i * 128) : "memory");
+    }
 }
 __device__ __forceinline__ void tt_load(void* dst, const void* map, int x, int head, int row, unsigned long long* bar, unsigned long long policy) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(
