@@ -158,25 +158,28 @@ __device__ __forceinline__ void tt_load(void* dst, const void* map, int x, int h
                  "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_addr(bar)), "l"(policy)
                  : "memory");
 }
-// Values that are not finite become zeros in a staged tile; true when there were any.
-__device__ __forceinline__ bool tt_clean(uint8_t* tile, int bytes, int tid) {
+// Values that are not finite become zeros in the keys r0 .. r1 of a staged tile (blocks of 64 columns, 128 bytes a key); true when there
+// were any.
+template <int KT>
+__device__ __forceinline__ bool tt_clean(uint8_t* tile, int blocks, int r0, int r1, int tid) {
     bool odd = false;
-#pragma unroll 8
-    for (int i = tid * 16; i < bytes; i += TT_COPY * 16) {
-        uint4* p = reinterpret_cast<uint4*>(tile + i);
-        const uint4 v = *p;
-        // an exponent of ones carries into the sign's place
-        auto carry = [](unsigned w) { return (w & 0x7f807f80u) + 0x00800080u; };
-        if (!((carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & 0x80008000u)) continue;
-        unsigned w[4] = {v.x, v.y, v.z, v.w};
+    for (int b = 0; b < blocks; b++)
+#pragma unroll 4
+        for (int i = r0 * 128 + tid * 16; i < r1 * 128; i += TT_COPY * 16) {
+            uint4* p = reinterpret_cast<uint4*>(tile + b * KT * 128 + i);
+            const uint4 v = *p;
+            // an exponent of ones carries into the sign's place
+            auto carry = [](unsigned w) { return (w & 0x7f807f80u) + 0x00800080u; };
+            if (!((carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & 0x80008000u)) continue;
+            unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u;
-            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu;
+            for (int j = 0; j < 4; j++) {
+                if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u;
+                if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu;
+            }
+            *p = make_uint4(w[0], w[1], w[2], w[3]);
+            odd = true;
         }
-        *p = make_uint4(w[0], w[1], w[2], w[3]);
-        odd = true;
-    }
     return odd;
 }
 
@@ -387,7 +390,9 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 ok = wait(&raw[sn], (looked >> sn) & 1u);
                 looked ^= 1u << sn;
                 if (!ok) break;
-                if (tt_clean(ring + (size_t)sn * sh.stage_bytes, sh.nvb * KT * 128, tid)) *reinterpret_cast<volatile int*>(&odd[item & 3]) = (int)item + 1;
+                const int k0 = (it.tile + t) * KT;
+                if (tt_clean<KT>(ring + (size_t)sn * sh.stage_bytes, sh.nvb, max(0, s.edge - k0), min(KT, s.len + s.n - k0), tid))
+                    *reinterpret_cast<volatile int*>(&odd[item & 3]) = (int)item + 1;
                 fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[sn]);
@@ -597,7 +602,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                         // values of attended nodes that are not finite (they entered the product as zeros)
                         const int k1 = min(s.len + s.n, (it.tile + it.n) * KT);
 #pragma unroll 1
-                        for (int k = max(it.tile, s.edge / KT) * KT; k < k1; k++) {
+                        for (int k = max(it.tile * KT, s.edge); k < k1; k++) {
                             unsigned sees[1];
                             tree_seen<1>(a, s, node, k, sees);
                             if (!(sees[0] & 1u)) continue;
