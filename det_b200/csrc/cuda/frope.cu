@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(256) k_frope_table(const RopeArgs a) {
         }
     pdl_wait();
     if (g >= groups) return;
-    for (int p = blockIdx.y * blockDim.y + threadIdx.y; p < a.n; p += gridDim.y * blockDim.y) {
-        const unsigned at = (unsigned)(a.pos0 + p);
+    for (unsigned p = blockIdx.y * blockDim.y + threadIdx.y; p < (unsigned)a.n; p += gridDim.y * blockDim.y) {      // n fits 31 bits, the sum 32
+        const unsigned at = (unsigned)a.pos0 + p;
         float c[V], s[V];
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -311,7 +311,7 @@ int det_f_rope_table(const det_frope_op* op, cudaStream_t st) {
     while (tx < groups && tx < 32) tx *= 2;
     const dim3 block(tx, 256 / tx);
     const int gx = (groups + tx - 1) / tx, want = std::max(1, 8 * sm_count() / gx);
-    const dim3 grid(gx, std::min(want, (a.n + (int)block.y - 1) / (int)block.y));
+    const dim3 grid(gx, std::min(want, (a.n - 1) / (int)block.y + 1));
     cudaStream_t q = queue_of(st);
     return launched(name, four ? launch_pdl_try(k_frope_table<4>, grid, block, 0, q, 1, a) : launch_pdl_try(k_frope_table<1>, grid, block, 0, q, 1, a));
 }

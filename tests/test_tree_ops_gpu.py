@@ -74,6 +74,23 @@ def test_rotation_tables(dims, n, pos0, scaling, gpu, libs):
         assert (got[n * cols:] == 9.0).all()
 
 
+def test_rotation_table_of_all_positions(gpu, libs):
+    """As many positions as 31 bits hold: the counters do not pass the end.  The bound is that of test_rotation_tables."""
+    n, guard = 2 ** 31 - 1, 4
+    cs, sn = gpu.space(4 * (n + guard)), gpu.space(4 * (n + guard))
+    for p in (cs, sn):
+        gpu.d.det_memcpy(p + 4 * n, np.full(guard, 9.0, np.float32).ctypes.data, 4 * guard, None)
+        gpu.d.det_sync()
+    op = libs.FRopeOp(dims=2, scaling=0, base=10007.0, factor=1.0, mscale=1.0, n=n, cos=cs, sin=sn)
+    assert gpu.d.det_f_rope_table(C.byref(op), None) == 0
+    for at in (0, 2 ** 30 - 3, n - 8):
+        a = at + np.arange(8, dtype=np.float64)
+        for p, want in ((cs, np.cos(a)), (sn, np.sin(a))):
+            assert (np.abs(gpu.get(p + 4 * at, 8).astype(float) - want) <= 4 * U32 + 8 * 2.0 ** -53 * a).all()
+    for p in (cs, sn):
+        assert (gpu.get(p + 4 * n, guard) == 9.0).all()
+
+
 # ------------------------------------------------------------------------------------------------------------------ norm and rotation
 class Step:
     """The rows of several sequences: `nodes` rows each behind `lens` cached ones, `extra` rows of the buffers that are nobody's."""
