@@ -465,7 +465,7 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     DETB_TAKE(blocks * op->seq.seqs <= 65535, "too many rows");
     DETB_TAKE(runtime_ready(), "no usable device");
     a.scale2 = op->scale * 1.4426950408889634f;
-    a.cap = op->cap; a.q = op->q; a.mask = op->mask; a.mask_ld = op->mask_ld; a.gate = op->gate; a.ldg = op->ldg; a.pos = op->pos;
+    a.cap = std::min(op->cap, TREE_MAX_KEYS); a.q = op->q; a.mask = op->mask; a.mask_ld = op->mask_ld; a.gate = op->gate; a.ldg = op->ldg; a.pos = op->pos;
     a.rope_len = op->rope_len; a.vcs = op->vrope_cos; a.vsn = op->vrope_sin; a.out = op->out; a.ldo = op->ldo;
     a.maps = op->scratch;
     a.part = reinterpret_cast<float*>(static_cast<char*>(op->scratch) + TREE_MAP_BYTES);

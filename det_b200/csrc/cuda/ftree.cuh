@@ -57,6 +57,7 @@ __device__ __forceinline__ TreePlace tree_place(const det_tree_ref& s, int row, 
 // beginning, so that such CTAs get fewer.
 constexpr int TREE_CTAS = 148;
 constexpr int TREE_SHARE = 2;      // tiles of a CTA at least, if there are enough
+constexpr int TREE_MAX_KEYS = 0x7fff0000;      // of a sequence: the end of its last tile fits 31 bits
 
 struct TreeArgs {
     int heads, kv_heads, per_kv, dim, vdim, kd, vd, ld, ldq;
@@ -190,7 +191,8 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
         const unsigned holds = __ballot_sync(FULL, base + sum > u0);
         if (holds) {
             const int src = __ffs(holds) - 1, per = __shfl_sync(FULL, places, src);
-            // places of the segment ahead of the share: below kv_heads * per, which fits 31 bits (per < 2^19, kv_heads <= 2^12)
+            // places of the segment ahead of the share: below kv_heads * per, two for 64 keys of a head, 32 bytes each at least; more than
+            // 32 bits of them would be a cache of 4 TB
             const unsigned in = (unsigned)(u0 - __shfl_sync(FULL, base + sum - (long long)places * a.kv_heads, src));
             w.seg = i - lane + src;
             w.g = (int)(in / (unsigned)per);

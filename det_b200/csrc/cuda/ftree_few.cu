@@ -251,15 +251,15 @@ static int few_ranks(long long clusters, int max_len) {
 //          of 65536; 32.3 / 43.7 for 16 sequences of 2048 keys and 5 rows, 98 / 49 with 40 rows
 //   there  15 for its start and its second launch, 5 for a turn, the larger of the bytes at 6 TB/s and 1.45 for a tile of 128 x 128
 bool ftree_few_takes(const TreeArgs& a, int rows) {
-    const int blocks = (rows + TF_ROWS - 1) / TF_ROWS, len = a.seq.max_len + a.seq.max_nodes;
-    const long long clusters = (long long)a.seq.seqs * a.kv_heads * blocks;
+    const int blocks = (rows + TF_ROWS - 1) / TF_ROWS;
+    const long long clusters = (long long)a.seq.seqs * a.kv_heads * blocks, len = (long long)a.seq.max_len + a.seq.max_nodes;
     if (blocks > 16 || (long long)a.kv_heads * blocks > 65535 || (float_flags() & 16)) return false;
     if (float_flags() & 32) return true;
     const int dv = a.vd <= 64 ? 64 : a.vd <= 128 ? 128 : 256;
-    const double row = 2.0 * (a.kd + a.vd), heads = (double)a.kv_heads * a.seq.seqs, bytes = row * heads * len;
+    const double row = 2.0 * (a.kd + a.vd), heads = (double)a.kv_heads * a.seq.seqs, bytes = row * heads * (double)len;
     const double slots = (few_smem(a.kd, dv) <= 113 * 1024 ? 2.0 : 1.0) * TREE_CTAS, ctas = (double)clusters * few_ranks(clusters, a.seq.max_len);
     const double here = 8.5e-6 * (double)((long long)(ctas / slots + 0.999)) + bytes * blocks / std::min(std::min(ctas, slots) * 24e9 * row / 512, 5.2e12);
-    const double tiles = heads * (len / 128 + 1) * ((rows + 127) / 128);
+    const double tiles = heads * (double)(len / 128 + 1) * ((rows + 127) / 128);
     const double there = 15e-6 + heads / TREE_CTAS * 5e-6 + std::max(bytes / 6e12, tiles / TREE_CTAS * 1.45e-6);
     return here <= there;
 }

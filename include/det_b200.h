@@ -669,7 +669,8 @@ void det_f_moe(const det_fmoe_op* op, cudaStream_t st);
  * its tree being row first[b] + i; its cache table[b].cache holds len[b] rows ahead of them, and node i belongs at cache row
  * len[b] + i.  table, first [seqs + 1] and len [seqs] are device arrays, so a captured step can be replayed with other lengths.
  * `rows` is the number of rows of the buffers: rows from first[seqs] on belong to nobody and are left as they were.  max_nodes
- * bounds a sequence's rows; max_len (>= 0) is the expected largest len: it sizes the launch, and results hold for any len.   */
+ * bounds a sequence's rows; max_len (>= 0) is the expected largest len: it sizes the launch, and results hold for any len (attention:
+ * up to 2^31 - 2^16 keys of a sequence).                                                                                     */
 typedef struct {
     const det_seq_slot* table;
     const int* first;

@@ -465,6 +465,26 @@ def test_sequences_that_do_not_fit_are_left_out(gpu, libs):
                 a.check(load(gpu, a.out, (a.s.rows, a.ldo), dtype), rows={1 - bad})
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_largest_bounds(dtype, gpu, libs):
+    """A caller that bounds nothing (cap and max_len the largest int): results as ever, and a length that no tile count fits is left out
+    without a look at its cache."""
+    rng = np.random.default_rng(17)
+    nodes, top = [8, 4], 2 ** 31 - 1
+    a = Attn(gpu, libs, dtype, 4, 2, 64, 64, [50, 20], nodes, masks=random_masks(nodes, rng))
+    op = a.op()
+    op.cap, op.seq.max_len = top, top
+    for lens, rows in [([50, 20], None), ([top - 100, 20], {1}), ([top - 8, 20], {1})]:
+        op.seq.len = ints(gpu, lens)
+        for flags in (0, 16, 32):
+            op.out = a.out = store(gpu, np.full((a.s.rows, a.ldo), 7.0), dtype)[0]
+            gpu.d.det_debug_set_float(flags)
+            assert gpu.d.det_f_tree_attn(C.byref(op), None) == 0
+            gpu.d.det_debug_set_float(0)
+            assert size_error(gpu) == (0 if rows is None else SIZE_ERROR)
+            a.check(load(gpu, a.out, (a.s.rows, a.ldo), dtype), rows=rows)
+
+
 def test_a_run_equals_the_attention_op_of_the_models(gpu, libs):
     """The same projections through det_f_attn and through det_f_qk_rope + det_f_tree_attn, over the same kind of cache."""
     H, G, d, v, n = 6, 2, 64, 64, 150
