@@ -376,7 +376,7 @@ template <int TR, int VJ>
 static cudaError_t launch_simt(const TreeArgs& a, cudaStream_t q) {
     const int stages = simt_smem(a.block, a.kd, a.vd, 2) <= 220 * 1024 ? 2 : 1;
     const size_t smem = simt_smem(a.block, a.kd, a.vd, stages);
-    const cudaError_t e = cudaFuncSetAttribute(k_ftree_simt<TR, VJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = most_smem(k_ftree_simt<TR, VJ>);
     if (e != cudaSuccess) return e;
     return launch_pdl_try(k_ftree_simt<TR, VJ>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a, stages);
 }

@@ -305,6 +305,12 @@ __device__ __forceinline__ void add4(float4& o, float f, float4 x) {
     o.w = fmaf(f, x.w, o.w);
 }
 
+// Lets the kernel have the dynamic shared memory of its largest call.  Every call sets the same limit, since calls of other sizes may run
+// on other threads; 1 KB is left for what the kernels declare themselves.
+constexpr int TREE_SMEM = 226 * 1024;
+template <class F>
+inline cudaError_t most_smem(F* kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TREE_SMEM); }
+
 // ftree_few.cu: bfloat16 activations, few rows.
 bool ftree_few_takes(const TreeArgs& a, int rows);
 void ftree_few_shape(int* block, int* tile);

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(TF_WARPS * 32) k_ftree_few(const TreeArgs a) {
 template <int DV>
 static cudaError_t launch(const TreeArgs& a, int ranks, cudaStream_t q) {
     const size_t smem = few_smem(a.kd, DV);
-    cudaError_t e = cudaFuncSetAttribute(k_ftree_few<DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = most_smem(k_ftree_few<DV>);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_ftree_few<DV>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     return launch_pdl_try(k_ftree_few<DV>, dim3(ranks, a.kv_heads * a.blocks, a.seq.seqs), dim3(TF_WARPS * 32), smem, q, ranks, a);

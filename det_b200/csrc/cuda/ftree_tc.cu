@@ -52,7 +52,6 @@ struct alignas(128) TtTables {
     unsigned tmem_slot;
     int odd[4];                                      // number (+ 1) of the stretch whose values were not all finite
 };
-constexpr size_t TT_SMEM = 227 * 1024;
 
 __device__ __forceinline__ void umma_f16_ss(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned acc) {
     asm volatile(
@@ -674,9 +673,9 @@ static cudaError_t launch(const TreeArgs& a, cudaStream_t q) {
     sh.stage_bytes = std::max(sh.nkb, sh.nvb) * KT * 128;
     sh.twice = SLOTS == 2 && a.block == TT_ROWS;
     const size_t fixed = (size_t)SLOTS * sh.q_bytes + sizeof(TtTables);
-    sh.stages = (int)std::min<size_t>(TT_STAGES, (TT_SMEM - fixed) / sh.stage_bytes);
+    sh.stages = (int)std::min<size_t>(TT_STAGES, (TREE_SMEM - fixed) / sh.stage_bytes);
     const size_t smem = fixed + (size_t)sh.stages * sh.stage_bytes;
-    const cudaError_t e = cudaFuncSetAttribute(k_ftree_tc<SLOTS, KT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = most_smem(k_ftree_tc<SLOTS, KT>);
     if (e != cudaSuccess) return e;
     CUtensorMap keys, values;
     if (!cache_map(&keys, a, a.kd, KT) || !cache_map(&values, a, a.vd, KT)) return cudaErrorInvalidValue;

@@ -1,6 +1,7 @@
 """The ops of a step of drafted tokens through the C ABI against the plain functions of tree_oracle.py in float64: types, layouts, head
 sizes, lengths from nothing to thousands of keys, masks that leave rows empty, rows that belong to nobody, lists that do not fit."""
 import ctypes as C
+import threading
 
 import numpy as np
 import pytest
@@ -629,6 +630,33 @@ def test_calls_on_two_streams_and_replays_of_two_graphs(gpu, libs):
             a.check(load(gpu, a.out, (a.s.rows, a.ldo), "bf16"))
     for g in graphs:
         gpu.d.det_graph_free(g)
+
+
+def test_calls_from_two_threads(gpu, libs):
+    """Two host threads queue calls of the same kernels with other sizes (other shared memory) at once: none is refused, all are right."""
+    rng = np.random.default_rng(31)
+    rt = C.CDLL("libcudart.so.12")
+    for dtype in ("f32", "bf16"):
+        cases = [Attn(gpu, libs, dtype, *heads, [70, 300], [9, 3], masks=random_masks([9, 3], rng)) for heads in [(4, 2, 16, 128), (4, 2, 128, 128)]]
+        streams, ops = [C.c_void_p() for _ in cases], [a.op() for a in cases]
+        for s in streams:
+            assert rt.cudaStreamCreateWithFlags(C.byref(s), 1) == 0
+        for flags in (16, 32):
+            gpu.d.det_debug_set_float(flags)
+            gpu.d.det_sync()
+            codes = [[], []]
+            threads = [threading.Thread(target=lambda i=i: codes[i].extend(gpu.d.det_f_tree_attn(C.byref(ops[i]), streams[i]) for _ in range(300))) for i in (0, 1)]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+            gpu.d.det_debug_set_float(0)
+            assert rt.cudaDeviceSynchronize() == 0
+            assert codes == [[0] * 300] * 2
+            for a in cases:
+                a.check(load(gpu, a.out, (a.s.rows, a.ldo), dtype))
+        for s in streams:
+            assert rt.cudaStreamDestroy(s) == 0
 
 
 # ------------------------------------------------------------------------------------------------------------------ kept rows
