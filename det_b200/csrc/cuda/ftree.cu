@@ -61,7 +61,9 @@ __device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t l
 }
 
 // Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.  With two stages the next tile's copies run
-// beside the products of this one.  Bound by the fp32 multiply-adds (a key costs all rows of the block, 16 TR, whatever is in them).
+// beside the products of this one.  Bound by the fp32 multiply-adds where keys are many (a key costs all rows of the block, 16 TR, whatever
+// is in them), by start, deal and second launch where they are few (6 / 2 heads of 40 and 24, five trees of 13 nodes behind up to 2000
+// keys: 23 us; the multiply-adds would take 2).
 template <int TR, int VJ>
 __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int stages) {
     extern __shared__ __align__(16) float tsm[];

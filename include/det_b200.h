@@ -663,7 +663,8 @@ void det_f_moe(const det_fmoe_op* op, cudaStream_t st);
  * The entry points below return 0 when the work was queued and 1 when the call was refused (bad sizes, a NULL pointer, a misaligned
  * buffer, no usable device): a refusal prints its reason, launches nothing and leaves every buffer as it was; they never abort.
  * What only device memory knows (first, len, pos, keep, count) is checked by the kernels: a sequence whose entries do not fit its
- * cache, the bounds of the call or the tables is left out, its outputs stay as they were, and det_last_error() returns 2.
+ * cache or the bounds of the call, and a row whose position the tables do not hold, is left out: its outputs stay as they were, and
+ * det_last_error() returns 2.  A call's outputs must not overlap its inputs.
  *
  * The rows of a step.  Sequence b owns the rows first[b] .. first[b + 1] - 1 (first[0] = 0, ascending; none is allowed), node i of
  * its tree being row first[b] + i; its cache table[b].cache holds len[b] rows ahead of them, and node i belongs at cache row
@@ -681,8 +682,9 @@ typedef struct {
     int max_len;
 } det_tree_ref;
 
-/* Tables of the position rotation: cos[p][i] = mscale * cos((pos0 + p) * f_i), sin likewise, p < n, i < dims / 2 (fp32, computed
- * in binary64 up to the last rounding).  f_i = base^(-2i / dims), scaled for contexts longer than the model was made for:
+/* Tables of the position rotation: cos[p][i] = mscale * cos((pos0 + p) * f_i), sin likewise, p < n, i < dims / 2 (fp32).
+ * f_i in binary64; the angle is kept as 64-bit turns, so far positions lose no more than binary64 does (2^-53 of the angle), and the
+ * result is within 4 units of 2^-24 * mscale of it.  f_i = base^(-2i / dims), scaled for contexts longer than the model was made for:
  *   DET_ROPE_LINEAR  f_i / factor
  *   DET_ROPE_BASE    base * factor^(dims / (dims - 2)) instead of base (dims > 2)
  *   DET_ROPE_RAMP    f_i * (w + (1 - w) / factor), w = (orig_ctx * f_i / 2 pi - low) / (high - low) clamped to 0 .. 1: columns
@@ -736,10 +738,10 @@ typedef struct {
 } det_fqk_op;
 int det_f_qk_rope(const det_fqk_op* op, cudaStream_t st);
 
-/* Attention of a step's rows over their sequences' caches (rows as det_f_qk_rope or det_f_attn_prep leave them).  Row i of sequence
- * b attends the cached rows j < len[b] and, of its own tree, the nodes j whose bit j % 32 of word mask[row * mask_ld + j / 32] is
- * set (its ancestors and itself, as a rule); mask NULL: the nodes j <= i, that is, the rows are a run of tokens.  Query head h reads
- * key/value head h / (heads / kv_heads); out[row][h * vdim + j] = sum softmax(scale * q . k) v, times sigmoid(gate[row * ldg + h])
+/* Attention of a step's rows over their sequences' caches (rows as det_f_qk_rope or det_f_attn_prep leave them; q as det_f_qk_rope
+ * leaves it: that of det_f_attn_prep carries its scale already).  Row i of sequence b attends the cached rows j < len[b] and, of its
+ * own tree, the nodes j whose bit j % 32 of word mask[row * mask_ld + j / 32] is set (its ancestors and itself, as a rule); mask
+ * NULL: the nodes j <= i, that is, the rows are a run of tokens.  Query head h reads key/value head h / (heads / kv_heads); out[row][h * vdim + j] = sum softmax(scale * q . k) v, times sigmoid(gate[row * ldg + h])
  * (gate NULL: 1), in the activation type, row stride ldo.  A row that attends nothing gets zeros; what masked and missing rows hold,
  * NaN included, has no influence.  vrope_cos / vrope_sin: the values are rotated, and a head's output is turned back by pos[row]
  * (then needed; rope_len rows in the tables).  scale > 0.  dim, vdim <= 256; with a mask max_nodes <= DET_MAX_TREE.
