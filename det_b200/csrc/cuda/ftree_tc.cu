@@ -134,6 +134,12 @@ __device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// One lane of the warp, which the compiler then knows to be alone: operands of tcgen05.mma and TMA stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    unsigned x;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+    return x != 0;
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // The tensor maps of a sequence's keys and values, made from the launch's by the whole warp: their addresses and number of rows are set
@@ -408,7 +414,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
         }
     } else if (warp == PRODUCTS) {
         // ---- products
-        if (lane == 0) {
+        if (elect_one()) {
             const unsigned id_s = tt_idesc(KT, false), vn = (unsigned)(a.vd + 15) / 16 * 16, id_o = tt_idesc((int)vn, true);
             const int ksteps = (a.kd + 15) / 16;
             const unsigned long long q_desc = umma_desc(Qs), k_desc = umma_desc(ring), v_desc = umma_desc_mn(ring, KT * 128);
@@ -492,6 +498,7 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                 item++;
             }
         }
+        ok = __all_sync(FULL, ok) != 0;
     } else {
         // ---- softmax
         const int slot = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
