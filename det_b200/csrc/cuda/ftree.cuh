@@ -274,8 +274,8 @@ struct TreeOut {
         }
         if (a.gate) w = sigmoid_fast(a.gate[(size_t)row * a.ldg + h]);
     }
-    __device__ __forceinline__ void put4at(int v, float4 x) const {
-        if (skip) return;
+    // ... turned back and gated
+    __device__ __forceinline__ float4 finished(int v, float4 x) const {
         float o[4] = {x.x * w, x.y * w, x.z * w, x.w * w};
         if (c) {
 #pragma unroll
@@ -286,9 +286,15 @@ struct TreeOut {
                     o[j + 1] = fmaf(o[j + 1], cj, -(u * sj));
                 }
         }
+        return make_float4(o[0], o[1], o[2], o[3]);
+    }
+    __device__ __forceinline__ void put4at(int v, float4 x) const {
+        if (skip) return;
+        x = finished(v, x);
+        const float o[4] = {x.x, x.y, x.z, x.w};
         T* to = out + v;
         if (v + 4 <= vdim && (reinterpret_cast<uintptr_t>(to) & (4 * sizeof(T) - 1)) == 0) {
-            put4(to, make_float4(o[0], o[1], o[2], o[3]));
+            put4(to, x);
             return;
         }
 #pragma unroll

@@ -268,6 +268,25 @@ __device__ __forceinline__ float tt_weights(unsigned ts, const unsigned (&words)
     return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
 
+// Eight lanes exchange: lane l had piece k of its row in x[k], afterwards it has piece l of row k (N words each).
+template <int N>
+__device__ __forceinline__ void tt_turn(unsigned (&x)[8][N], int lane) {
+#pragma unroll
+    for (int s = 1; s < 8; s *= 2) {
+        const bool up = lane & s;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (k & s) continue;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const unsigned y = __shfl_xor_sync(FULL, up ? x[k][i] : x[k + s][i], s);
+                if (up) x[k][i] = y;
+                else x[k + s][i] = y;
+            }
+        }
+    }
+}
+
 template <int SLOTS, int KT>
 __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                                const TreeArgs a, const TtShape sh) {
@@ -627,17 +646,41 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
                             }
                         }
                     }
-                    if (mine) {
-                        if (it.whole) {
+                    // eight lanes store a row's 32 values side by side, row after row (a lane per row would touch 32 lines at a time)
+                    const int group = lane & 24, col = q + (lane & 7) * 4;
+                    if (it.whole) {
+                        unsigned x[8][2];
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                if (q + i < a.vd) out.put4at(q + i, make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
-                        } else {
-                            float* to4 = piece + 2 * a.block + (size_t)br * a.vd + q;
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                if (q + i < a.vd) put4(to4 + i, make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+                        for (int i = 0; i < 8; i++) {
+                            const float4 y = out.finished(q + i * 4, make_float4(o[i * 4] * inv, o[i * 4 + 1] * inv, o[i * 4 + 2] * inv, o[i * 4 + 3] * inv));
+                            x[i][0] = pack_bf(y.x, y.y);
+                            x[i][1] = pack_bf(y.z, y.w);
                         }
+                        tt_turn<2>(x, lane);
+                        const unsigned long long own = mine && !out.skip ? reinterpret_cast<unsigned long long>(out.out) : 0;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            bf16* to = reinterpret_cast<bf16*>(__shfl_sync(FULL, own, group + k));
+                            if (!to || col >= a.vdim) continue;
+                            to += col;
+                            if (col + 4 <= a.vdim && (reinterpret_cast<uintptr_t>(to) & 7) == 0) {
+                                *reinterpret_cast<uint2*>(to) = make_uint2(x[k][0], x[k][1]);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; j++)
+                                    if (col + j < a.vdim) reinterpret_cast<unsigned short*>(to)[j] = (unsigned short)(x[k][j >> 1] >> (j & 1) * 16);
+                            }
+                        }
+                    } else {
+                        unsigned x[8][4];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i >> 2][i & 3] = __float_as_uint(o[i]);
+                        tt_turn<4>(x, lane);
+                        const int first = br - (lane & 7);
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            if (first + k < s.rows && col < a.vd)
+                                *reinterpret_cast<uint4*>(piece + 2 * a.block + (size_t)(first + k) * a.vd + col) = make_uint4(x[k][0], x[k][1], x[k][2], x[k][3]);
                     }
                     __syncwarp();
                 }
