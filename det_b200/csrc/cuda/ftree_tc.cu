@@ -395,6 +395,8 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
         // ---- query rows, and values that not every row sees
         const int tid = threadIdx.x - ROWS * 32;
         const int kp = (a.kd + 15) / 16 * 2, lanes = kp <= 8 ? 8 : kp <= 16 ? 16 : 32, qc = lane % lanes, qstep = TT_COPY / lanes;
+        const int head_step = qstep % a.per_kv;      // from a thread's row to its next one: heads, and elements without and with one more node
+        const ptrdiff_t ahead = (ptrdiff_t)(qstep / a.per_kv) * a.ldq + head_step * a.kd, wrap = (ptrdiff_t)a.ldq - a.per_kv * a.kd;
         unsigned c = 0, looked = 0;                  // tiles of the stretches before; phases of `raw`, a bit per stage
         while (ok && tree_next(a, walk, it)) {
             const TreeSeg& s = it.s;
@@ -403,14 +405,24 @@ __global__ void __launch_bounds__(TtCfg<SLOTS, KT>::THREADS, 1) k_ftree_tc(const
             if (!ok) break;
             // a row per `lanes` lanes; rows that are not there keep what is there (a row's scores are its own)
             const bf16* q = static_cast<const bf16*>(a.q) + (size_t)s.first * a.ldq + (size_t)it.g * a.per_kv * a.kd;
-            if (qc < kp)
+            if (qc < kp) {
+                const int row = s.r0 + tid / lanes, node = (int)(row * a.per_magic >> 32);
+                int head = row - node * a.per_kv;
+                const bf16* src = q + (size_t)node * a.ldq + head * a.kd + (qc * 8 < a.kd ? qc * 8 : 0);
+                const int bytes = qc * 8 < a.kd ? 16 : 0;
+                const unsigned dst = smem_addr(Qs) + (unsigned)((twice ? qb * sh.q_bytes : 0) + (qc >> 3) * TT_ROWS * 128);
 #pragma unroll 4
                 for (int r = tid / lanes; r < s.rows; r += qstep) {
-                    const int row = s.r0 + r, node = (int)(row * a.per_magic >> 32), x = r & (TT_ROWS - 1);
-                    const bf16* src = q + (size_t)node * a.ldq + (row - node * a.per_kv) * a.kd;
-                    copy16(smem_addr(Qs + (size_t)(twice ? qb : r / TT_ROWS) * sh.q_bytes) + (unsigned)((qc >> 3) * TT_ROWS * 128 + x * 128 + (((qc ^ x) & 7) << 4)),
-                           qc * 8 < a.kd ? src + qc * 8 : src, qc * 8 < a.kd ? 16 : 0);
+                    const unsigned half = r >= TT_ROWS ? (unsigned)(sh.q_bytes - TT_ROWS * 128) : 0u;       // the second slot's rows
+                    copy16(dst + half + (unsigned)(r * 128 + (((qc ^ r) & 7) << 4)), src, bytes);
+                    src += ahead;
+                    head += head_step;
+                    if (head >= a.per_kv) {
+                        head -= a.per_kv;
+                        src += wrap;
+                    }
                 }
+            }
             copies_wait_all();
             fence_async();
             __syncwarp();
