@@ -3,7 +3,7 @@
 //
 //   k_ftree_few    bfloat16, few rows or short caches: ftree_few.cu.
 //   k_ftree_tc     bfloat16: ftree_tc.cu.
-//   k_ftree_simt   fp32: products on the CUDA cores, 256 threads over a tile of query rows x 64 keys.
+//   k_ftree_simt   fp32: products on the CUDA cores, 256 threads over a tile of query rows x 32 keys.
 //   k_ftree_merge  adds the pieces of the segments that several CTAs shared.
 #include "ftree.cuh"
 #include <algorithm>
@@ -11,7 +11,7 @@
 
 namespace detb {
 
-constexpr int TS_KEYS = 64, TS_THREADS = 256;
+constexpr int TS_KEYS = 32, TS_NJ = TS_KEYS / 16, TS_THREADS = 256;
 
 static size_t simt_smem(int block, int kd, int vd, int stages) {
     return ((size_t)block * (kd + 4) + (size_t)stages * TS_KEYS * (kd + vd + 8) + (size_t)block * (TS_KEYS + 4)) * sizeof(float);
@@ -34,7 +34,7 @@ __device__ __forceinline__ float row_sum(float v) {
 __device__ __forceinline__ void copy16(float* dst, const float* src, int bytes) {      // what is missing of 16 bytes becomes zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
 }
-// The 64 rows of a tile, n floats (a multiple of 4) each, `ld` apart, into rows of n + 4; rows past `have` become zeros.  LANES threads take
+// The 32 rows of a tile, n floats (a multiple of 4) each, `ld` apart, into rows of n + 4; rows past `have` become zeros.  LANES threads take
 // the 16-byte pieces of a row, so an address is one addition.
 template <int LANES>
 __device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t ld, int n, int have) {
@@ -65,7 +65,7 @@ __device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t l
 // is in them), by start, deal and second launch where they are few (6 / 2 heads of 40 and 24, five trees of 13 nodes behind up to 2000
 // keys: 23 us; the multiply-adds would take 2).
 template <int TR, int VJ>
-__global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int stages) {
+__global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const TreeArgs a, int stages) {
     extern __shared__ __align__(16) float tsm[];
     __shared__ TreeShare share;
     __shared__ int odd;                          // a staged value that not every row sees was not finite
@@ -73,8 +73,10 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int
     const int ldk = a.kd + 4, ldv = a.vd + 4, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     float* Q = tsm;                              // [RB][ldk]
     float* P = Q + RB * ldk;                     // [RB][LDP]
-    float* KV = P + RB * LDP;                    // [stage] K [64][ldk] | V [64][ldv]
+    float* KV = P + RB * LDP;                    // [stage] K [32][ldk] | V [32][ldv]
     const int stage_floats = TS_KEYS * (ldk + ldv);
+    // lanes that a row's values need; with fewer than 16 the others take other keys (a run of 4 after the other goes round)
+    const int lv = VJ > 1 || a.vd > 32 ? 16 : a.vd > 16 ? 8 : 4, vx = tx & (lv - 1), kstep = 64 / lv;
     pdl_wait();
     pdl_trigger();                               // behind the wait: what k_ftree_merge reads ahead of its own is then there
     if (tid < 32) {
@@ -133,34 +135,36 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int
                     if (!isfinite(*p)) *p = 0.0f, odd = 1;
                 }
             }
-            float sc[TR][4];
+            float sc[TR][TS_NJ];
 #pragma unroll
             for (int i = 0; i < TR; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) sc[i][j] = 0.0f;
+                for (int j = 0; j < TS_NJ; j++) sc[i][j] = 0.0f;
 #pragma unroll 2
             for (int e = 0; e < a.kd; e += 4) {
-                float4 kv[4];
+                float4 kv[TS_NJ];
 #pragma unroll
-                for (int j = 0; j < 4; j++) kv[j] = load4(K + (tx + 16 * j) * ldk + e);
+                for (int j = 0; j < TS_NJ; j++) kv[j] = load4(K + (tx + 16 * j) * ldk + e);
 #pragma unroll
                 for (int i = 0; i < TR; i++) {
                     const float4 qv = load4(Q + (ty + 16 * i) * ldk + e);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) sc[i][j] = dot4(qv, kv[j], sc[i][j]);
+                    for (int j = 0; j < TS_NJ; j++) sc[i][j] = dot4(qv, kv[j], sc[i][j]);
                 }
             }
 #pragma unroll
             for (int i = 0; i < TR; i++) {
                 const int r = ty + 16 * i;
-                unsigned seen[2] = {FULL, FULL};
+                unsigned seen[TS_KEYS / 32];
+#pragma unroll
+                for (int j = 0; j < TS_KEYS / 32; j++) seen[j] = FULL;
                 if (tree) {
                     const int row = s.r0 + min(r, s.rows - 1);
-                    tree_seen<2>(a, s, (int)(row * a.per_magic >> 32), k0, seen);
+                    tree_seen<TS_KEYS / 32>(a, s, (int)(row * a.per_magic >> 32), k0, seen);
                 }
                 float mx = m[i];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < TS_NJ; j++) {
                     sc[i][j] = (seen[j >> 1] >> (tx + 16 * (j & 1))) & 1u ? sc[i][j] * a.scale2 : -INFINITY;
                     mx = fmaxf(mx, sc[i][j]);
                 }
@@ -171,20 +175,20 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int
 #pragma unroll
                 for (int j = 0; j < VJ; j++) o[i][j] = scaled4(o[i][j], f);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < TS_NJ; j++) {
                     const float p = exp2f(sc[i][j] - base);
                     l[i] += p;
                     P[r * LDP + tx + 16 * j] = p;
                 }
             }
             __syncthreads();
-            for (int k = 0; k < TS_KEYS; k += 4) {
+            for (int k = tx / lv * 4; k < TS_KEYS; k += kstep) {
                 float4 p[TR];
 #pragma unroll
                 for (int i = 0; i < TR; i++) p[i] = load4(P + (ty + 16 * i) * LDP + k);
 #pragma unroll
                 for (int j = 0; j < VJ; j++) {
-                    const int c = 4 * tx + 64 * j;
+                    const int c = 4 * vx + 64 * j;
                     if (c >= a.vd) continue;
                     const float4 v0 = load4(V + k * ldv + c), v1 = load4(V + (k + 1) * ldv + c), v2 = load4(V + (k + 2) * ldv + c),
                                  v3 = load4(V + (k + 3) * ldv + c);
@@ -211,7 +215,13 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int
         for (int i = 0; i < TR; i++) {
             const int r = ty + 16 * i, row = s.r0 + min(r, s.rows - 1), node = (int)(row * a.per_magic >> 32);
             const float sum = row_sum(l[i]);
-            if (r >= s.rows) continue;
+            for (int off = 8; off >= lv; off >>= 1) {
+                o[i][0].x += __shfl_xor_sync(FULL, o[i][0].x, off);
+                o[i][0].y += __shfl_xor_sync(FULL, o[i][0].y, off);
+                o[i][0].z += __shfl_xor_sync(FULL, o[i][0].z, off);
+                o[i][0].w += __shfl_xor_sync(FULL, o[i][0].w, off);
+            }
+            if (r >= s.rows || tx >= lv) continue;
             if (fix)                             // values of attended keys that are not finite (they entered the product as zeros)
                 for (int k = max(it.tile, s.edge / TS_KEYS) * TS_KEYS; k < min(s.len + s.n, (it.tile + it.n) * TS_KEYS); k++) {
                     unsigned sees[1];
@@ -243,7 +253,7 @@ __global__ void __launch_bounds__(TS_THREADS) k_ftree_simt(const TreeArgs a, int
 }
 
 // ------------------------------------------------------------------------------------------------------ pieces
-constexpr int TM_WARPS = 8, TM_ML = (TREE_CTAS + 31) / 32;
+constexpr int TM_WARPS = 8, TM_ML = (2 * TREE_CTAS + 31) / 32;
 // grid (X, groups of `per` rows).  With few segments X counts them; else block x looks at the border between the shares of CTAs x and
 // x + 1, and when it is the first border inside a segment, the block adds that segment's pieces.  WIDE: the warps of a block share the
 // pieces of one row after the other (few rows); else a warp has rows of its own.  HI: values above 128.  Bound by the latency of the
@@ -408,6 +418,8 @@ static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
     return wide ? launch_pdl_try(k_ftree_merge<T, true, true>, grid, block, 0, q, 1, a, per, by_segment)
                 : launch_pdl_try(k_ftree_merge<T, false, true>, grid, block, 0, q, 1, a, per, by_segment);
 }
+// CTAs of an SM: two where registers and shared memory allow it.
+static int simt_ctas(const TreeArgs& a) { return a.vd <= 128 && simt_smem(a.block, a.kd, a.vd, 2) <= 112 * 1024 ? 2 : 1; }
 // Rows of a block, keys of a tile, tiles that a turn costs.  A tile takes about as long for its copies, waits and softmax as for the
 // products of 48 rows.
 static void simt_shape(int rows, int* block, int* tile, int* turn) {
@@ -473,7 +485,7 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     a.part = reinterpret_cast<float*>(static_cast<char*>(op->scratch) + TREE_MAP_BYTES);
     a.error_flag = error_word();
     a.blocks = (int)blocks;
-    a.ctas = std::min(TREE_CTAS, sm_count());
+    a.ctas = std::min(TREE_CTAS, sm_count()) * (op->dtype == DET_F32 ? simt_ctas(a) : 1);
     cudaStream_t q = queue_of(st);
     if (few) return launched(name, ftree_few_launch(a, q));
     if (op->dtype == DET_BF16) {
