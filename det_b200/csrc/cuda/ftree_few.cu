@@ -249,10 +249,11 @@ static int few_ranks(long long clusters, int max_len) {
     return ranks;
 }
 // This kernel or k_ftree_tc, by what both were measured to take (in us, 8 key/value heads of 128, this one / the other):
-//   here   8.5 for every round of CTAs, and the cache's bytes once per 16 rows at 24 GB/s a CTA (keys and values of 128 in its ring), 5.2 TB/s
-//          together: 11.0 / 16.3 at 5 rows of 512 keys, 14.3 / 19.9 at 40 rows of 2048, 30.4 / 25.0 at 40 rows of 8192, 88 / 68 at 5 rows
-//          of 65536; 32.3 / 43.7 for 16 sequences of 2048 keys and 5 rows, 98 / 49 with 40 rows
-//   there  15 for its start and its second launch, 5 for a turn, the larger of the bytes at 6 TB/s and 1.45 for a tile of 128 x 128
+//   here   8.5 for every round of CTAs, and the cache's bytes once per 16 rows at 24 GB/s a CTA (keys and values of 128 in its ring; 32 for
+//          larger ones, 33 / 23 at 64 rows of 4096 keys of 256), 6 TB/s together: 11.3 / 16.9 at 5 rows of 512 keys, 14.3 / 20.1 at 40
+//          rows of 2048, 30.4 / 24.1 at 40 rows of 8192, 48 / 41 at 5 rows of 32768; 95 / 109 for 4 sequences of those; 32 / 41 for 16
+//          sequences of 2048 keys and 5 rows, 98 / 45 with 40 rows
+//   there  15 for its start and its second launch, 5 for a turn, the larger of the bytes at 5.8 TB/s and 1.45 for a tile of 128 x 128
 bool ftree_few_takes(const TreeArgs& a, int rows) {
     const int blocks = (rows + TF_ROWS - 1) / TF_ROWS;
     const long long clusters = (long long)a.seq.seqs * a.kv_heads * blocks, len = (long long)a.seq.max_len + a.seq.max_nodes;
@@ -261,9 +262,9 @@ bool ftree_few_takes(const TreeArgs& a, int rows) {
     const int dv = a.vd <= 64 ? 64 : a.vd <= 128 ? 128 : 256;
     const double row = 2.0 * (a.kd + a.vd), heads = (double)a.kv_heads * a.seq.seqs, bytes = row * heads * (double)len;
     const double slots = (few_smem(a.kd, dv) <= 113 * 1024 ? 2.0 : 1.0) * TREE_CTAS, ctas = (double)clusters * few_ranks(clusters, a.seq.max_len);
-    const double here = 8.5e-6 * (double)((long long)(ctas / slots + 0.999)) + bytes * blocks / std::min(std::min(ctas, slots) * 24e9 * row / 512, 5.2e12);
+    const double here = 8.5e-6 * (double)((long long)(ctas / slots + 0.999)) + bytes * blocks / std::min(std::min(ctas, slots) * std::min(24e9 * row / 512, 32e9), 6e12);
     const double tiles = heads * (double)(len / 128 + 1) * ((rows + 127) / 128);
-    const double there = 15e-6 + heads / TREE_CTAS * 5e-6 + std::max(bytes / 6e12, tiles / TREE_CTAS * 1.45e-6);
+    const double there = 15e-6 + heads / TREE_CTAS * 5e-6 + std::max(bytes / 5.8e12, tiles / TREE_CTAS * 1.45e-6);
     return here <= there;
 }
 void ftree_few_shape(int* block, int* tile) {
