@@ -61,9 +61,10 @@ __device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t l
 }
 
 // Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.  With two stages the next tile's copies run
-// beside the products of this one.  Bound by the fp32 multiply-adds where keys are many (a key costs all rows of the block, 16 TR, whatever
-// is in them), by start, deal and second launch where they are few (6 / 2 heads of 40 and 24, five trees of 13 nodes behind up to 2000
-// keys: 23 us; the multiply-adds would take 2).
+// beside the products of this one; two CTAs on an SM cover one another's latencies.  Bound by the fp32 multiply-adds and their operands
+// from shared memory where keys are many (a key costs all rows of the block, 16 TR, whatever is in them: 16 nodes of 4 sequences behind 4096
+// keys, 40 / 8 heads of 128, 272 us), by start, deal and second launch where they are few (6 / 2 heads of 40 and 24, five trees of 13
+// nodes behind 2000 keys: 23.8 us; 27.7 with tiles of 64 keys and one CTA on an SM).
 template <int TR, int VJ>
 __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const TreeArgs a, int stages) {
     extern __shared__ __align__(16) float tsm[];
