@@ -444,7 +444,7 @@ size_t det_f_tree_scratch_bytes(int heads, int kv_heads, int vdim, int max_nodes
     int block = 0, other = 0, tile = 0, turn = 0;
     simt_shape(rows, &block, &tile, &turn);
     ftree_tc_shape(rows, 8, vd, &other, &tile, &turn);      // the smallest keys have the largest blocks
-    block = std::max(block, other);
+    block = std::max(2 * block, other);                     // fp32: two CTAs an SM
     return TREE_MAP_BYTES + TREE_CTAS * 2 * tree_piece_floats(block, vd) * sizeof(float);
 }
 

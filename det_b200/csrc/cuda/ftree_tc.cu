@@ -23,8 +23,8 @@
 //
 // What bounds it (40 / 8 heads of 128).  Trees of 16 nodes read the cache once: 16 nodes behind 65536 keys 63 us (269 MB from HBM, what
 // they cannot do without), 32 sequences of 16 behind 4096 keys 104 us (5.2 TB/s).  A prompt of 2048 behind 6144 takes 306 us, 980
-// TFLOP/s: a tile of 128 rows x 128 keys is 1040 cycles of products (half as many again with the tiles' copies into the same shared
-// memory), then comes the chain from scores over a warp's exponentials (about 1600 cycles) to the weights, which two slots hide in part:
+// TFLOP/s: a tile of 128 rows x 128 keys is 1040 cycles of products (measured alone), beside the tiles' copies into the same shared
+// memory; then comes the chain from scores over a warp's exponentials (about 1600 cycles) to the weights, which two slots hide in part:
 // the pipe is busy 41 % of the time.  The products are issued by an elected lane: by a branch on the lane's number, operands went through
 // vector registers and the issue was the bound (358 us).  Measured and not taken: copies of the tiles by warps in place of TMA (prompt 532
 // us against 401), tiles of 64 keys with two score buffers (515 against 354), a product warp for each slot (405 against 354), TMEM loads

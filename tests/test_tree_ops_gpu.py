@@ -427,6 +427,21 @@ def test_long_unequal_contexts_are_shared_out(dtype, gpu, libs):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads", [(8, 2, 64, 64), (4, 1, 128, 128), (2, 1, 200, 256), (5, 5, 40, 24)], ids=str)
+def test_pieces_stay_in_the_scratch(heads, dtype, gpu, libs):
+    """Every CTA leaves pieces; what lies behind det_f_tree_scratch_bytes stays as it was."""
+    rng = np.random.default_rng(sum(heads))
+    for lens, nodes in [([7000], [16]), ([2500, 900, 3100], [64, 70, 12]), ([3000], [300])]:
+        masks = random_masks(nodes, rng) if nodes[0] < 100 else None
+        a = Attn(gpu, libs, dtype, *heads, lens, nodes, masks=masks)
+        n, guard = gpu.d.det_f_tree_scratch_bytes(heads[0], heads[1], heads[3], max(nodes)), 4096
+        a.scratch = gpu.space(n + guard)
+        gpu.d.det_memset(a.scratch + n, 0x5a, guard, None)
+        a.check_each()
+        assert (gpu.get(a.scratch + n, guard, np.uint8) == 0x5a).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_many_small_sequences(dtype, gpu, libs):
     rng = np.random.default_rng(5)
     nodes = [int(n) for n in rng.integers(0, 4, 300)]
