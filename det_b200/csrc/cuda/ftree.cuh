@@ -179,7 +179,7 @@ __device__ __forceinline__ TreeShare tree_start(const TreeArgs& a, int cta, int 
     }
     w.left = min(share, total - u0);
     w.cta = cta;
-    long long base = 0;                                       // places ahead of this round's segments
+    long long base = 0;                                       // places ahead of these 32 segments
     for (int i = lane;; i += 32) {
         const int places = i >= segs ? 0 : segs <= 32 ? mine : tree_places(a, tree_seg(a, i));
         long long sum = (long long)places * a.kv_heads;
