@@ -12,9 +12,10 @@
 namespace detb {
 
 constexpr int TS_KEYS = 32, TS_NJ = TS_KEYS / 16, TS_THREADS = 256;
+constexpr int TS_LDS = TS_KEYS + 8, TS_FEW = 4 * 16 * TS_LDS + 16;      // blocks of 16 rows: partial scores, factors
 
 static size_t simt_smem(int block, int kd, int vd, int stages) {
-    return ((size_t)block * (kd + 4) + (size_t)stages * TS_KEYS * (kd + vd + 8) + (size_t)block * (TS_KEYS + 4)) * sizeof(float);
+    return ((size_t)block * (kd + 4) + (size_t)stages * TS_KEYS * (kd + vd + 8) + (size_t)block * (TS_KEYS + 4) + (block == 16 ? TS_FEW : 0)) * sizeof(float);
 }
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
@@ -65,7 +66,7 @@ __device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t l
 // from shared memory where keys are many (a key costs all rows of the block, 16 TR, whatever is in them: 16 nodes of 4 sequences behind 4096
 // keys, 40 / 8 heads of 128, 272 us), by start, deal and second launch where they are few (6 / 2 heads of 40 and 24, five trees of 13
 // nodes behind 2000 keys: 23.8 us; 27.7 with tiles of 64 keys and one CTA on an SM).
-template <int TR, int VJ>
+template <int TR, int VJ, bool FEW>
 __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const TreeArgs a, int stages) {
     extern __shared__ __align__(16) float tsm[];
     __shared__ TreeShare share;
@@ -77,7 +78,13 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
     float* KV = P + RB * LDP;                    // [stage] K [32][ldk] | V [32][ldv]
     const int stage_floats = TS_KEYS * (ldk + ldv);
     // lanes that a row's values need; with fewer than 16 the others take other keys (a run of 4 after the other goes round)
-    const int lv = VJ > 1 || a.vd > 32 ? 16 : a.vd > 16 ? 8 : 4, vx = tx & (lv - 1), kstep = 64 / lv;
+    const int lv = FEW || VJ > 1 || a.vd > 32 ? 16 : a.vd > 16 ? 8 : 4, vx = tx & (lv - 1), kstep = 64 / lv;
+    // FEW (16 rows): every warp would read all keys for two rows of its own, so here a warp has all rows, 16 keys and a quarter of the elements
+    // of the scores, and four keys of the values; what the warps have is added up per tile and per stretch
+    constexpr int NQ = VJ == 4 ? 2 : 1, KPL = VJ == 1 ? 2 : 4;           // a lane's columns in fours, its keys
+    const int warp = tid >> 5, lane = tid & 31, fc = (VJ == 1 ? lane & 15 : lane) * 4, fk = warp * 4 + (VJ == 1 ? (lane >> 4) * 2 : 0);
+    float* S4 = KV + stages * stage_floats;      // [quarter][16][TS_LDS]
+    float* Fs = S4 + 4 * 16 * TS_LDS;            // a row's factor
     pdl_wait();
     pdl_trigger();                               // behind the wait: what k_ftree_merge reads ahead of its own is then there
     if (tid < 32) {
@@ -118,6 +125,11 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
 #pragma unroll
             for (int j = 0; j < VJ; j++) o[i][j] = make_float4(0, 0, 0, 0);
         }
+        float4 acc[FEW ? 16 : 1][NQ];
+#pragma unroll
+        for (int r = 0; r < (FEW ? 16 : 1); r++)
+#pragma unroll
+            for (int n = 0; n < NQ; n++) acc[r][n] = make_float4(0, 0, 0, 0);
         for (int t = it.tile, stage = 0; t < it.tile + it.n; t++) {
             const int k0 = t * TS_KEYS;
             const bool tree = k0 + TS_KEYS > s.edge;
@@ -141,16 +153,40 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
             for (int i = 0; i < TR; i++)
 #pragma unroll
                 for (int j = 0; j < TS_NJ; j++) sc[i][j] = 0.0f;
+            if constexpr (FEW) {
+                const int rg = lane >> 3, kg = (warp & 1) * 16 + (lane & 7), quarter = warp >> 1;
+                float part[4][2] = {};
 #pragma unroll 2
-            for (int e = 0; e < a.kd; e += 4) {
-                float4 kv[TS_NJ];
+                for (int e = quarter * 4; e < a.kd; e += 16) {
+                    const float4 k0v = load4(K + kg * ldk + e), k1v = load4(K + (kg + 8) * ldk + e);
 #pragma unroll
-                for (int j = 0; j < TS_NJ; j++) kv[j] = load4(K + (tx + 16 * j) * ldk + e);
+                    for (int i = 0; i < 4; i++) {
+                        const float4 qv = load4(Q + (rg + 4 * i) * ldk + e);
+                        part[i][0] = dot4(qv, k0v, part[i][0]);
+                        part[i][1] = dot4(qv, k1v, part[i][1]);
+                    }
+                }
 #pragma unroll
-                for (int i = 0; i < TR; i++) {
-                    const float4 qv = load4(Q + (ty + 16 * i) * ldk + e);
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int j = 0; j < TS_NJ; j++) sc[i][j] = dot4(qv, kv[j], sc[i][j]);
+                    for (int j = 0; j < 2; j++) S4[(quarter * 16 + rg + 4 * i) * TS_LDS + kg + 8 * j] = part[i][j];
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < TS_NJ; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) sc[0][j] += S4[(c * 16 + ty) * TS_LDS + tx + 16 * j];
+            } else {
+#pragma unroll 2
+                for (int e = 0; e < a.kd; e += 4) {
+                    float4 kv[TS_NJ];
+#pragma unroll
+                    for (int j = 0; j < TS_NJ; j++) kv[j] = load4(K + (tx + 16 * j) * ldk + e);
+#pragma unroll
+                    for (int i = 0; i < TR; i++) {
+                        const float4 qv = load4(Q + (ty + 16 * i) * ldk + e);
+#pragma unroll
+                        for (int j = 0; j < TS_NJ; j++) sc[i][j] = dot4(qv, kv[j], sc[i][j]);
+                    }
                 }
             }
 #pragma unroll
@@ -173,8 +209,12 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
                 const float base = mx == -INFINITY ? 0.0f : mx, f = exp2f(m[i] - base);
                 m[i] = mx;
                 l[i] *= f;
+                if constexpr (FEW) {
+                    if (tx == 0) Fs[ty] = f;
+                } else {
 #pragma unroll
-                for (int j = 0; j < VJ; j++) o[i][j] = scaled4(o[i][j], f);
+                    for (int j = 0; j < VJ; j++) o[i][j] = scaled4(o[i][j], f);
+                }
 #pragma unroll
                 for (int j = 0; j < TS_NJ; j++) {
                     const float p = exp2f(sc[i][j] - base);
@@ -183,22 +223,48 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
                 }
             }
             __syncthreads();
-            for (int k = tx / lv * 4; k < TS_KEYS; k += kstep) {
-                float4 p[TR];
+            if constexpr (FEW) {
 #pragma unroll
-                for (int i = 0; i < TR; i++) p[i] = load4(P + (ty + 16 * i) * LDP + k);
+                for (int n = 0; n < NQ; n++) {
+                    if (fc + 128 * n >= a.vd) continue;
+                    float4 v[KPL];
 #pragma unroll
-                for (int j = 0; j < VJ; j++) {
-                    const int c = 4 * vx + 64 * j;
-                    if (c >= a.vd) continue;
-                    const float4 v0 = load4(V + k * ldv + c), v1 = load4(V + (k + 1) * ldv + c), v2 = load4(V + (k + 2) * ldv + c),
-                                 v3 = load4(V + (k + 3) * ldv + c);
+                    for (int k = 0; k < KPL; k++) v[k] = load4(V + (fk + k) * ldv + fc + 128 * n);
 #pragma unroll
-                    for (int i = 0; i < TR; i++) {
-                        add4(o[i][j], p[i].x, v0);
-                        add4(o[i][j], p[i].y, v1);
-                        add4(o[i][j], p[i].z, v2);
-                        add4(o[i][j], p[i].w, v3);
+                    for (int r = 0; r < 16; r++) {
+                        acc[r][n] = scaled4(acc[r][n], Fs[r]);
+                        const float* p = P + r * LDP + fk;
+                        if (KPL == 4) {
+                            const float4 w = load4(p);
+                            add4(acc[r][n], w.x, v[0]);
+                            add4(acc[r][n], w.y, v[1]);
+                            add4(acc[r][n], w.z, v[KPL - 2]);
+                            add4(acc[r][n], w.w, v[KPL - 1]);
+                        } else {
+                            const float2 w = *reinterpret_cast<const float2*>(p);
+                            add4(acc[r][n], w.x, v[0]);
+                            add4(acc[r][n], w.y, v[1]);
+                        }
+                    }
+                }
+            } else {
+                for (int k = tx / lv * 4; k < TS_KEYS; k += kstep) {
+                    float4 p[TR];
+#pragma unroll
+                    for (int i = 0; i < TR; i++) p[i] = load4(P + (ty + 16 * i) * LDP + k);
+#pragma unroll
+                    for (int j = 0; j < VJ; j++) {
+                        const int c = 4 * vx + 64 * j;
+                        if (c >= a.vd) continue;
+                        const float4 v0 = load4(V + k * ldv + c), v1 = load4(V + (k + 1) * ldv + c), v2 = load4(V + (k + 2) * ldv + c),
+                                     v3 = load4(V + (k + 3) * ldv + c);
+#pragma unroll
+                        for (int i = 0; i < TR; i++) {
+                            add4(o[i][j], p[i].x, v0);
+                            add4(o[i][j], p[i].y, v1);
+                            add4(o[i][j], p[i].z, v2);
+                            add4(o[i][j], p[i].w, v3);
+                        }
                     }
                 }
             }
@@ -209,6 +275,35 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
                 fetch(t + 1, 0);
             }
             if (stages == 2) __syncthreads();    // the stage that the next round fills has been read
+        }
+        if constexpr (FEW) {                 // the warps' sums, over the stages (4 x 16 rows of values fit them for any sizes)
+            if (VJ == 1) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    acc[r][0].x += __shfl_xor_sync(FULL, acc[r][0].x, 16);
+                    acc[r][0].y += __shfl_xor_sync(FULL, acc[r][0].y, 16);
+                    acc[r][0].z += __shfl_xor_sync(FULL, acc[r][0].z, 16);
+                    acc[r][0].w += __shfl_xor_sync(FULL, acc[r][0].w, 16);
+                }
+            }
+            for (int h = 4;; h >>= 1) {          // the last round: warp 0 leaves the result
+                __syncthreads();
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+                        if (warp >= h && warp < max(1, 2 * h) && fc + 128 * n < a.vd) put4(KV + ((warp - h) * 16 + r) * a.vd + fc + 128 * n, acc[r][n]);
+                __syncthreads();
+                if (h == 0) break;
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+                        if (warp < h && fc + 128 * n < a.vd) add4(acc[r][n], 1.0f, load4(KV + (warp * 16 + r) * a.vd + fc + 128 * n));
+            }
+#pragma unroll
+            for (int j = 0; j < VJ; j++)
+                if (4 * tx + 64 * j < a.vd) o[0][j] = load4(KV + ty * a.vd + 4 * tx + 64 * j);
         }
         float* piece = a.part + ((size_t)blockIdx.x * 2 + it.piece) * tree_piece_floats(RB, a.vd);
         const bool fix = odd != 0;
@@ -385,24 +480,30 @@ __global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs
 }
 
 // ------------------------------------------------------------------------------------------------------ host side
-template <int TR, int VJ>
+template <int TR, int VJ, bool FEW>
 static cudaError_t launch_simt(const TreeArgs& a, cudaStream_t q) {
     const int stages = simt_smem(a.block, a.kd, a.vd, 2) <= 220 * 1024 ? 2 : 1;
     const size_t smem = simt_smem(a.block, a.kd, a.vd, stages);
-    const cudaError_t e = most_smem(k_ftree_simt<TR, VJ>);
+    const cudaError_t e = most_smem(k_ftree_simt<TR, VJ, FEW>);
     if (e != cudaSuccess) return e;
-    return launch_pdl_try(k_ftree_simt<TR, VJ>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a, stages);
+    return launch_pdl_try(k_ftree_simt<TR, VJ, FEW>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a, stages);
 }
-template <int TR>
+template <int TR, bool FEW>
 static cudaError_t launch_simt_v(const TreeArgs& a, cudaStream_t q) {
-    return a.vd <= 64 ? launch_simt<TR, 1>(a, q) : a.vd <= 128 ? launch_simt<TR, 2>(a, q) : launch_simt<TR, 4>(a, q);
+    return a.vd <= 64 ? launch_simt<TR, 1, FEW>(a, q) : a.vd <= 128 ? launch_simt<TR, 2, FEW>(a, q) : launch_simt<TR, 4, FEW>(a, q);
+}
+// FEW saves reads of shared memory in every tile and adds the warps' sums in every stretch.  With larger values it is the faster one even at
+// two tiles a CTA (8 / 1 heads of 128, two nodes of three sequences behind 2274 keys: 19.8 us, 21.9 without), with smaller ones from a few
+// tiles on (8 / 8 heads of 64, 10 tiles: 40.6 / 45.1; 4 / 2 heads of 40 and 24, 2 tiles: 15.8 / 13.2).
+static bool simt_few(const TreeArgs& a) {
+    return a.block == 16 && (a.vd > 64 || (long long)a.seq.seqs * a.kv_heads * a.blocks * (a.seq.max_len / TS_KEYS + 1) >= 6ll * a.ctas);
 }
 static cudaError_t launch_simt_r(const TreeArgs& a, cudaStream_t q) {
     switch (a.block) {
-        case 16: return launch_simt_v<1>(a, q);
-        case 32: return launch_simt_v<2>(a, q);
-        case 48: return launch_simt_v<3>(a, q);
-        default: return launch_simt_v<4>(a, q);
+        case 16: return simt_few(a) ? launch_simt_v<1, true>(a, q) : launch_simt_v<1, false>(a, q);
+        case 32: return launch_simt_v<2, false>(a, q);
+        case 48: return launch_simt_v<3, false>(a, q);
+        default: return launch_simt_v<4, false>(a, q);
     }
 }
 template <class T>

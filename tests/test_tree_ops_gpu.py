@@ -441,6 +441,28 @@ def test_pieces_stay_in_the_scratch(heads, dtype, gpu, libs):
         assert (gpu.get(a.scratch + n, guard, np.uint8) == 0x5a).all()
 
 
+@pytest.mark.parametrize("heads", [(4, 4, 64, 64), (6, 3, 40, 24), (1, 1, 16, 8), (5, 1, 96, 96), (2, 1, 128, 256), (3, 1, 24, 200)], ids=str)
+def test_few_rows_of_long_and_short_contexts_in_32_bits(heads, gpu, libs):
+    """Up to 16 rows of a key/value head: the kernel that spreads the keys over its warps (larger values, or many tiles) and the other one,
+    with masks, values that are not finite, and NaN that nobody attends."""
+    rng = np.random.default_rng(heads[0] * heads[3])
+    for lens, nodes in [([40], [1]), ([33, 0, 700], [3, 2, 1]), ([30000, 29000], [2, 1])]:
+        a = Attn(gpu, libs, "f32", *heads, lens, nodes, masks=random_masks(nodes, rng), sharp=2.0)
+        a.check_each()
+    for max_len in (0, 10 ** 6):                               # either choice for the same rows
+        a = Attn(gpu, libs, "f32", *heads, [300], [3], masks=[np.eye(3, dtype=bool)])
+        a.s.max_len = max_len
+        a.check_each()
+        H, G, d, v = heads
+        c = a.values[0].copy()
+        at = 302 - 1, G * round8(d) + v - 1                    # the last value of node 1, which node 1 alone attends
+        c[at] = np.inf
+        a.caches[0], a.values[0] = store(gpu, c, "f32")
+        got = a.call().reshape(3, H, v)
+        hit = np.arange(H) * G // H == 0 if G > 1 else np.ones(H, bool)
+        assert (got[1, hit, v - 1] == np.inf).all() and np.isfinite(got[[0, 2]]).all() and np.isfinite(got[1, :, :v - 1]).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_many_small_sequences(dtype, gpu, libs):
     rng = np.random.default_rng(5)
