@@ -101,8 +101,9 @@ __device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, int seg) {
     s.first = a.seq.first[s.b];
     s.n = a.seq.first[s.b + 1] - s.first;
     s.len = a.seq.len[s.b];
-    s.bad = s.first < 0 || s.n < 0 || s.n > a.seq.max_nodes || s.first > a.seq.rows - s.n || s.len < 0 || s.n > a.cap || s.len > a.cap - s.n ||
-            !usable_cache(a.seq.table[s.b].cache);
+    // a sequence without rows has nothing that could not fit: a slot that a batch leaves unused may hold anything
+    s.bad = s.n != 0 && (s.first < 0 || s.n < 0 || s.n > a.seq.max_nodes || s.first > a.seq.rows - s.n || s.len < 0 || s.n > a.cap || s.len > a.cap - s.n ||
+                         !usable_cache(a.seq.table[s.b].cache));
     if (s.bad) s.n = 0;
     s.rows = min(a.block, s.n * a.per_kv - s.r0);
     const int seen = a.mask ? s.n : min(s.n, (s.r0 + s.rows + a.per_kv - 1) / a.per_kv);

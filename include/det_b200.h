@@ -668,7 +668,8 @@ void det_f_moe(const det_fmoe_op* op, cudaStream_t st);
  *
  * The rows of a step.  Sequence b owns the rows first[b] .. first[b + 1] - 1 (first[0] = 0, ascending; none is allowed), node i of
  * its tree being row first[b] + i; its cache table[b].cache holds len[b] rows ahead of them, and node i belongs at cache row
- * len[b] + i.  table, first [seqs + 1] and len [seqs] are device arrays, so a captured step can be replayed with other lengths.
+ * len[b] + i.  Of a sequence without rows nothing else is looked at (a place of a batch that is not in use may have cache NULL).
+ * table, first [seqs + 1] and len [seqs] are device arrays, so a captured step can be replayed with other lengths.
  * `rows` is the number of rows of the buffers: rows from first[seqs] on belong to nobody and are left as they were.  max_nodes
  * bounds a sequence's rows; max_len (>= 0) is the expected largest len: it sizes the launch, and results hold for any len (attention:
  * up to 2^31 - 2^16 keys of a sequence).                                                                                     */
