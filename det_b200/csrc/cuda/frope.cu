@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(QK_THREADS, 4) k_fqk_rope(const QkArgs a, int 
     if (at.b < 0) return;
     const int pos = a.pos ? a.pos[row] : at.slot;
     void* base = a.seq.table[at.b].cache;
-    if (at.node < 0 || at.node >= a.seq.max_nodes || at.slot < at.node || at.slot >= a.cap || !usable_cache(base) ||
+    if (at.node < 0 || at.node >= a.seq.max_nodes || at.slot < 0 || at.slot >= a.cap || !usable_cache(base) ||
         ((a.rot || a.vcs) && (pos < 0 || pos >= a.rope_len))) {
         if (lane == 0) report_size(a.error_flag);
         return;

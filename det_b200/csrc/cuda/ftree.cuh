@@ -35,7 +35,7 @@ __device__ __forceinline__ void put4(bf16* p, float4 v) { *reinterpret_cast<uint
 // A cache pointer from device memory.
 __device__ __forceinline__ bool usable_cache(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// The place of a row: sequence, node of its tree, row of its cache.  b < 0: nobody's row.  Called by whole warps with one row.
+// The place of a row: sequence, node of its tree, row of its cache (negative: none).  b < 0: nobody's row.  Called by whole warps with one row.
 struct TreePlace {
     int b, node, slot;
 };
@@ -43,8 +43,9 @@ __device__ __forceinline__ TreePlace tree_place(const det_tree_ref& s, int row, 
     int b = 0;
     for (int i = lane; i - lane < s.seqs; i += 32) b += __popc(__ballot_sync(FULL, i < s.seqs && s.first[i + 1] <= row));
     if (b >= s.seqs) return {-1, 0, 0};
-    const int node = row - s.first[b];
-    return {b, node, s.len[b] + node};
+    const int node = (int)((unsigned)row - (unsigned)s.first[b]), len = s.len[b];
+    // a sum that passes 2^31 is none: a test of the sum itself would not hold, as signed sums are compiled as if they never overflowed
+    return {b, node, node < 0 || len < 0 || len > 0x7fffffff - node ? -1 : len + node};
 }
 
 // ------------------------------------------------------------------------------------------------------ attention

@@ -7,7 +7,7 @@ import pytest
 
 import tree_oracle as to
 from float_ops import code
-from test_tree_ops_gpu import Attn, gpu, ints, load, random_masks, rope_tables, size_error, slots, store  # noqa: F401  (gpu: a fixture)
+from test_tree_ops_gpu import Attn, gpu, ints, load, random_masks, size_error, slots, store  # noqa: F401  (gpu: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,32 @@ def test_places_of_a_batch_that_are_not_in_use(unused, dtype, gpu, libs):  # noq
                 gpu.d.det_debug_set_float(0)
                 assert size_error(gpu) == 0
                 a.check(load(gpu, op.out, (a.s.rows, a.ldo), dtype))
+
+
+# ------------------------------------------------------------------------------------------------------------------ lengths near 2^31
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 2, -2 ** 31, -1])
+def test_a_length_whose_rows_have_no_place_writes_nothing(length, dtype, gpu, libs):  # noqa: F811
+    """len + node passes 2^31, or is negative: no row of the sequence has a place in its cache, whose neighbours in memory stay as they were."""
+    H, G, d, cap, nodes = 2, 1, 16, 12, [4, 2]
+    ld, rows = 2 * G * d, 6
+    rng = np.random.default_rng(1)
+    y = np.float32(rng.standard_normal((rows, (H + 2 * G) * d)))
+    for order in (0, 1):
+        lens = [length, 3] if order == 0 else [3, length]
+        n = nodes[::1 if order == 0 else -1]
+        first = [0, n[0], rows]
+        caches = [store(gpu, np.full((cap, ld), KEPT), dtype)[0] for _ in lens]
+        q = store(gpu, np.full((rows, H * d), KEPT), dtype)[0]
+        ref = libs.TreeRef(table=slots(gpu, libs, caches), first=ints(gpu, first), len=ints(gpu, lens), seqs=2, rows=rows, max_nodes=4, max_len=cap)
+        op = libs.FQkOp(heads=H, kv_heads=G, dim=d, vdim=d, rot_dims=0, half=0, eps=0.0, cap=cap, dtype=code(libs, dtype), y=gpu.f32(y), ldy=y.shape[1],
+                        q_off=0, k_off=H * d, v_off=(H + G) * d, q=q, seq=ref)
+        assert gpu.d.det_f_qk_rope(C.byref(op), None) == 0
+        assert size_error(gpu) == SIZE_ERROR
+        stored, good = store(gpu, y, dtype)[1], 1 - order
+        r = slice(first[good], first[good + 1])
+        want_q, want = np.full((rows, H * d), KEPT), [np.full((cap, ld), KEPT) for _ in lens]
+        want_q[r], want[good][3:3 + n[good]] = stored[r, :H * d], stored[r, H * d:]
+        assert np.array_equal(load(gpu, q, (rows, H * d), dtype), want_q)
+        for p, c in zip(caches, want):
+            assert np.array_equal(load(gpu, p, (cap, ld), dtype), c)
