@@ -227,23 +227,28 @@ __device__ __forceinline__ QkLane qk_lane(const float* cs, const float* sn, size
     }
     return k;
 }
+// Block 0 looks through the sequences and reports those that do not fit (of which the buffers may hold no row); the others take the rows.
 template <class T, bool VEC, int LPH>
 __global__ void __launch_bounds__(QK_THREADS, 4) k_fqk_rope(const QkArgs a, int parts) {
     pdl_trigger();
-    const int lane = threadIdx.x & 31, task = (int)(((long long)blockIdx.x * QK_THREADS + threadIdx.x) >> 5), row = task / parts, part = task - row * parts;
     pdl_wait();
+    if (blockIdx.x == 0) {
+        bool bad = false;
+        for (int b = threadIdx.x; b < a.seq.seqs; b += QK_THREADS) bad |= tree_span(a.seq, a.cap, b).bad;
+        if (bad) report_size(a.error_flag);
+        return;
+    }
+    const int lane = threadIdx.x & 31, task = (int)(((long long)(blockIdx.x - 1) * QK_THREADS + threadIdx.x) >> 5), row = task / parts, part = task - row * parts;
     if (row >= a.seq.rows) return;
-    const TreePlace at = tree_place(a.seq, row, lane);
-    if (at.b < 0) return;
+    const TreePlace at = tree_place(a.seq, a.cap, row, lane);
+    if (at.nobodys) return;
     const int pos = a.pos ? a.pos[row] : at.slot;
-    void* base = a.seq.table[at.b].cache;
-    if (at.node < 0 || at.node >= a.seq.max_nodes || at.slot < 0 || at.slot >= a.cap || !usable_cache(base) ||
-        ((a.rot || a.vcs) && (pos < 0 || pos >= a.rope_len))) {
+    if (at.slot < 0 || ((a.rot || a.vcs) && (pos < 0 || pos >= a.rope_len))) {
         if (lane == 0) report_size(a.error_flag);
         return;
     }
     const float* y = a.y + (size_t)row * a.ldy;
-    T* cache = static_cast<T*>(base) + (size_t)at.slot * a.ld;
+    T* cache = static_cast<T*>(at.cache) + (size_t)at.slot * a.ld;
     // a group of heads after the other goes round the warps of the row: queries, then keys, then values
     constexpr int HEADS = 32 / LPH;
     const int gq = (a.heads + HEADS - 1) / HEADS, gk = (a.kv_heads + HEADS - 1) / HEADS;
@@ -264,7 +269,7 @@ static cudaError_t launch_qk(const QkArgs& a, cudaStream_t q) {
     // a group per warp while that leaves SMs idle, fourteen in long runs (8192 rows of 40/8 x 128: 87 us with four, 74 with seven, 70)
     const int parts = (int)std::max<long long>((groups + 13) / 14, std::min<long long>(groups, 32ll * sm_count() / a.seq.rows));
     const long long warps = (long long)a.seq.rows * parts;
-    const dim3 grid((unsigned)((warps + QK_THREADS / 32 - 1) / (QK_THREADS / 32))), block(QK_THREADS);
+    const dim3 grid((unsigned)(1 + (warps + QK_THREADS / 32 - 1) / (QK_THREADS / 32))), block(QK_THREADS);
     return lph == 8    ? launch_pdl_try(k_fqk_rope<T, VEC, 8>, grid, block, 0, q, 1, a, parts)
            : lph == 16 ? launch_pdl_try(k_fqk_rope<T, VEC, 16>, grid, block, 0, q, 1, a, parts)
                        : launch_pdl_try(k_fqk_rope<T, VEC, 32>, grid, block, 0, q, 1, a, parts);

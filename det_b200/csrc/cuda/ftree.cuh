@@ -35,17 +35,41 @@ __device__ __forceinline__ void put4(bf16* p, float4 v) { *reinterpret_cast<uint
 // A cache pointer from device memory.
 __device__ __forceinline__ bool usable_cache(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// The place of a row: sequence, node of its tree, row of its cache (negative: none).  b < 0: nobody's row.  Called by whole warps with one row.
-struct TreePlace {
-    int b, node, slot;
+// A sequence as device memory has it.  `bad`: its entries do not fit its cache (of `cap` rows) or the bounds of the call, and every op of the
+// step leaves it out whole (it then has no rows here).  A sequence without rows has nothing that could not fit: a place that a batch leaves
+// unused may hold anything.
+struct TreeSpan {
+    void* cache;
+    int first, n, len;
+    bool bad;
 };
-__device__ __forceinline__ TreePlace tree_place(const det_tree_ref& s, int row, int lane) {
+__device__ __forceinline__ TreeSpan tree_span(const det_tree_ref& s, int cap, int b) {
+    TreeSpan t;
+    const int next = s.first[b + 1];
+    t.cache = s.table[b].cache;
+    t.first = s.first[b];
+    t.n = (int)((unsigned)next - (unsigned)t.first);           // no sum or difference of what was not checked before may overflow
+    t.len = s.len[b];
+    // (conditions joined without branches: k_fqk_rope has no registers to spare)
+    t.bad = (t.n != 0) & ((t.first < 0) | (next < t.first) | (next > s.rows) | (t.n > s.max_nodes) | (t.n > cap) | (t.len < 0) |
+                          (t.len > (int)((unsigned)cap - (unsigned)t.n)) | !usable_cache(t.cache));
+    if (t.bad) t.n = 0;
+    if (t.n == 0) t.len = 0;
+    return t;
+}
+// The place of a row: its sequence's cache and the row there (negative: left out).  Called by whole warps with one row.
+struct TreePlace {
+    void* cache;
+    int slot;
+    bool nobodys;
+};
+__device__ __forceinline__ TreePlace tree_place(const det_tree_ref& s, int cap, int row, int lane) {
     int b = 0;
     for (int i = lane; i - lane < s.seqs; i += 32) b += __popc(__ballot_sync(FULL, i < s.seqs && s.first[i + 1] <= row));
-    if (b >= s.seqs) return {-1, 0, 0};
-    const int node = (int)((unsigned)row - (unsigned)s.first[b]), len = s.len[b];
-    // a sum that passes 2^31 is none: a test of the sum itself would not hold, as signed sums are compiled as if they never overflowed
-    return {b, node, node < 0 || len < 0 || len > 0x7fffffff - node ? -1 : len + node};
+    if (b >= s.seqs) return {nullptr, -1, true};
+    const TreeSpan t = tree_span(s, cap, b);
+    const unsigned node = (unsigned)row - (unsigned)t.first;
+    return {t.cache, node < (unsigned)t.n ? t.len + (int)node : -1, false};
 }
 
 // ------------------------------------------------------------------------------------------------------ attention
@@ -99,13 +123,11 @@ __device__ __forceinline__ TreeSeg tree_seg(const TreeArgs& a, int seg) {
     TreeSeg s;
     s.b = seg / a.blocks;
     s.r0 = (seg - s.b * a.blocks) * a.block;
-    s.first = a.seq.first[s.b];
-    s.n = a.seq.first[s.b + 1] - s.first;
-    s.len = a.seq.len[s.b];
-    // a sequence without rows has nothing that could not fit: a slot that a batch leaves unused may hold anything
-    s.bad = s.n != 0 && (s.first < 0 || s.n < 0 || s.n > a.seq.max_nodes || s.first > a.seq.rows - s.n || s.len < 0 || s.n > a.cap || s.len > a.cap - s.n ||
-                         !usable_cache(a.seq.table[s.b].cache));
-    if (s.bad) s.n = 0;
+    const TreeSpan t = tree_span(a.seq, a.cap, s.b);
+    s.first = t.first;
+    s.n = t.n;
+    s.len = t.len;
+    s.bad = t.bad;
     s.rows = min(a.block, s.n * a.per_kv - s.r0);
     const int seen = a.mask ? s.n : min(s.n, (s.r0 + s.rows + a.per_kv - 1) / a.per_kv);
     s.keys = s.len + seen;

@@ -64,3 +64,68 @@ def test_a_length_whose_rows_have_no_place_writes_nothing(length, dtype, gpu, li
         assert np.array_equal(load(gpu, q, (rows, H * d), dtype), want_q)
         for p, c in zip(caches, want):
             assert np.array_equal(load(gpu, p, (cap, ld), dtype), c)
+
+
+# ------------------------------------------------------------------------------------------------------------------ what does not fit
+BAD = {  # first, lens, rows of the buffers, places of the table that hold no cache, sequences that are left out (caches of 12 rows, trees of 4)
+    "full cache": ([0, 3, 5, 9], [10, 2, 1], 9, {}, {0}),
+    "full cache, last": ([0, 2, 5, 9], [10, 2, 9], 9, {}, {2}),
+    "large tree": ([0, 2, 7, 11], [1, 2, 3], 11, {}, {1}),
+    "negative length": ([0, 2, 4, 8], [1, -1, 8], 8, {}, {1}),
+    "largest length": ([0, 2, 4, 8], [2 ** 31 - 1, 10, 0], 8, {}, {0}),
+    "rows behind the buffers": ([0, 2, 4, 8], [0, 1, 2], 6, {}, {2}),
+    "no row in the buffers": ([0, 2, 6, 9], [0, 1, 2], 6, {}, {2}),
+    "first row negative": ([-1, 2, 4, 8], [0, 1, 2], 9, {}, {0}),
+    "no cache": ([0, 2, 4, 8], [0, 1, 2], 8, {1: None}, {1}),
+    "misaligned cache": ([0, 2, 4, 8], [0, 1, 2], 8, {0: 8}, {0}),
+    "all": ([0, 5, 5, 7], [0, 0, 11], 7, {}, {0, 2}),
+}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 24, 11], ids=["64", "24", "11 (no vectors)"])
+@pytest.mark.parametrize("kind", BAD)
+def test_a_sequence_that_does_not_fit_is_left_out_whole(kind, dim, dtype, gpu, libs):  # noqa: F811
+    """Every row of q and every row of the cache of such a sequence stay as they were, rows among them that would have fitted alone; the
+    attention of the same step leaves out the same sequences.  Without norm and rotation the rows are the activations, rounded once."""
+    first, lens, rows, missing, bad = BAD[kind]
+    H, G, cap, max_nodes, seqs = 4, 2, 12, 4, len(lens)
+    kd = (dim + 7) // 8 * 8
+    ld = 2 * G * kd
+    rng = np.random.default_rng(dim)
+    y = np.float32(rng.standard_normal((rows, (H + 2 * G) * dim)))
+    caches = [store(gpu, np.full((cap, ld), KEPT), dtype)[0] for _ in lens]
+    q = store(gpu, np.full((rows, H * kd), KEPT), dtype)[0]
+    table = slots(gpu, libs, [missing.get(b, c) for b, c in enumerate(caches)])
+    ref = libs.TreeRef(table=table, first=ints(gpu, first), len=ints(gpu, lens), seqs=seqs, rows=rows, max_nodes=max_nodes, max_len=cap)
+    op = libs.FQkOp(heads=H, kv_heads=G, dim=dim, vdim=dim, rot_dims=0, half=0, eps=0.0, cap=cap, dtype=code(libs, dtype), y=gpu.f32(y), ldy=y.shape[1],
+                    q_off=0, k_off=H * dim, v_off=(H + G) * dim, q=q, seq=ref)
+    assert gpu.d.det_f_qk_rope(C.byref(op), None) == 0
+    assert size_error(gpu) == SIZE_ERROR
+    stored = store(gpu, y, dtype)[1].reshape(rows, H + 2 * G, dim)
+    want_q, want = np.full((rows, H, kd), KEPT), [np.full((cap, 2 * G, kd), KEPT) for _ in lens]
+    for b in set(range(seqs)) - bad:
+        r = slice(first[b], first[b + 1])
+        n = first[b + 1] - first[b]
+        want_q[r] = 0.0
+        want_q[r, :, :dim] = stored[r, :H]
+        want[b][lens[b]:lens[b] + n] = 0.0
+        want[b][lens[b]:lens[b] + n, :, :dim] = stored[r, H:]
+    assert np.array_equal(load(gpu, q, (rows, H, kd), dtype), want_q)
+    for p, c in zip(caches, want):
+        assert np.array_equal(load(gpu, p, (cap, 2 * G, kd), dtype), c)
+    mask = to.bits(np.ones((rows, 32), bool), 1)
+    for masked in (0, 1):
+        for flags in (0, 16, 32):
+            out = store(gpu, np.full((rows, H * dim), -3.0), dtype)[0]
+            ta = libs.FTreeOp(heads=H, kv_heads=G, dim=dim, vdim=dim, scale=0.3, cap=cap, dtype=code(libs, dtype), q=q, mask=gpu.put(mask) if masked else None,
+                              mask_ld=masked, out=out, ldo=H * dim, scratch=gpu.space(gpu.d.det_f_tree_scratch_bytes(H, G, dim, max_nodes)), seq=ref)
+            gpu.d.det_debug_set_float(flags)
+            assert gpu.d.det_f_tree_attn(C.byref(ta), None) == 0
+            gpu.d.det_debug_set_float(0)
+            assert size_error(gpu) == SIZE_ERROR
+            left = (load(gpu, out, (rows, H * dim), dtype) == -3.0).all(1)      # (a row may well be the 7 of the cached rows)
+            own = np.zeros(rows, bool)
+            for b in set(range(seqs)) - bad:
+                own[first[b]:first[b + 1]] = True
+            assert np.array_equal(left, ~own)
