@@ -9,7 +9,7 @@
 namespace detb {
 
 struct KeepArgs {
-    int seqs, cap, pieces;      // 16-byte pieces of a row
+    int layers, seqs, cap, pieces;      // 16-byte pieces of a row
     const det_seq_slot* table;
     const int* len;
     const int* keep;
@@ -28,14 +28,18 @@ __global__ void __launch_bounds__(KEEP_THREADS) k_fkeep(const KeepArgs a) {
     pdl_wait();
     const int e = blockIdx.x, b = e % a.seqs, len = a.len[b];
     int n = a.count[b];
-    bool fits = len >= 0 && n >= 0 && n <= a.max_count && len <= a.cap && usable_cache(a.table[e].cache);
+    bool fits = len >= 0 && n >= 0 && n <= a.max_count && len <= a.cap;
+    // the caches of all layers of the sequence (a thread's first one is asked for ahead of the list): its blocks agree, and none moves rows when
+    // one of them cannot
+    bool usable = (int)threadIdx.x >= a.layers || usable_cache(a.table[b + (int)threadIdx.x * a.seqs].cache);
     if (fits)
         for (int i = threadIdx.x; i < n; i += KEEP_THREADS) {
             const int k = a.keep[(size_t)b * a.keep_ld + i];
             list[i] = k;
             if (k < i || k >= a.cap - len || (i > 0 && a.keep[(size_t)b * a.keep_ld + i - 1] >= k)) fits = false;
         }
-    fits = __syncthreads_and(fits);
+    for (int i = threadIdx.x + KEEP_THREADS; i < a.layers; i += KEEP_THREADS) usable = usable && usable_cache(a.table[b + i * a.seqs].cache);
+    fits = __syncthreads_and(fits && usable);
     if (!fits) {
         if (threadIdx.x == 0) report_size(a.error_flag);
         n = 0;
@@ -70,7 +74,7 @@ extern "C" int det_f_tree_keep(const det_fkeep_op* op, cudaStream_t st) {
     DETB_TAKE(op->table && op->len && op->count && (op->keep || op->max_count == 0), "table, len, keep or count is NULL");
     DETB_TAKE(op->len_out != op->len, "len_out must not be len");
     DETB_TAKE(runtime_ready(), "no usable device");
-    KeepArgs a{op->seqs, op->cap, op->row_bytes / 16, op->table, op->len, op->keep, op->keep_ld, op->count, op->max_count, op->len_out, error_word()};
+    KeepArgs a{op->caches / op->seqs, op->seqs, op->cap, op->row_bytes / 16, op->table, op->len, op->keep, op->keep_ld, op->count, op->max_count, op->len_out, error_word()};
     const int pieces = (a.pieces + KEEP_THREADS - 1) / KEEP_THREADS;
     DETB_TAKE(pieces <= 65535, "the row is too long");
     return launched(name, launch_pdl_try(k_fkeep, dim3(op->caches, pieces), dim3(KEEP_THREADS), 0, queue_of(st), 1, a));

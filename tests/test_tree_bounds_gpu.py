@@ -129,3 +129,42 @@ def test_a_sequence_that_does_not_fit_is_left_out_whole(kind, dim, dtype, gpu, l
             for b in set(range(seqs)) - bad:
                 own[first[b]:first[b + 1]] = True
             assert np.array_equal(left, ~own)
+
+
+# ------------------------------------------------------------------------------------------------------------------ kept rows
+class Kept:
+    """det_f_tree_keep over `layers` caches of every sequence, with the table's entries as given (entry e belongs to sequence e % seqs)."""
+
+    def __init__(self, gpu, libs, lens, lists, layers, cap, missing, most=6):  # noqa: F811
+        self.gpu, self.lens, self.lists, self.cap, self.width = gpu, lens, lists, cap, 8
+        seqs = len(lens)
+        rng = np.random.default_rng(seqs)
+        self.before = rng.standard_normal((layers * seqs, cap, self.width)).astype(np.float32)
+        self.caches = [gpu.put(c) for c in self.before]
+        keep = np.zeros((seqs, most), np.int32)
+        for b, k in enumerate(lists):
+            keep[b, :len(k)] = k
+        self.out = ints(gpu, [-1] * seqs)
+        op = libs.FKeepOp(caches=layers * seqs, seqs=seqs, cap=cap, row_bytes=self.width * 4, table=slots(gpu, libs, [missing.get(e, c) for e, c in enumerate(self.caches)]),
+                          len=ints(gpu, lens), keep=gpu.put(keep), keep_ld=most, count=ints(gpu, [len(k) for k in lists]), max_count=most, len_out=self.out)
+        assert gpu.d.det_f_tree_keep(C.byref(op), None) == 0
+
+    def check(self, bad):
+        """The sequences `bad` as they were in every layer, the others moved up."""
+        seqs = len(self.lens)
+        for e, p in enumerate(self.caches):
+            want, b = self.before[e].copy(), e % seqs
+            if b not in bad:
+                for i, k in enumerate(self.lists[b]):
+                    want[self.lens[b] + i] = self.before[e][self.lens[b] + k]
+            assert np.array_equal(self.gpu.get(p, (self.cap, self.width)), want), e
+        assert np.array_equal(self.gpu.get(self.out, seqs, np.int32), [-1 if b in bad else n + len(k) for b, (n, k) in enumerate(zip(self.lens, self.lists))])
+
+
+@pytest.mark.parametrize("slot", [None, 8, 4096 + 4], ids=["NULL", "8", "4100"])
+@pytest.mark.parametrize("layers,entry", [(1, 0), (3, 0), (3, 3), (3, 4), (3, 6), (3, 8), (400, 599), (400, 1199)])
+def test_a_sequence_is_kept_in_all_layers_or_in_none(layers, entry, slot, gpu, libs):  # noqa: F811
+    """One layer of a sequence holds no usable cache: none of its layers moves and its length stays, the other sequences move."""
+    k = Kept(gpu, libs, [4, 5, 3], [[0, 2, 3], [1, 4], [0, 1, 5]], layers, 12, {entry: slot})
+    assert size_error(gpu) == SIZE_ERROR
+    k.check({entry % 3})
