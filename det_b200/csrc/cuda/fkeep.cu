@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) k_fkeep(const KeepArgs a) {
             if (k < i || k >= a.cap - len || (i > 0 && a.keep[(size_t)b * a.keep_ld + i - 1] >= k)) fits = false;
         }
     for (int i = threadIdx.x + KEEP_THREADS; i < a.layers; i += KEEP_THREADS) usable = usable && usable_cache(a.table[b + i * a.seqs].cache);
-    fits = __syncthreads_and(fits && usable);
+    fits = __syncthreads_and(fits && (usable || n == 0));      // with nothing to move the caches need not be there (a place not in use)
     if (!fits) {
         if (threadIdx.x == 0) report_size(a.error_flag);
         n = 0;

@@ -773,8 +773,8 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st);
 
 /* The accepted nodes of every tree become cached rows: in each cache, row len[b] + keep[b * keep_ld + i] moves to row len[b] + i,
  * i < count[b].  keep must ascend strictly.  table holds `caches` slots, layer after layer: entry e belongs to sequence e % seqs
- * (no cache twice; a sequence is moved in all of its caches or, where one of them or the list does not fit, in none).  row_bytes is a
- * multiple of 16 (any cache of this part whose rows are 16-byte aligned).  len_out (not len;
+ * (no cache twice; a sequence is moved in all of its caches or, where one of them or the list does not fit, in none; with count 0 its
+ * caches are not looked at).  row_bytes is a multiple of 16 (any cache of this part whose rows are 16-byte aligned).  len_out (not len;
  * NULL: none) receives len[b] + count[b].  max_count bounds count, <= DET_MAX_TREE.  All arrays are device arrays.          */
 typedef struct {
     int caches;

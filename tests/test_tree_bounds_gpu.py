@@ -168,3 +168,10 @@ def test_a_sequence_is_kept_in_all_layers_or_in_none(layers, entry, slot, gpu, l
     k = Kept(gpu, libs, [4, 5, 3], [[0, 2, 3], [1, 4], [0, 1, 5]], layers, 12, {entry: slot})
     assert size_error(gpu) == SIZE_ERROR
     k.check({entry % 3})
+
+
+def test_sequences_that_keep_nothing_need_no_cache(gpu, libs):  # noqa: F811
+    """Places of a batch that are not in use: count 0, no cache in any layer, or none in one; the new length is the old one."""
+    k = Kept(gpu, libs, [0, 5, 3, 0], [[], [1, 4], [], []], 2, 12, {0: None, 4: None, 2: 8, 3: 4, 7: None})
+    assert size_error(gpu) == 0
+    k.check(set())
