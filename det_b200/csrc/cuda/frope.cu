@@ -336,7 +336,7 @@ int det_f_qk_rope(const det_fqk_op* op, cudaStream_t st) {
     DETB_TAKE(op->q_off >= 0 && op->k_off >= 0 && op->v_off >= 0 && op->ldy >= 0, "bad columns");
     DETB_TAKE(std::isfinite(op->eps) && op->eps >= 0.0f, "bad eps");
     if (const char* why = bad_ref(op->seq)) return refuse(name, why);
-    if (op->seq.rows == 0 || op->seq.seqs == 0) return 0;
+    if (op->seq.rows == 0 || op->seq.seqs == 0 || op->seq.max_nodes == 0) return 0;
     DETB_TAKE(op->y && op->q && aligned16(op->q), "y or q is NULL or misaligned");
     DETB_TAKE(!op->rot_dims || (op->rope_cos && op->rope_sin), "no tables");
     DETB_TAKE((!op->rot_dims && !op->vrope_cos) || op->rope_len > 0, "empty tables");

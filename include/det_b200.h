@@ -671,8 +671,8 @@ void det_f_moe(const det_fmoe_op* op, cudaStream_t st);
  * len[b] + i.  Of a sequence without rows nothing else is looked at (a place of a batch that is not in use may have cache NULL).
  * table, first [seqs + 1] and len [seqs] are device arrays, so a captured step can be replayed with other lengths.
  * `rows` is the number of rows of the buffers: rows from first[seqs] on belong to nobody and are left as they were.  max_nodes
- * bounds a sequence's rows; max_len (>= 0) is the expected largest len: it sizes the launch, and results hold for any len (attention:
- * up to 2^31 - 2^16 keys of a sequence).                                                                                     */
+ * bounds a sequence's rows; 0 says that none has any, and the call returns 0 without a look at device memory.  max_len (>= 0) is the
+ * expected largest len: it sizes the launch, and results hold for any len (attention: up to 2^31 - 2^16 keys of a sequence).   */
 typedef struct {
     const det_seq_slot* table;
     const int* first;
