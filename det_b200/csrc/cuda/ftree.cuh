@@ -14,11 +14,12 @@ inline int refuse(const char* op, const char* why) {
         if (!(cond)) return refuse(name, why); \
     } while (0)
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// The verdict of a launch as a return code.
-inline int launched(const char* name, cudaError_t e) {
+// The verdict of a launch as a return code.  A failed launch is no refusal: an earlier one of the same call may have been queued.
+inline int launched(const char* op, cudaError_t e) {
     if (e == cudaSuccess) return 0;
     (void)cudaGetLastError();
-    return refuse(name, cudaGetErrorString(e));
+    fprintf(stderr, "det_b200: %s: the launch failed: %s\n", op, cudaGetErrorString(e));
+    return 1;
 }
 inline const char* bad_ref(const det_tree_ref& s) {
     if (s.seqs < 0 || s.rows < 0 || s.max_len < 0 || s.max_nodes < 0) return "negative sizes";

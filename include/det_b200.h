@@ -661,7 +661,9 @@ void det_f_moe(const det_fmoe_op* op, cudaStream_t st);
 
 /* ---- A step of drafted tokens (speculative decoding): several sequences, each with a tree of tokens behind its cached rows.
  * The entry points below return 0 when the work was queued and 1 when the call was refused (bad sizes, a NULL pointer, a misaligned
- * buffer, no usable device): a refusal prints its reason, launches nothing and leaves every buffer as it was; they never abort.
+ * buffer, no usable device): a refusal prints its reason, launches nothing and leaves every buffer as it was; they never abort.  They
+ * also return 1, and print the CUDA error, when a launch fails (a capture that was invalidated, a context in error): that is no refusal,
+ * det_f_tree_attn queues up to two kernels, and where the second fails out and scratch may be written in part.
  * What only device memory knows (first, len, pos, keep, count) is checked by the kernels: a sequence whose entries do not fit its
  * cache or the bounds of the call, and a row whose position the tables do not hold, is left out: its outputs stay as they were, and
  * det_last_error() returns 2.  A call's outputs must not overlap its inputs.

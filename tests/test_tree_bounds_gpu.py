@@ -175,3 +175,46 @@ def test_sequences_that_keep_nothing_need_no_cache(gpu, libs):  # noqa: F811
     k = Kept(gpu, libs, [0, 5, 3, 0], [[], [1, 4], [], []], 2, 12, {0: None, 4: None, 2: 8, 3: 4, 7: None})
     assert size_error(gpu) == 0
     k.check(set())
+
+
+# ------------------------------------------------------------------------------------------------------------------ failed launches
+def test_a_launch_that_fails_is_reported_and_ends_nothing(gpu, libs, capfd):  # noqa: F811
+    """A stream whose capture was invalidated takes no kernel (an error of the host alone): every op returns 1 and names the CUDA error,
+    nothing is written, and the same calls work afterwards."""
+    rt = C.CDLL("libcudart.so.12")
+    a = Attn(gpu, libs, "bf16", 4, 2, 64, 64, [130], [5])
+    b = Attn(gpu, libs, "f32", 4, 2, 64, 64, [130], [5])
+    y = gpu.f32(np.ones((5, 8 * 64), np.float32))
+    q, tab = gpu.space(5 * 4 * 64 * 4), gpu.space(2 * 4 * 4 * 8)
+    k = Kept(gpu, libs, [4, 5], [[0, 2, 3], [1, 4]], 2, 12, {})
+    gpu.d.det_memset(q, 0, 5 * 4 * 64 * 4, None)
+    gpu.d.det_memset(tab, 0, 2 * 4 * 4 * 8, None)
+    ops = [(gpu.d.det_f_tree_attn, a.op()), (gpu.d.det_f_tree_attn, b.op()),
+           (gpu.d.det_f_rope_table, libs.FRopeOp(dims=8, scaling=0, base=1e4, factor=1.0, mscale=1.0, n=8, cos=tab, sin=tab + 4 * 4 * 8)),
+           (gpu.d.det_f_qk_rope, libs.FQkOp(heads=4, kv_heads=2, dim=64, vdim=64, rot_dims=0, half=0, eps=0.0, cap=a.cap, dtype=libs.DET_BF16, y=y, ldy=512,
+                                            q_off=0, k_off=256, v_off=384, q=q, seq=a.s.ref(a.caches))),
+           (gpu.d.det_f_tree_keep, libs.FKeepOp(caches=1, seqs=1, cap=a.cap, row_bytes=a.ld * 2, table=a.s.ref(a.caches).table, len=a.s.len_p,
+                                                keep=ints(gpu, [1]), keep_ld=1, count=ints(gpu, [1]), max_count=1))]
+    gpu.d.det_sync()
+    before = load(gpu, a.caches[0], (a.cap, a.ld), "bf16")
+    stream, graph = C.c_void_p(), C.c_void_p()
+    assert rt.cudaStreamCreateWithFlags(C.byref(stream), 1) == 0
+    assert rt.cudaStreamBeginCapture(stream, 2) == 0             # relaxed: other streams are not restricted
+    assert rt.cudaStreamSynchronize(stream) != 0                 # not allowed in a capture, which it ends
+    capfd.readouterr()
+    for entry, op in ops:
+        assert entry(C.byref(op), stream) == 1
+        err = capfd.readouterr().err
+        assert "the launch failed" in err and "refused" not in err
+    rt.cudaStreamEndCapture(stream, C.byref(graph))
+    assert not graph
+    rt.cudaGetLastError()
+    assert rt.cudaStreamDestroy(stream) == 0
+    gpu.d.det_sync()
+    assert (gpu.get(q, 5 * 4 * 64) == 0).all() and (gpu.get(tab, 2 * 4 * 8) == 0).all()
+    assert np.array_equal(load(gpu, a.caches[0], (a.cap, a.ld), "bf16"), before, equal_nan=True)
+    for x in (a, b):
+        assert (load(gpu, x.out, (x.s.rows, x.ldo), x.dtype) == KEPT).all()
+        x.check_each()
+    k.check(set())
+    assert size_error(gpu) == 0
