@@ -17,7 +17,10 @@ struct RopeArgs {
     float* cs;
     float* sn;
 };
-// Turns per position of column i.
+// Turns per position of column i.  In units u = 2^-53: log2 of the base is off by 2 u of itself (with a scaled base the sum by 5 u of its terms),
+// the quotient and the product by one each, so f by ln 2 * (4 or 7) u * g, g the size of the exponent; exp2 adds 2 u, 1 / 2 pi and its product 2,
+// the linear factor 2: together below (5 g + 9) u.  The ramp's weight is off by (2.8 g + 9) u of (weight + low / span), which the factor between
+// both ends of the ramp scales.
 __device__ __forceinline__ double turns_of(const RopeArgs& a, int i) {
     constexpr double INV_2PI = 0.15915494309189533577;
     const double f = exp2(-2.0 * i / a.dims * a.log2_base);

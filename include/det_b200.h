@@ -686,8 +686,10 @@ typedef struct {
 } det_tree_ref;
 
 /* Tables of the position rotation: cos[p][i] = mscale * cos((pos0 + p) * f_i), sin likewise, p < n, i < dims / 2 (fp32).
- * f_i in binary64; the angle is kept as 64-bit turns, so far positions lose no more than binary64 does (2^-53 of the angle), and the
- * result is within 4 units of 2^-24 * mscale of it.  f_i = base^(-2i / dims), scaled for contexts longer than the model was made for:
+ * f_i is formed in binary64 and the angle a kept as 64-bit turns; the result is within mscale * (4 * 2^-24 + |a| (5 g + 9) 2^-53) of
+ * the exact one, g = 2i / dims * (|log2 base| + |log2 factor| dims / (dims - 2), the latter with DET_ROPE_BASE only): the roundings of an
+ * exponent grow with it.  With DET_ROPE_RAMP and factor >= 1 the second term is up to 2 + factor |low| / (high - low) times as large.
+ * f_i = base^(-2i / dims), scaled for contexts longer than the model was made for:
  *   DET_ROPE_LINEAR  f_i / factor
  *   DET_ROPE_BASE    base * factor^(dims / (dims - 2)) instead of base (dims > 2)
  *   DET_ROPE_RAMP    f_i * (w + (1 - w) / factor), w = (orig_ctx * f_i / 2 pi - low) / (high - low) clamped to 0 .. 1: columns

@@ -1,6 +1,8 @@
 """Which rows of a step of drafted tokens belong to whom, and what is left out: places of a batch that are not in use, sequences that do
 not fit, through every op that reads a det_tree_ref, against the plain functions of tree_oracle.py in float64."""
 import ctypes as C
+import decimal
+import math
 
 import numpy as np
 import pytest
@@ -218,3 +220,60 @@ def test_a_launch_that_fails_is_reported_and_ends_nothing(gpu, libs, capfd):  # 
         x.check_each()
     k.check(set())
     assert size_error(gpu) == 0
+
+
+# ------------------------------------------------------------------------------------------------------------------ far positions
+def exact_frequencies(dims, base, scaling, factor, orig, low, high):
+    """As decimals of 60 digits; everything that comes in is a binary64 number, taken as it is."""
+    D = decimal.Decimal
+    base, factor, orig, low, high = (D(x) for x in (base, factor, orig, low, high))
+    log_base = base.ln()
+    if scaling == "base":
+        log_base += factor.ln() * dims / (dims - 2)
+    f = [(-2 * i * log_base / dims).exp() for i in range(dims // 2)]
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    if scaling == "ramp":
+        w = [min(max((orig * x / (2 * decimal_pi()) - low) / (high - low), D(0)), D(1)) for x in f]
+        f = [x * (y + (1 - y) / factor) for x, y in zip(f, w)]
+    return f
+
+
+def decimal_pi():
+    """16 atan(1/5) - 4 atan(1/239)."""
+    def atan(n):
+        x = decimal.Decimal(1) / n
+        s, term, k = x, x, 1
+        while abs(term) > decimal.Decimal(10) ** -65:
+            term = -term / (n * n)
+            k += 2
+            s += term / k
+        return s
+    return 16 * atan(5) - 4 * atan(239)
+
+
+@pytest.mark.parametrize("dims,base", [(8, 10007.0), (128, 1000003.0), (26, 500.5), (256, 3.0e7), (64, 0.37)])
+@pytest.mark.parametrize("scaling,factor,low,high", [("plain", 1.0, 1.0, 2.0), ("linear", 7.3, 1.0, 2.0), ("base", 4.1, 1.0, 2.0), ("base", 0.3, 1.0, 2.0),
+                                                     ("ramp", 32.7, 1.0, 32.0), ("ramp", 4.2, 0.0, 3.0), ("ramp", 11.0, 40.0, 41.0)])
+def test_tables_of_far_positions(scaling, factor, low, high, dims, base, gpu, libs):  # noqa: F811
+    """Every column at the first positions, at 2^20 and at the last ones of 31 bits, against frequencies and angles of 60 digits: within the
+    bound that the header states, the angle's loss growing with the exponent of the frequency."""
+    orig, m, n = 4096.0, np.float32(1.1), 5
+    cols = dims // 2
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60
+        f = exact_frequencies(dims, base, scaling, factor, orig, low, high)
+        turn = 2 * decimal_pi()
+        for pos0 in (0, 2 ** 20, 2 ** 31 - 1 - n):
+            cs, sn = gpu.space(4 * n * cols), gpu.space(4 * n * cols)
+            op = libs.FRopeOp(dims=dims, scaling=["plain", "linear", "base", "ramp"].index(scaling), base=base, factor=factor, orig_ctx=orig, low=low, high=high,
+                              mscale=m, pos0=pos0, n=n, cos=cs, sin=sn)
+            assert gpu.d.det_f_rope_table(C.byref(op), None) == 0
+            a = np.array([[float(p * x) for x in f] for p in range(pos0, pos0 + n)])
+            rest = np.array([[float(p * x % turn) for x in f] for p in range(pos0, pos0 + n)])      # known to 2^-53 * 2 pi
+            g = 2 * np.arange(cols) / dims * (abs(math.log2(base)) + (abs(math.log2(factor)) * dims / (dims - 2) if scaling == "base" else 0))
+            loss = (5 * g + 9) * 2.0 ** -53 * (2 + factor * abs(low) / (high - low) if scaling == "ramp" else 1)
+            tol = float(m) * (4 * to.U32 + a * loss) + 2.0 ** -50
+            for p, want in ((cs, np.cos(rest)), (sn, np.sin(rest))):
+                err = np.abs(gpu.get(p, n * cols).astype(float).reshape(n, cols) - float(m) * want)
+                assert (err <= tol).all(), (err / tol).max()
