@@ -14,8 +14,9 @@ namespace detb {
 constexpr int TS_KEYS = 32, TS_NJ = TS_KEYS / 16, TS_THREADS = 256;
 constexpr int TS_LDS = TS_KEYS + 8, TS_FEW = 4 * 16 * TS_LDS + 16;      // blocks of 16 rows: partial scores, factors
 
-static size_t simt_smem(int block, int kd, int vd, int stages) {
-    return ((size_t)block * (kd + 4) + (size_t)stages * TS_KEYS * (kd + vd + 8) + (size_t)block * (TS_KEYS + 4) + (block == 16 ? TS_FEW : 0)) * sizeof(float);
+// Of a CTA: query rows, two stages of keys and values, weights (208,896 bytes at most: 64 rows, heads of 256).
+static size_t simt_smem(int block, int kd, int vd) {
+    return ((size_t)block * (kd + 4) + (size_t)2 * TS_KEYS * (kd + vd + 8) + (size_t)block * (TS_KEYS + 4) + (block == 16 ? TS_FEW : 0)) * sizeof(float);
 }
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float dot4(float4 a, float4 b, float s) {
@@ -61,13 +62,13 @@ __device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t l
     else copy_tile<64>(dst, src, ld, n, have);
 }
 
-// Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.  With two stages the next tile's copies run
+// Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.  Two stages: the next tile's copies run
 // beside the products of this one; two CTAs on an SM cover one another's latencies.  Bound by the fp32 multiply-adds and their operands
 // from shared memory where keys are many (a key costs all rows of the block, 16 TR, whatever is in them: 16 nodes of 4 sequences behind 4096
 // keys, 40 / 8 heads of 128, 272 us), by start, deal and second launch where they are few (6 / 2 heads of 40 and 24, five trees of 13
 // nodes behind 2000 keys: 23.8 us; 27.7 with tiles of 64 keys and one CTA on an SM).
 template <int TR, int VJ, bool FEW>
-__global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const TreeArgs a, int stages) {
+__global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const TreeArgs a) {
     extern __shared__ __align__(16) float tsm[];
     __shared__ TreeShare share;
     __shared__ int odd;                          // a staged value that not every row sees was not finite
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
     // of the scores, and four keys of the values; what the warps have is added up per tile and per stretch
     constexpr int NQ = VJ == 4 ? 2 : 1, KPL = VJ == 1 ? 2 : 4;           // a lane's columns in fours, its keys
     const int warp = tid >> 5, lane = tid & 31, fc = (VJ == 1 ? lane & 15 : lane) * 4, fk = warp * 4 + (VJ == 1 ? (lane >> 4) * 2 : 0);
-    float* S4 = KV + stages * stage_floats;      // [quarter][16][TS_LDS]
+    float* S4 = KV + 2 * stage_floats;      // [quarter][16][TS_LDS]
     float* Fs = S4 + 4 * 16 * TS_LDS;            // a row's factor
     pdl_wait();
     pdl_trigger();                               // behind the wait: what k_ftree_merge reads ahead of its own is then there
@@ -130,17 +131,13 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
         for (int r = 0; r < (FEW ? 16 : 1); r++)
 #pragma unroll
             for (int n = 0; n < NQ; n++) acc[r][n] = make_float4(0, 0, 0, 0);
-        for (int t = it.tile, stage = 0; t < it.tile + it.n; t++) {
+        for (int t = it.tile, stage = 0; t < it.tile + it.n; t++, stage ^= 1) {
             const int k0 = t * TS_KEYS;
             const bool tree = k0 + TS_KEYS > s.edge;
             float* K = KV + stage * stage_floats;
             float* V = K + TS_KEYS * ldk;
-            if (stages == 2) {
-                fetch(t + 1, stage ^ 1);
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-            } else {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-            }
+            fetch(t + 1, stage ^ 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncthreads();
             if (tree) {                          // a weight of zero does not undo a value that is not finite
                 for (int i = tid; i < TS_KEYS * a.vd; i += TS_THREADS) {
@@ -156,7 +153,7 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
             if constexpr (FEW) {
                 const int rg = lane >> 3, kg = (warp & 1) * 16 + (lane & 7), quarter = warp >> 1;
                 float part[4][2] = {};
-#pragma unroll 2
+#pragma unroll 1
                 for (int e = quarter * 4; e < a.kd; e += 16) {
                     const float4 k0v = load4(K + kg * ldk + e), k1v = load4(K + (kg + 8) * ldk + e);
 #pragma unroll
@@ -268,13 +265,7 @@ __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const
                     }
                 }
             }
-            if (stages == 2) {
-                stage ^= 1;
-            } else {
-                __syncthreads();
-                fetch(t + 1, 0);
-            }
-            if (stages == 2) __syncthreads();    // the stage that the next round fills has been read
+            __syncthreads();                     // the stage that the next round fills has been read
         }
         if constexpr (FEW) {                 // the warps' sums, over the stages (4 x 16 rows of values fit them for any sizes)
             if (VJ == 1) {
@@ -482,11 +473,10 @@ __global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs
 // ------------------------------------------------------------------------------------------------------ host side
 template <int TR, int VJ, bool FEW>
 static cudaError_t launch_simt(const TreeArgs& a, cudaStream_t q) {
-    const int stages = simt_smem(a.block, a.kd, a.vd, 2) <= 220 * 1024 ? 2 : 1;
-    const size_t smem = simt_smem(a.block, a.kd, a.vd, stages);
+    const size_t smem = simt_smem(a.block, a.kd, a.vd);
     const cudaError_t e = most_smem(k_ftree_simt<TR, VJ, FEW>);
     if (e != cudaSuccess) return e;
-    return launch_pdl_try(k_ftree_simt<TR, VJ, FEW>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a, stages);
+    return launch_pdl_try(k_ftree_simt<TR, VJ, FEW>, dim3(a.ctas), dim3(TS_THREADS), smem, q, 1, a);
 }
 template <int TR, bool FEW>
 static cudaError_t launch_simt_v(const TreeArgs& a, cudaStream_t q) {
@@ -521,7 +511,7 @@ static cudaError_t launch_merge(const TreeArgs& a, cudaStream_t q) {
                 : launch_pdl_try(k_ftree_merge<T, false, true>, grid, block, 0, q, 1, a, per, by_segment);
 }
 // CTAs of an SM: two where registers and shared memory allow it.
-static int simt_ctas(const TreeArgs& a) { return a.vd <= 128 && simt_smem(a.block, a.kd, a.vd, 2) <= 112 * 1024 ? 2 : 1; }
+static int simt_ctas(const TreeArgs& a) { return a.vd <= 128 && simt_smem(a.block, a.kd, a.vd) <= 112 * 1024 ? 2 : 1; }
 // Rows of a block, keys of a tile, tiles that a turn costs.  A tile takes about as long for its copies, waits and softmax as for the
 // products of 48 rows.
 static void simt_shape(int rows, int* block, int* tile, int* turn) {
