@@ -471,6 +471,7 @@ __global__ void __launch_bounds__(TM_WARPS * 32, 4) k_ftree_merge(const TreeArgs
 }
 
 // ------------------------------------------------------------------------------------------------------ host side
+constexpr float LOG2_E = 1.4426950408889634f;
 template <int TR, int VJ, bool FEW>
 static cudaError_t launch_simt(const TreeArgs& a, cudaStream_t q) {
     const size_t smem = simt_smem(a.block, a.kd, a.vd);
@@ -546,7 +547,7 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
               "bad sizes");
     DETB_TAKE(op->dim <= 256 && op->vdim <= 256, "the head is too large");
     DETB_TAKE(op->dtype == DET_F32 || op->dtype == DET_BF16, "unknown activation type");
-    DETB_TAKE(std::isfinite(op->scale) && op->scale > 0.0f, "bad scale");
+    DETB_TAKE(std::isfinite(op->scale * LOG2_E) && op->scale > 0.0f, "bad scale");
     DETB_TAKE(!op->vrope_cos == !op->vrope_sin && (!op->vrope_cos || (op->vdim % 2 == 0 && op->pos && op->rope_len > 0)), "bad rotation of the values");
     if (const char* why = bad_ref(op->seq)) return refuse(name, why);
     const long long rows = (long long)op->seq.max_nodes * (op->heads / op->kv_heads);
@@ -570,7 +571,7 @@ int det_f_tree_attn(const det_ftree_op* op, cudaStream_t st) {
     const long long blocks = (rows + a.block - 1) / a.block;
     DETB_TAKE(blocks * op->seq.seqs <= 65535, "too many rows");
     DETB_TAKE(runtime_ready(), "no usable device");
-    a.scale2 = op->scale * 1.4426950408889634f;
+    a.scale2 = op->scale * LOG2_E;
     a.cap = std::min(op->cap, TREE_MAX_KEYS); a.q = op->q; a.mask = op->mask; a.mask_ld = op->mask_ld; a.gate = op->gate; a.ldg = op->ldg; a.pos = op->pos;
     a.rope_len = op->rope_len; a.vcs = op->vrope_cos; a.vsn = op->vrope_sin; a.out = op->out; a.ldo = op->ldo;
     a.maps = op->scratch;

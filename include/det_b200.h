@@ -749,7 +749,7 @@ int det_f_qk_rope(const det_fqk_op* op, cudaStream_t st);
  * NULL: the nodes j <= i, that is, the rows are a run of tokens.  Query head h reads key/value head h / (heads / kv_heads); out[row][h * vdim + j] = sum softmax(scale * q . k) v, times sigmoid(gate[row * ldg + h])
  * (gate NULL: 1), in the activation type, row stride ldo.  A row that attends nothing gets zeros; what masked and missing rows hold,
  * NaN included, has no influence.  vrope_cos / vrope_sin: the values are rotated, and a head's output is turned back by pos[row]
- * (then needed; rope_len rows in the tables).  scale > 0.  dim, vdim <= 256; with a mask max_nodes <= DET_MAX_TREE.
+ * (then needed; rope_len rows in the tables).  scale > 0, scale * log2 e finite.  dim, vdim <= 256; with a mask max_nodes <= DET_MAX_TREE.
  * `scratch` (128-byte aligned, det_f_tree_scratch_bytes) holds descriptors of the caches and the pieces of rows whose keys several CTAs
  * share: calls that may overlap on the GPU need scratch of their own.  Results do not depend on the order of arrival.        */
 #define DET_MAX_TREE 1024
