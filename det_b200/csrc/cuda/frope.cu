@@ -122,8 +122,9 @@ __device__ __forceinline__ void put8(bf16* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf(v[0], v[1]), pack_bf(v[2], v[3]), pack_bf(v[4], v[5]), pack_bf(v[6], v[7]));
 }
 
-// One pass, bound by HBM: 8192 rows of 40 / 8 heads of 128 into bfloat16 take 70-73 us (357 MB, 5.0 TB/s); a single row 3.2 us, the
-// latency of place, row and tables one after the other.
+// One pass, bound by HBM: 8192 rows of 40 / 8 heads of 128 into bfloat16 take 70-73 us (357 MB, 5.0 TB/s), in fp32 85 us (474 MB, 5.6 TB/s);
+// a single row 3.2 us, the latency of place, row and tables one after the other.  Without VEC: heads of 124 137 us (2.5 TB/s, bound by loads
+// and table reads of four bytes), heads of 128 with 24 elements rotated in pairs 83 us.
 //
 // A warp takes a part of a row's heads, 32 / LPH at a time, eight neighbouring elements a lane; the row's place, its cosines and sines and
 // the norm's weights are fetched once.  VEC: heads are multiples of 8 elements, everything is 16-byte aligned and the halves of a

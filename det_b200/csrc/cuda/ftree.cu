@@ -65,8 +65,8 @@ __device__ __forceinline__ void copy_tile(float* dst, const float* src, size_t l
 // Thread (ty, tx) of 16 x 16 has rows ty + 16 i, keys tx + 16 j and value columns 4 tx + 64 j.  Two stages: the next tile's copies run
 // beside the products of this one; two CTAs on an SM cover one another's latencies.  Bound by the fp32 multiply-adds and their operands
 // from shared memory where keys are many (a key costs all rows of the block, 16 TR, whatever is in them: 16 nodes of 4 sequences behind 4096
-// keys, 40 / 8 heads of 128, 272 us), by start, deal and second launch where they are few (6 / 2 heads of 40 and 24, five trees of 13
-// nodes behind 2000 keys: 23.8 us; 27.7 with tiles of 64 keys and one CTA on an SM).
+// keys, 40 / 8 heads of 128, 255 us), by start, deal and second launch where they are few (6 / 2 heads of 40 and 24, five trees of 13
+// nodes behind 2000 keys: 22.7 us; when it was 23.8, tiles of 64 keys and one CTA on an SM took 27.7).
 template <int TR, int VJ, bool FEW>
 __global__ void __launch_bounds__(TS_THREADS, VJ < 4 ? 2 : 1) k_ftree_simt(const TreeArgs a) {
     extern __shared__ __align__(16) float tsm[];
@@ -484,8 +484,9 @@ static cudaError_t launch_simt_v(const TreeArgs& a, cudaStream_t q) {
     return a.vd <= 64 ? launch_simt<TR, 1, FEW>(a, q) : a.vd <= 128 ? launch_simt<TR, 2, FEW>(a, q) : launch_simt<TR, 4, FEW>(a, q);
 }
 // FEW saves reads of shared memory in every tile and adds the warps' sums in every stretch.  With larger values it is the faster one even at
-// two tiles a CTA (8 / 1 heads of 128, two nodes of three sequences behind 2274 keys: 19.8 us, 21.9 without), with smaller ones from a few
-// tiles on (8 / 8 heads of 64, 10 tiles: 40.6 / 45.1; 4 / 2 heads of 40 and 24, 2 tiles: 15.8 / 13.2).
+// two tiles a CTA (8 / 1 heads of 128, two nodes of three sequences behind 2274 keys: 19.8 us, 20.6 without; 21 / 3 heads of 96, a token of four
+// sequences behind 22854: 116 / 161), with smaller ones from a few tiles on (8 / 8 heads of 64, 10 tiles: 38.1 / 43.1, 2 tiles: 16.8 / 15.2;
+// 4 / 2 heads of 40 and 24, 2 tiles: 14.9 / 11.8).  Values of 24 would want it later still (7 tiles: 27.7 / 22.8).
 static bool simt_few(const TreeArgs& a) {
     return a.block == 16 && (a.vd > 64 || (long long)a.seq.seqs * a.kv_heads * a.blocks * (a.seq.max_len / TS_KEYS + 1) >= 6ll * a.ctas);
 }

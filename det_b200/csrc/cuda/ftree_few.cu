@@ -3,8 +3,10 @@
 // launch: a cluster of CTAs shares the keys of a (sequence, key/value head, block of 16 rows), each of its warps walks 16-key tiles
 // through a ring of its own, and the cluster adds its pieces over distributed shared memory.
 //
-// 40 / 8 heads of 128: a token behind 2048 keys 10.8 us (8.4 MB; latency: the table, the first tiles, a chain of 8 tiles a warp, the
-// cluster's sum), tokens of 32 sequences behind 4096 keys 101 us (537 MB, 5.3 TB/s).
+// 40 / 8 heads of 128: a token behind 2048 keys 10.5 - 11.4 us (8.4 MB; 129 tiles for the 64 warps of a cluster: a warp walks two or three),
+// behind 64 keys 9.0.  So it is the fixed part that it takes: the sequence's place and cache from device memory, the first tiles, one tile's
+// products and softmax, two barriers of the cluster and its sum, each waiting for the one before; nearly all of it is the kernel's own time
+// (10.0 and 12.5 us from a cold start under ncu).  Tokens of 32 sequences behind 4096 keys 101 us (537 MB, 5.3 TB/s).
 #include "flash.cuh"
 #include "ftree.cuh"
 #include <algorithm>

@@ -7,7 +7,9 @@
 //
 // Two slots per CTA take turns, so that the products of one run beside the exponentials of the other.  Up to 128 rows: both hold the
 // same rows and take every other tile of keys, and their results are added at the end; more rows: 128 rows each over the same tiles.
-// Heads above 128: one slot (TMEM and shared memory hold no more), tiles of 64 keys.
+// Heads above 128: one slot, tiles of 64 keys, and products and softmax take turns, which costs them (512 rows behind 4096, 16 / 2 heads of
+// 256: 75 us, 487 TFLOP/s).  It is not what TMEM and shared memory could hold: heads of 192 with values of 128 would have room for two
+// slots, heads of 256 for a second set of scores.
 //
 // Warps: four per slot for the softmax; one that loads tiles of K and V (TMA, 128-byte swizzle; K K-major, V as it lies in the cache,
 // MN-major); one that issues the products; two that bring the query rows (16-byte asynchronous copies, a head's rows are not evenly
@@ -22,13 +24,16 @@
 // key); sums and references are fp32.
 //
 // What bounds it (40 / 8 heads of 128).  Trees of 16 nodes read the cache once: 16 nodes behind 65536 keys 63 us (269 MB from HBM, what
-// they cannot do without), 32 sequences of 16 behind 4096 keys 104 us (5.2 TB/s).  A prompt of 2048 behind 6144 takes 306 us, 980
-// TFLOP/s: a tile of 128 rows x 128 keys is 1040 cycles of products (measured alone), beside the tiles' copies into the same shared
-// memory; then comes the chain from scores over a warp's exponentials (about 1600 cycles) to the weights, which two slots hide in part:
-// the pipe is busy 41 % of the time.  The products are issued by an elected lane: by a branch on the lane's number, operands went through
-// vector registers and the issue was the bound (358 us).  Measured and not taken: copies of the tiles by warps in place of TMA (prompt 532
-// us against 401), tiles of 64 keys with two score buffers (515 against 354), a product warp for each slot (405 against 354), TMEM loads
-// of 16 columns asked for ahead (369 against 354), a polynomial in place of an eighth to three eighths of the ex2 (312 to 331 against 306).
+// they cannot do without), 32 sequences of 16 behind 4096 keys 104 us (5.2 TB/s).  A prompt of 2048 behind 6144 takes 332 us with inputs
+// that change from call to call (905 TFLOP/s) and 300 to 306 with inputs that stay (984 to 1001), 20 of them the merge: a tile of 128 rows x
+// 128 keys is 1040 cycles of products (measured alone), beside the tiles' copies into the same shared memory; then comes the chain from scores
+// over a warp's exponentials (about 1600 cycles) to the weights, which two slots hide in part.  The pipe is busy 52 % of the attention
+// kernel's time there, 41 % with 512 rows, 40 % with a tree of 61 behind 32749 (80 to 84 us).  The softmax of a slot has 168 registers a
+// thread, with spills, and waits for each load of TMEM before it asks for the next.  The products are issued by an elected lane: by a branch
+// on the lane's number, operands went through vector registers and the issue was the bound (358 us).  Measured with inputs that stay, and not
+// taken: copies of the tiles by warps in place of TMA (prompt 532 us against 401), tiles of 64 keys with two score buffers (515 against 354), a
+// product warp for each slot (405 against 354), TMEM loads of 16 columns asked for ahead (369 against 354), a polynomial in place of an
+// eighth to three eighths of the ex2 (312 to 331 against 306).
 #include "ftree.cuh"
 #include "umma.cuh"
 #include <algorithm>
